@@ -330,6 +330,104 @@ TD_API int td_cls_backward(const td_rnn_config *cfg, const void *packT, const fl
                     const float *grad_prob, int32_t batch, int32_t seq_len, void *workspace, float *const *grad_layer,
                     float *grad_w, float *grad_b, void *stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Decay attention: linear attention with one decay per head, the recurrence whose training form is matrix products.
+ * No counterpart in the reference; it stands beside the recurrent layers above.  Per sequence and head, g = exp(log_decay):
+ *     S_t = g S_{t-1} + k_t v_t^T,     o_t = scale * S_t^T q_t,     t = 1 .. length, S_0 = `state_in` (NULL: zeros)
+ * Sequences are dense, tensors (n_seq, rows, heads, d), or packed, tensors (rows, heads, d) with `offsets` (n_seq + 1 device
+ * int32, non-decreasing): sequence i is the rows offsets[i] .. offsets[i + 1] - 1.  Lengths are read on the device (a captured
+ * graph may be replayed with other offsets); rows of no sequence come back as zeros, offsets outside 0 .. rows are clamped.
+ * q, k and v may have fewer heads than log_decay (q_heads, k_heads, v_heads divide heads; head h reads head
+ * h / (heads / q_heads), ...): their gradients are the sums over the heads that share them.
+ * Types: q, k, v, o and their gradients TD_F32 or TD_BF16 (dtype); log_decay, states and their gradients float32.  The
+ * recurrence is computed in float32: bf16 matrix products whose rounded operands are carried as two or three bf16 terms.
+ * Limits: dk, dv <= TD_DECAY_MAX_DIM.  log_decay is meant to be <= 0 (-inf: no memory); a positive one grows as the formula says.
+ * ------------------------------------------------------------------------------------------ */
+enum { TD_F32 = 0, TD_BF16 = 1 };
+#define TD_DECAY_MAX_DIM 128
+
+typedef struct td_decay_config {
+    int32_t n_seq;     /* sequences                                                             */
+    int32_t rows;      /* rows of each sequence (dense) or of the packed tensors                */
+    int32_t packed;    /* 1: `offsets` says where sequences begin                               */
+    int32_t heads;     /* of log_decay, o and the states                                        */
+    int32_t q_heads, k_heads, v_heads;
+    int32_t dk, dv;
+    int32_t dtype;     /* TD_F32 or TD_BF16                                                     */
+    float scale;
+    int32_t reserved;
+    int64_t q_stride[3], k_stride[3], v_stride[3], grad_o_stride[3]; /* elements between sequences (dense), rows, heads; the last
+                                                                        dimension of every tensor is contiguous */
+} td_decay_config;
+
+/* Scratch of one forward (backward = 0) or backward (1) call; 0 with td_last_error() set for a bad configuration. */
+TD_API size_t td_decay_workspace_bytes(const td_decay_config *cfg, int32_t backward);
+/* o: (.., rows, heads, dv) contiguous; state_in, state_out: (n_seq, heads, dk, dv) float32 or NULL (not the same memory). */
+TD_API int td_decay_forward(const td_decay_config *cfg, const void *q, const void *k, const void *v, const float *log_decay,
+                     const int32_t *offsets, const float *state_in, void *o, float *state_out, void *workspace, void *stream);
+/* Gradients of sum(o * grad_o) + sum(state_out * grad_state_out); grad_state_out may be NULL, and so may every output that is
+ * not wanted.  grad_q, grad_k, grad_v: contiguous, of their tensor's shape and type; grad_log_decay (heads) and grad_state_in
+ * float32.  All outputs are overwritten; no float atomics, the same inputs give the same bits. */
+TD_API int td_decay_backward(const td_decay_config *cfg, const void *q, const void *k, const void *v, const float *log_decay,
+                      const int32_t *offsets, const float *state_in, const void *grad_o, const float *grad_state_out, void *grad_q,
+                      void *grad_k, void *grad_v, float *grad_log_decay, float *grad_state_in, void *workspace, void *stream);
+/* One row for each of n_seq sequences (cfg: rows = 1, packed = 0; tensors (n_seq, heads, d), row strides unused): `state`
+ * (n_seq, heads, dk, dv) float32 is updated in place, o (n_seq, heads, dv) written. */
+TD_API int td_decay_step(const td_decay_config *cfg, const void *q, const void *k, const void *v, const float *log_decay, float *state,
+                  void *o, void *stream);
+
+/* ------------------------------------------------------------------------------------------
+ * AdamW over a list of tensors at once (Adam with decoupled weight decay; no counterpart in the reference, whose classifier
+ * uses torch.optim.AdamW, evaluate/nn_classifier.py:150).  For each value, g' = grad * grad_scale[0] (1 if NULL):
+ *     m = beta1 m + (1 - beta1) g',   v = beta2 v + (1 - beta2) g'^2,
+ *     param = param (1 - lr weight_decay) - lr / (1 - beta1^step) * m / (sqrt(v) / sqrt(1 - beta2^step) + eps)
+ * state_bits 32: exp_avg = m and exp_avg_sq = v, float32.  state_bits 8: exp_avg holds m and exp_avg_sq holds sqrt(v) as e4m3
+ * bytes, times a float32 scale for each block of TD_ADAMW_BLOCK values (scales[2 b] and scales[2 b + 1]: the block's largest
+ * magnitude / 448; a block whose largest is below 2^-100 is stored as zeros).  A value between two e4m3 neighbours goes up with
+ * the probability of its distance (an average with beta2 = 0.999 moves sqrt(v) by 0.05 % a step and neighbours are 6 to 12 %
+ * apart: rounding to the nearest would hold it still for good); a second moment above zero never becomes zero.  `random`: n words
+ * whose low 16 bits round m and whose high 16 bits round sqrt(v), u = (bits + 0.5) / 65536; NULL: Philox4x32-10 words of (seed,
+ * position in the list, index, step).  The update itself uses the unrounded m and v.
+ * ------------------------------------------------------------------------------------------ */
+#define TD_ADAMW_BLOCK 256
+
+typedef struct td_adamw_tensor {
+    float *param;
+    const void *grad;
+    void *exp_avg, *exp_avg_sq;
+    float *scales;         /* state_bits 8: 2 * ceil(n / TD_ADAMW_BLOCK) floats        */
+    const int32_t *random; /* state_bits 8: n words, or NULL                           */
+    int64_t n;             /* values; 0 is skipped                                     */
+    int32_t grad_dtype;    /* TD_F32 or TD_BF16                                        */
+    int32_t reserved;
+} td_adamw_tensor;
+
+/* What changes from one step to the next, in device memory, for steps captured in a graph (as td_step_record). */
+typedef struct td_adamw_record {
+    uint64_t seed;
+    int64_t step;
+    float step_size;      /* lr / (1 - beta1^step)     */
+    float inv_sqrt_bc2;   /* 1 / sqrt(1 - beta2^step)  */
+    float decay;          /* 1 - lr * weight_decay     */
+    float reserved;
+} td_adamw_record;
+
+typedef struct td_adamw_config {
+    double lr, beta1, beta2, eps, weight_decay;
+    int64_t step;              /* from 1                                                                   */
+    uint64_t seed;
+    const float *grad_scale;   /* device scalar or NULL                                                    */
+    const td_adamw_record *record; /* device, or NULL; read when the kernel runs instead of lr, weight_decay, step and seed */
+    int32_t state_bits;        /* 32 or 8                                                                  */
+    int32_t reserved;
+} td_adamw_config;
+
+/* `tensors_host`: `count` records in host memory, read during the call.  One launch for every 48 tensors. */
+TD_API int td_adamw(const td_adamw_config *cfg, const td_adamw_tensor *tensors_host, int32_t count, void *stream);
+/* The record of (lr, betas, weight_decay, step, seed) of cfg, computed as td_adamw computes its own values and written by a
+ * one-thread kernel (stream-ordered). */
+TD_API int td_adamw_record_set(td_adamw_record *record_dev, const td_adamw_config *cfg, void *stream);
+
 /* Kernel-selection knobs for tests and measurements, no counterpart in the reference (process-wide, not
  * thread-safe against concurrent launches).
  *   td_set_layer_kernel: which recurrent-layer kernel family runs hidden sizes <= 256.  AUTO picks by batch

@@ -1,0 +1,89 @@
+"""Decay attention without a GPU: what the entry points refuse, and the 64-bit reference against the recurrence it stands for."""
+import ctypes as C
+
+import pytest
+import torch
+
+import decay_reference as ref
+from timediff_amd import _lib
+from timediff_amd.decay_attention import decay_attention, decay_attention_step
+
+
+def _x(*shape, dtype=torch.float32):
+    return torch.zeros(*shape, dtype=dtype)
+
+
+def _call(**kw):
+    a = dict(q=_x(2, 5, 2, 8), k=_x(2, 5, 2, 8), v=_x(2, 5, 4, 6), log_decay=_x(4))
+    a.update(kw)
+    return decay_attention(a.pop("q"), a.pop("k"), a.pop("v"), a.pop("log_decay"), **a)
+
+
+@pytest.mark.parametrize("bad, error, text", [
+    (dict(q=_x(2, 5, 8)), ValueError, "q must have 4 dimensions"),
+    (dict(k=_x(2, 5, 2, 8, dtype=torch.bfloat16)), TypeError, "float32 or all bfloat16"),
+    (dict(q=_x(2, 5, 2, 8, dtype=torch.float16)), TypeError, "float32 or all bfloat16"),
+    (dict(v=_x(2, 4, 4, 6)), ValueError, "leading dimensions"),
+    (dict(k=_x(2, 5, 2, 7)), ValueError, "q and k must agree"),
+    (dict(q=_x(2, 5, 3, 8)), ValueError, "heads of q"),
+    (dict(log_decay=_x(4, dtype=torch.float64)), ValueError, "log_decay must be a float32 vector"),
+    (dict(log_decay=_x(0)), ValueError, "heads of q"),
+    (dict(v=_x(2, 5, 4, 129)), ValueError, "must be 1 .. 128"),
+    (dict(v=_x(2, 5, 4, 0)), ValueError, "must be 1 .. 128"),
+    (dict(initial_state=_x(2, 4, 8, 7)), ValueError, "the state must be float32 of shape"),
+    (dict(initial_state=_x(2, 4, 8, 6, dtype=torch.bfloat16)), ValueError, "the state must be float32 of shape"),
+    (dict(offsets=torch.tensor([0, 5], dtype=torch.int32)), ValueError, "q must have 3 dimensions"),
+    (dict(q=_x(5, 2, 8), k=_x(5, 2, 8), v=_x(5, 4, 6), offsets=torch.tensor([0, 5])), ValueError, "offsets must be an int32 vector"),
+    (dict(q=_x(5, 2, 8), k=_x(5, 2, 8), v=_x(5, 4, 6), offsets=torch.tensor([0], dtype=torch.int32)), ValueError, "at least 2 entries"),
+    (dict(), ValueError, "one ROCm device"),
+])
+def test_refusals(bad, error, text):
+    with pytest.raises(error, match=text):
+        _call(**bad)
+
+
+def test_step_refusals():
+    a = dict(q=_x(2, 2, 8), k=_x(2, 2, 8), v=_x(2, 4, 6), log_decay=_x(4), state=_x(2, 4, 8, 6))
+    for bad, error, text in [(dict(q=_x(2, 1, 2, 8)), ValueError, "q must have 3 dimensions"), (dict(state=_x(2, 4, 6, 8)), ValueError, "of shape"),
+                             (dict(v=_x(3, 4, 6)), ValueError, "leading dimensions"), (dict(), ValueError, "one ROCm device"),
+                             (dict(q=_x(2, 2, 8).requires_grad_()), RuntimeError, "no gradient")]:
+        with pytest.raises(error, match=text):
+            decay_attention_step(**dict(a, **bad))
+
+
+@pytest.mark.parametrize("field, value, text", [
+    ("n_seq", 0, b"n_seq"), ("rows", -1, b"rows"), ("packed", 2, b"packed"), ("dtype", 2, b"dtype"), ("dk", 129, b"dk and dv"), ("dv", 0, b"dk and dv"),
+    ("q_heads", 3, b"must divide heads"), ("k_heads", 0, b"must divide heads"), ("heads", 0, b"must divide heads")])
+def test_library_refuses_bad_configurations(field, value, text):
+    L = _lib.lib()
+    cfg = _lib.DecayConfig(n_seq=2, rows=5, heads=4, q_heads=2, k_heads=2, v_heads=4, dk=8, dv=6, dtype=_lib.F32, scale=1.0)
+    assert L.td_decay_workspace_bytes(C.byref(cfg), 0) > 0 and L.td_decay_workspace_bytes(C.byref(cfg), 1) > 0
+    setattr(cfg, field, value)
+    assert L.td_decay_workspace_bytes(C.byref(cfg), 1) == 0 and text in L.td_last_error()
+    assert L.td_decay_forward(C.byref(cfg), *[None] * 10) == 1 and text in L.td_last_error()
+    assert L.td_decay_backward(C.byref(cfg), *[None] * 15) == 1
+    assert L.td_decay_step(C.byref(cfg), *[None] * 7) == 1
+
+
+def test_library_refuses_null_pointers_and_wrong_forms():
+    L = _lib.lib()
+    cfg = _lib.DecayConfig(n_seq=2, rows=5, heads=4, q_heads=2, k_heads=2, v_heads=4, dk=8, dv=6, dtype=_lib.F32, scale=1.0)
+    some = C.c_void_p(256)            # never dereferenced: the calls below return before any launch
+    assert L.td_decay_forward(C.byref(cfg), *[None] * 10) == 1 and b"null pointer" in L.td_last_error()
+    assert L.td_decay_forward(C.byref(cfg), some, some, some, some, None, some, some, some, some, None) == 1 and b"same memory" in L.td_last_error()
+    assert L.td_decay_backward(C.byref(cfg), *[None] * 15) == 1 and b"null pointer" in L.td_last_error()
+    assert L.td_decay_step(C.byref(cfg), some, some, some, some, some, some, None) == 1 and b"one row" in L.td_last_error()
+    cfg.packed = 1
+    assert L.td_decay_forward(C.byref(cfg), some, some, some, some, None, None, some, None, some, None) == 1 and b"offsets" in L.td_last_error()
+
+
+def test_reference_is_the_recurrence():
+    g = torch.Generator().manual_seed(3)
+    q, k, v, s0 = (torch.randn(*s, generator=g, dtype=torch.float64) for s in ((9, 5), (9, 5), (9, 4), (5, 4)))
+    ld = torch.tensor(-0.3, dtype=torch.float64)
+    o, s = ref.sequence(q, k, v, ld, 0.7, s0)
+    S = s0
+    for t in range(9):
+        S = torch.exp(ld) * S + k[t][:, None] * v[t][None, :]
+        assert torch.allclose(o[t], 0.7 * q[t] @ S, rtol=1e-12, atol=1e-12)
+    assert torch.allclose(s, S, rtol=1e-12, atol=1e-12)

@@ -23,6 +23,8 @@ MISC_KEYS = ["time_emb.1.weight", "time_emb.1.bias", "time_emb.3.weight", "time_
 LAYER_KERNEL_AUTO, LAYER_KERNEL_BATCH, LAYER_KERNEL_UNITS, LAYER_KERNEL_CLUSTER = 0, 1, 2, 3     # td_set_layer_kernel
 PROFILE_LAYER_INFER, PROFILE_LAYER_SAVE, PROFILE_BPTT_SWEEP = 1, 2, 4     # td_profile_enable
 HEAD_FUSION_AUTO, HEAD_FUSION_OFF, HEAD_FUSION_ON = 0, 1, 2             # td_set_head_fusion
+F32, BF16 = 0, 1                                                         # element types (td_decay_config.dtype, td_adamw_tensor.grad_dtype)
+DECAY_MAX_DIM, ADAMW_BLOCK = 128, 256
 STEP_LAUNCH_AUTO, STEP_LAUNCH_OFF, STEP_LAUNCH_ON = 0, 1, 2             # td_set_step_launch
 
 
@@ -45,6 +47,30 @@ class StepRecord(C.Structure):
     """td_step_record: what changes from one optimizer step to the next (read on the device by a captured training step)."""
     _fields_ = [("seed", C.c_uint64), ("step_size", C.c_float), ("inv_sqrt_bc2", C.c_float), ("ema_decay", C.c_float),
                 ("ema_mode", C.c_int32), ("reserved", C.c_uint64)]
+
+
+class DecayConfig(C.Structure):
+    """td_decay_config: shape, types and strides of a decay-attention call."""
+    _fields_ = [(n, C.c_int32) for n in ("n_seq", "rows", "packed", "heads", "q_heads", "k_heads", "v_heads", "dk", "dv", "dtype")] + [
+        ("scale", C.c_float), ("reserved", C.c_int32), ("q_stride", C.c_int64 * 3), ("k_stride", C.c_int64 * 3),
+        ("v_stride", C.c_int64 * 3), ("grad_o_stride", C.c_int64 * 3)]
+
+
+class AdamwTensor(C.Structure):
+    _fields_ = [("param", C.c_void_p), ("grad", C.c_void_p), ("exp_avg", C.c_void_p), ("exp_avg_sq", C.c_void_p),
+                ("scales", C.c_void_p), ("random", C.c_void_p), ("n", C.c_int64), ("grad_dtype", C.c_int32), ("reserved", C.c_int32)]
+
+
+class AdamwRecord(C.Structure):
+    """td_adamw_record: what changes from one AdamW step to the next (read on the device by a captured step)."""
+    _fields_ = [("seed", C.c_uint64), ("step", C.c_int64), ("step_size", C.c_float), ("inv_sqrt_bc2", C.c_float), ("decay", C.c_float),
+                ("reserved", C.c_float)]
+
+
+class AdamwConfig(C.Structure):
+    _fields_ = [(n, C.c_double) for n in ("lr", "beta1", "beta2", "eps", "weight_decay")] + [
+        ("step", C.c_int64), ("seed", C.c_uint64), ("grad_scale", C.c_void_p), ("record", C.c_void_p), ("state_bits", C.c_int32),
+        ("reserved", C.c_int32)]
 
 
 class TimediffError(RuntimeError):
@@ -106,6 +132,12 @@ _SIGS = {
     "td_cls_workspace_bytes": (C.c_size_t, [C.POINTER(RnnConfig), _I, _I]),
     "td_cls_forward": (C.c_int, [C.POINTER(RnnConfig), _P, _P, _P, _P, _I, _I, _P, _P, _P]),
     "td_cls_backward": (C.c_int, [C.POINTER(RnnConfig), _P, _P, _P, _P, _P, _I, _I, _P, C.POINTER(_P), _P, _P, _P]),
+    "td_decay_workspace_bytes": (C.c_size_t, [C.POINTER(DecayConfig), _I]),
+    "td_decay_forward": (C.c_int, [C.POINTER(DecayConfig)] + [_P] * 10),
+    "td_decay_backward": (C.c_int, [C.POINTER(DecayConfig)] + [_P] * 15),
+    "td_decay_step": (C.c_int, [C.POINTER(DecayConfig)] + [_P] * 7),
+    "td_adamw": (C.c_int, [C.POINTER(AdamwConfig), C.POINTER(AdamwTensor), _I, _P]),
+    "td_adamw_record_set": (C.c_int, [_P, C.POINTER(AdamwConfig), _P]),
     "td_set_head_fusion": (C.c_int, [_I]),
     "td_set_side_gemm": (C.c_int, [_I]),
     "td_set_step_launch": (C.c_int, [_I]),

@@ -1,7 +1,7 @@
 """The TSTR (train-on-synthetic, test-on-real) RNN classifier with the reference's interface
 (evaluate/nn_classifier.py:89-171: `RNN`, `nnTimeSeriesClassifier`, `normalize_data`, `standardize_data`), on the
 recurrent kernels of the denoiser: forward with saves, BPTT and weight gradients are td_cls_forward / td_cls_backward
-(csrc/rnn_train.hip); the update is AdamW on one flat fp32 buffer (decoupled decay + td_clip_adam_ema).
+(csrc/rnn_train.hip); the update is AdamW on one flat fp32 buffer (td_adamw).
 
 Same constructor signatures, `forward(X)` with X (B, C, L) -> P(y = 1) of shape (B,), `train()`, `predict_proba(X)`,
 and the same state_dict keys (`lstm.*` / `gru.*`, `final.0.*`), so weights move between the two implementations.  The
@@ -15,6 +15,7 @@ import torch.nn as nn
 
 from . import _lib
 from ._lib import check, lib, ptr
+from .optim import adamw_
 
 
 def _stream():
@@ -184,10 +185,10 @@ class nnTimeSeriesClassifier:
         self.flat_grad.zero_()
         self.model._backward_kernels(prob, y=y.contiguous(), sink=self.grads)
         self.step += 1
-        self.flat.mul_(1.0 - self.lr * self.weight_decay)            # AdamW's decoupled decay
-        check(lib().td_clip_adam_ema(ptr(self.flat), ptr(self.flat_grad), ptr(self.exp_avg), ptr(self.exp_avg_sq), None,
-                                     self.flat.numel(), None, 0.0, self.lr, self.betas[0], self.betas[1], self.eps, self.step, 0,
-                                     0.0, _stream()))
+        # lr and betas in float32, as td_clip_adam_ema takes them: the weights of a run stay what they were
+        f = np.float32
+        adamw_([self.flat], [self.flat_grad], [self.exp_avg], [self.exp_avg_sq], lr=float(f(self.lr)),
+               betas=(float(f(self.betas[0])), float(f(self.betas[1]))), eps=self.eps, weight_decay=self.weight_decay, step=self.step)
         self.last_prob, self.last_y = prob, y
 
     def train(self):

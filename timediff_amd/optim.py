@@ -1,0 +1,170 @@
+"""AdamW over many tensors at once, its moments in 32 or in 8 bits (td_adamw), beside the trainers' flat td_clip_adam_ema.
+
+`adamw_` steps lists of tensors that the caller owns; `AdamW` is a torch.optim.Optimizer around it.  With 8-bit moments a value
+costs 2 bytes of state instead of 8: exp_avg holds m and exp_avg_sq holds sqrt(v) as float8_e4m3fn, times one float32 scale
+for each 256 values (a moment's value is code.float() * scale), rounded stochastically.  No counterpart in the reference.
+"""
+import ctypes as C
+
+import torch
+
+from . import _lib, ops
+from ._lib import ADAMW_BLOCK, AdamwConfig, AdamwRecord, check, lib, ptr
+
+
+def _check_list(name, tensors, like, dtypes):
+    if len(tensors) != len(like):
+        raise ValueError(f"{len(tensors)} {name} for {len(like)} params")
+    kinds = {t.dtype for t in tensors}
+    if not kinds <= dtypes:
+        raise TypeError(f"{name} must be {' or '.join(sorted(str(d) for d in dtypes))}, got {', '.join(sorted(str(d) for d in kinds - dtypes))}")
+    if not all(map(torch.Tensor.is_contiguous, tensors)):
+        raise ValueError(f"{name} must be contiguous")
+
+
+def adamw_(params, grads, exp_avgs, exp_avg_sqs, scales=None, *, lr, betas, eps, weight_decay, step, grad_scale=None, random=None,
+           seed=0, record=None):
+    """One AdamW step in place over lists of tensors (one launch for every 48): params float32, grads float32 or bfloat16, all
+    contiguous and on one device.
+    Moments in 32 bits: exp_avgs (m) and exp_avg_sqs (v) float32.  In 8 bits, where `scales` is given: exp_avgs (m) and exp_avg_sqs
+    (sqrt(v)) float8_e4m3fn, scales float32 (ceil(n / 256), 2); all zeros is the state before the first step.
+    random: for 8-bit moments, int32 tensors of the params' sizes whose low and high 16 bits round m and sqrt(v); by default the
+    library draws them from (seed, position in the list, index, step).  step counts from 1.  grad_scale: a float32 device scalar that
+    multiplies every gradient.  record: a device td_adamw_record (AdamW's capturable mode) read instead of lr, weight_decay, step
+    and seed.  A gradient that is not finite makes its values (8 bits: the moments of its block of 256) not finite."""
+    if not params:
+        return
+    bits = 32 if scales is None else 8
+    state = {torch.float32} if bits == 32 else {torch.float8_e4m3fn}
+    lists = [("params", params, {torch.float32}), ("grads", grads, {torch.float32, torch.bfloat16}), ("exp_avgs", exp_avgs, state),
+             ("exp_avg_sqs", exp_avg_sqs, state)]
+    n = list(map(torch.Tensor.numel, params))
+    if bits == 8:
+        lists.append(("scales", scales, {torch.float32}))
+        if list(map(torch.Tensor.numel, scales)) != [2 * -(-k // ADAMW_BLOCK) for k in n]:
+            raise ValueError(f"scales must have 2 values for each {ADAMW_BLOCK} of their param")
+        if random is not None:
+            lists.append(("random", random, {torch.int32}))
+    elif random is not None:
+        raise ValueError("random is for 8-bit moments")
+    for name, tensors, dtypes in lists:
+        _check_list(name, tensors, params, dtypes)
+        if name not in ("params", "scales") and list(map(torch.Tensor.numel, tensors)) != n:
+            raise ValueError(f"{name} must have their params' sizes")
+    for name, tensors, _ in lists:
+        if set(map(torch.Tensor.get_device, tensors)) != {params[0].get_device()} or not params[0].is_cuda:
+            raise ValueError(f"{name} must be on one ROCm device, the params'")
+    if grad_scale is not None and (grad_scale.dtype != torch.float32 or grad_scale.numel() != 1 or grad_scale.device != params[0].device):
+        raise ValueError("grad_scale must be one float32 value on the params' device")
+    _launch(lists, n, AdamwConfig(lr=lr, beta1=betas[0], beta2=betas[1], eps=eps, weight_decay=weight_decay, step=step, seed=seed,
+                                  grad_scale=None if grad_scale is None else grad_scale.data_ptr(),
+                                  record=None if record is None else record.data_ptr(), state_bits=bits))
+
+
+def _launch(lists, n, cfg):
+    """lists: params, grads, exp_avgs, exp_avg_sqs[, scales[, random]] as (name, tensors, ..)."""
+    count = len(n)
+    table = (C.c_uint64 * (8 * count))()         # td_adamw_tensor is eight 64-bit words
+    for word, (_, tensors, *_rest) in enumerate(lists):
+        table[word::8] = list(map(torch.Tensor.data_ptr, tensors))
+    table[6::8] = n
+    table[7::8] = [_lib.F32 if g.dtype is torch.float32 else _lib.BF16 for g in lists[1][1]]
+    with torch.cuda.device(lists[0][1][0].device):
+        check(lib().td_adamw(C.byref(cfg), C.cast(table, C.POINTER(_lib.AdamwTensor)), count, ops._stream()))
+
+
+class AdamW(torch.optim.Optimizer):
+    """torch.optim.AdamW's formula and arguments on td_adamw; params float32, grads float32 or bfloat16.
+    state_bits: 32 or 8 (state: exp_avg, exp_avg_sq[, scales], step).  seed: of the 8-bit moments' stochastic rounding.
+    capturable: step() may be captured in a graph.  A captured step() reads step count, learning rate, weight decay and seed from
+    device records; call advance() before each replay (an eager step() calls it itself)."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, state_bits=32, seed=0, capturable=False):
+        if state_bits not in (32, 8):
+            raise ValueError(f"state_bits must be 32 or 8, got {state_bits}")
+        if not (lr >= 0 and eps >= 0 and weight_decay >= 0 and 0 <= betas[0] < 1 and 0 <= betas[1] < 1):
+            raise ValueError(f"bad lr {lr}, betas {betas}, eps {eps} or weight_decay {weight_decay}")
+        self.state_bits, self.seed, self.capturable = state_bits, int(seed), bool(capturable)
+        self._records = {}
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+
+    def add_param_group(self, group):
+        super().add_param_group(group)
+        for p in self.param_groups[-1]["params"]:
+            if p.dtype != torch.float32 or not p.is_contiguous():
+                self.param_groups.pop()
+                raise ValueError(f"params must be contiguous float32, got {p.dtype} of strides {tuple(p.stride())}")
+
+    def _state(self, p):
+        s = self.state[p]
+        if not s:
+            kind = torch.float32 if self.state_bits == 32 else torch.float8_e4m3fn
+            s["step"] = 0
+            s["exp_avg"], s["exp_avg_sq"] = (torch.zeros(p.shape, dtype=torch.float32, device=p.device).to(kind) for _ in range(2))
+            if self.state_bits == 8:
+                s["scales"] = torch.zeros(-(-p.numel() // ADAMW_BLOCK), 2, dtype=torch.float32, device=p.device)
+        return s
+
+    def _config(self, i, step):
+        g = self.param_groups[i]
+        # each group rounds from a stream of its own
+        return AdamwConfig(lr=float(g["lr"]), beta1=g["betas"][0], beta2=g["betas"][1], eps=g["eps"], weight_decay=g["weight_decay"], step=step,
+                           seed=(self.seed + (i << 32)) & (2 ** 64 - 1), state_bits=self.state_bits)
+
+    def advance(self):
+        """capturable: counts one step and writes what changes with it (step count, lr, weight decay, seed) to the device records
+        that a captured step() reads."""
+        if not self.capturable:
+            raise RuntimeError("advance() belongs to AdamW(capturable=True)")
+        for i, g in enumerate(self.param_groups):
+            if not g["params"]:
+                continue
+            if i not in self._records:
+                self._records[i] = torch.zeros(C.sizeof(AdamwRecord), dtype=torch.uint8, device=g["params"][0].device)
+            states = [self._state(p) for p in g["params"]]
+            if len({s["step"] for s in states}) != 1:
+                raise RuntimeError("capturable: the params of a group must be at the same step")
+            for s in states:
+                s["step"] += 1
+            rec = self._records[i]
+            with torch.cuda.device(rec.device):
+                check(lib().td_adamw_record_set(ptr(rec), C.byref(self._config(i, states[0]["step"])), ops._stream()))
+
+    @torch.no_grad()
+    def step(self, closure=None, *, grad_scale=None):
+        """grad_scale: a float32 device scalar that multiplies every gradient (a clipping coefficient, an inverse loss scale)."""
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        capturing = torch.cuda.is_current_stream_capturing()
+        if capturing and (not self.capturable or not self._records):
+            raise RuntimeError("step() under graph capture needs AdamW(capturable=True) and one step() or advance() before the capture")
+        if self.capturable and not capturing:
+            self.advance()
+        for i, group in enumerate(self.param_groups):
+            live = [p for p in group["params"] if p.grad is not None]
+            for p in live:
+                if p.grad.is_sparse:
+                    raise RuntimeError("sparse gradients are not supported")
+            if not self.capturable:
+                for p in live:
+                    self._state(p)["step"] += 1
+            for step in sorted({self.state[p]["step"] for p in live}):
+                ps = [p for p in live if self.state[p]["step"] == step]
+                st = [self.state[p] for p in ps]
+                cfg = self._config(i, step)
+                adamw_(ps, [p.grad.contiguous() for p in ps], [s["exp_avg"] for s in st], [s["exp_avg_sq"] for s in st],
+                       [s["scales"] for s in st] if self.state_bits == 8 else None, lr=cfg.lr, betas=(cfg.beta1, cfg.beta2), eps=cfg.eps,
+                       weight_decay=cfg.weight_decay, step=step, grad_scale=grad_scale, seed=cfg.seed,
+                       record=self._records.get(i))
+        return loss
+
+    def load_state_dict(self, state_dict):
+        for s in state_dict["state"].values():
+            if ("scales" in s) != (self.state_bits == 8):
+                raise ValueError(f"the state was saved with {8 if 'scales' in s else 32}-bit moments, this optimizer has state_bits={self.state_bits}")
+        super().load_state_dict(state_dict)
+        if self.state_bits == 8:          # torch casts a state to its param's type: float32 holds every e4m3 value, so the way back is exact
+            for s in self.state.values():
+                s["exp_avg"], s["exp_avg_sq"] = s["exp_avg"].to(torch.float8_e4m3fn), s["exp_avg_sq"].to(torch.float8_e4m3fn)
