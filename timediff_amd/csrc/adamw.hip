@@ -31,6 +31,19 @@ __device__ __forceinline__ float decayed(float p, float decay) {
     return p * decay;
 }
 
+// The moments.  With 8-bit moments every operation is rounded on its own (no fused multiply-add): which neighbour a value goes to
+// then follows from the formula in float32 alone, whoever computes it.
+template <int BITS> __device__ __forceinline__ void moments(float &m, float &v, float g, float beta1, float beta2, float omb1, float omb2) {
+    if (BITS == 8) {
+#pragma clang fp contract(off)
+        m = beta1 * m + omb1 * g;
+        v = beta2 * v + omb2 * g * g;
+    } else {
+        m = beta1 * m + omb1 * g;
+        v = beta2 * v + omb2 * g * g;
+    }
+}
+
 // one of the two e4m3 neighbours of y in [0, 448]: t = y / (its binade's step) in [8, 16) (below 2^-6: [0, 8)), up where
 // the fraction plus u in (0, 1) passes one
 __device__ __forceinline__ uint32_t e4m3_round(float y, uint32_t bits16) {
@@ -114,8 +127,7 @@ __device__ __forceinline__ void step_block(const Batch &B, const Scalars &s, con
     float root[4];
     for (int j = 0; j < 4; ++j) {
         g[j] = g[j] * gs;
-        m[j] = B.beta1 * m[j] + B.omb1 * g[j];
-        v[j] = B.beta2 * v[j] + B.omb2 * g[j] * g[j];
+        moments<BITS>(m[j], v[j], g[j], B.beta1, B.beta2, B.omb1, B.omb2);
         root[j] = sqrtf(v[j]);
         p[j] = decayed(p[j], s.decay) - s.step_size * m[j] / (root[j] * s.inv_sqrt_bc2 + B.eps);
     }
@@ -171,7 +183,7 @@ __device__ __forceinline__ void step_block(const Batch &B, const Scalars &s, con
     top_m = wave_top(top_m);
     top_v = wave_top(top_v);
     const bool some_m = !(top_m < 0x1p-100f), some_v = !(top_v < 0x1p-100f);
-    const float im = some_m ? 448.0f / top_m : 0.0f, iv = some_v ? 448.0f / top_v : 0.0f;
+    const float im = some_m ? 448.0f * (1.0f / top_m) : 0.0f, iv = some_v ? 448.0f * (1.0f / top_v) : 0.0f;
     mb = vb = 0;
     for (int j = 0; j < 4; ++j) {
         float ym = fabsf(m[j]) * im, yv = root[j] * iv;
@@ -194,8 +206,8 @@ __device__ __forceinline__ void step_block(const Batch &B, const Scalars &s, con
             }
     }
     if (lane == 0) {
-        t.scales[2 * block] = some_m ? top_m / 448.0f : 0.0f;
-        t.scales[2 * block + 1] = some_v ? top_v / 448.0f : 0.0f;
+        t.scales[2 * block] = some_m ? top_m * (1.0f / 448.0f) : 0.0f;
+        t.scales[2 * block + 1] = some_v ? top_v * (1.0f / 448.0f) : 0.0f;
     }
 }
 
