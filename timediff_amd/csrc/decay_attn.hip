@@ -7,127 +7,34 @@
 // the state BEHIND a row: it enters a row undecayed and decays when it leaves it.
 // The decay's gradient is sum_t <grad_o_t, d o_t / d log g>, and d M_t / d log g = g (M'_{t-1} + M_{t-1}) is carried beside M in the
 // pass that computes grad_q: a sum without cancellation, where sum_t t (q.grad_q - k.grad_k) would lose everything for fast decays.
-#include "common.h"
+#include "decay_chunk.h"
+
+using namespace decay;
 
 namespace {
 
-struct View {                 // rows of one tensor; head h of the recurrence reads head h / share
-    const void *p;
-    int64_t seq, row, head;
-    int share;
-};
+template <typename T> __device__ __forceinline__ float as_float(T x) { return (float)x; }
 
-struct Pass {
-    View a, b, c, e;          // e: what the tangent's output is dotted with (tangent form only)
-    const float *log_decay;
-    const int32_t *offsets;   // packed: n_seq + 1, else NULL
-    const float *state_in;    // (n_seq, heads, ..): element (i, j) of (da, dc) at i * st_a + j * st_c, NULL: zeros
-    float *state_out;         // NULL: not wanted
-    const float *grad_state;  // tangent form: the gradient of the state left behind, NULL: none
-    double *slope;            // tangent form: one sum for each (sequence, head)
-    int64_t st_a, st_c;
-    void *out;                // (rows, heads, dc), float32 (out_f32) or the tensors' type; NULL: not wanted
-    int out_f32;
-    int n_seq, rows, heads, da, dc, reverse;
-    float out_scale, upd_scale;
-};
-
-template <typename T> __device__ __forceinline__ float as_float(T x);
-template <> __device__ __forceinline__ float as_float<float>(float x) { return x; }
-template <> __device__ __forceinline__ float as_float<__bf16>(__bf16 x) { return (float)x; }
-
-// g^e for a whole number e: 1 for e = 0, also where log g is -inf
-__device__ __forceinline__ float decay_pow(float lg2, int e) { return e == 0 ? 1.0f : exp2f(lg2 * (float)e); }
-
-// The rows of sequence n: [lo, hi) of the packed tensors or of its own rows.  Whatever the offsets hold, 0 <= lo <= hi <= rows.
-__device__ __forceinline__ void row_range(const int32_t *offsets, int rows, int n, int &lo, int &hi) {
-    lo = 0;
-    hi = rows;
-    if (offsets) {
-        lo = min(max(offsets[n], 0), rows);
-        hi = min(max(offsets[n + 1], lo), rows);
-    }
-}
-
-template <typename T> __device__ __forceinline__ const T *row_ptr(const View &t, int packed, int n, int h, int row) {
-    return (const T *)t.p + (packed ? 0 : n * t.seq) + row * t.row + (h / t.share) * t.head;
-}
-
-// The recurrence one row at a time: a workgroup per (sequence, head), a thread holds half a column of the state.
-template <typename T, bool TANGENT>
-__global__ __launch_bounds__(256) void td_decay_serial_kernel(Pass P) {
-    constexpr int D = TD_DECAY_MAX_DIM, HALF = D / 2;
-    __shared__ float sa[D], sb[D], sc[D], part[2][D];
-    __shared__ double red[256];
-    const int h = blockIdx.x % P.heads, n = blockIdx.x / P.heads, tid = threadIdx.x;
-    const int col = tid & (D - 1), half = tid / D, packed = P.offsets != nullptr;
+// The state entering each segment from what each segment adds: in place, one thread an element
+template <bool TAN> __global__ __launch_bounds__(256) void td_decay_scan_kernel(Pass P) {
+    const int size = P.da * P.dc, blocks = (size + 255) / 256, el = blockIdx.x % blocks * 256 + threadIdx.x;
+    const int h = blockIdx.x / blocks % P.heads, n = blockIdx.x / blocks / P.heads;
     int lo, hi;
     row_range(P.offsets, P.rows, n, lo, hi);
-    const float g = expf(P.log_decay[h]);
-    const int64_t state_at = ((int64_t)n * P.heads + h) * P.da * P.dc;
-    float S[HALF], H[TANGENT ? HALF : 1];
-#pragma unroll
-    for (int r = 0; r < HALF; ++r) {
-        const int i = half * HALF + r;
-        S[r] = P.state_in && i < P.da && col < P.dc ? P.state_in[state_at + i * P.st_a + col * P.st_c] : 0.0f;
-        if (TANGENT) H[r] = 0.0f;
-    }
-    double slope = 0.0;
-    for (int t = 0; t < hi - lo; ++t) {
-        const int row = P.reverse ? hi - 1 - t : lo + t;
-        __syncthreads();
-        if (tid < D) {
-            sa[tid] = tid < P.da ? as_float<T>(row_ptr<T>(P.a, packed, n, h, row)[tid]) : 0.0f;
-            sb[tid] = tid < P.da ? as_float<T>(row_ptr<T>(P.b, packed, n, h, row)[tid]) : 0.0f;
-        } else {
-            sc[col] = col < P.dc ? as_float<T>(row_ptr<T>(P.c, packed, n, h, row)[col]) : 0.0f;
-        }
-        __syncthreads();
-        const float c = sc[col] * P.upd_scale;
-        float sum = 0.0f, tan = 0.0f;
-#pragma unroll
-        for (int r = 0; r < HALF; ++r) {
-            const float a = sa[half * HALF + r], b = sb[half * HALF + r];
-            if (P.reverse) {
-                S[r] += b * c;
-                sum += a * S[r];
-                S[r] *= g;
-            } else {
-                if (TANGENT) {
-                    H[r] = g * (H[r] + S[r]);
-                    tan += a * H[r];
-                }
-                S[r] = g * S[r] + b * c;
-                sum += a * S[r];
-            }
-        }
-        part[half][col] = sum;
-        __syncthreads();
-        const int64_t at = ((int64_t)(packed ? 0 : n) * P.rows + row) * P.heads + h;
-        if (half == 0 && col < P.dc && P.out) {
-            const float v = (part[0][col] + part[1][col]) * P.out_scale;
-            if (P.out_f32) ((float *)P.out)[at * P.dc + col] = v;
-            else ((T *)P.out)[at * P.dc + col] = (T)v;
-        }
-        if (TANGENT && col < P.dc) slope += (double)(tan * P.out_scale * as_float<T>(row_ptr<T>(P.e, packed, n, h, row)[col]));
-    }
-#pragma unroll
-    for (int r = 0; r < HALF; ++r) {
-        const int i = half * HALF + r;
-        if (i < P.da && col < P.dc) {
-            const int64_t at = state_at + i * P.st_a + col * P.st_c;
-            if (P.state_out) P.state_out[at] = S[r];
-            if (TANGENT && P.grad_state) slope += (double)(H[r] * P.grad_state[at]);
-        }
-    }
-    if (TANGENT) {
-        red[tid] = slope;
-        __syncthreads();
-        for (int o = 128; o > 0; o >>= 1) {
-            if (tid < o) red[tid] += red[tid + o];
-            __syncthreads();
-        }
-        if (tid == 0) P.slope[blockIdx.x] = red[0];
+    const int segments = (hi - lo + P.seg_len - 1) / P.seg_len;
+    if (segments < 2 || el >= size) return;
+    const double whole_d = exp((double)P.log_decay[h] * P.seg_len);
+    const float whole = (float)whole_d;
+    const int64_t first = P.offsets ? first_slot(P, n) : (int64_t)n * P.segs, by = (int64_t)P.heads * size;
+    float *seg = P.seg + (first * P.heads + h) * size + el, *tan = TAN ? P.seg_tan + (first * P.heads + h) * size + el : nullptr;
+    float F = P.state_in ? P.state_in[((int64_t)n * P.heads + h) * size + el] : 0.0f, H = 0.0f;
+    float add = seg[0], add_tan = TAN ? tan[0] : 0.0f;
+    for (int p = 1; p < segments; ++p) {
+        const float next = p < segments - 1 ? seg[p * by] : 0.0f, next_tan = TAN && p < segments - 1 ? tan[p * by] : 0.0f;
+        if (TAN) tan[p * by] = H = whole * (H + (float)P.seg_len * F) + add_tan;
+        seg[p * by] = F = whole * F + add;
+        add = next;
+        add_tan = next_tan;
     }
 }
 
@@ -174,8 +81,8 @@ __global__ __launch_bounds__(256) void td_decay_step_kernel(Pass P) {
     const float g = expf(P.log_decay[h]);
     float sum = 0.0f;
     if (col < P.dc) {
-        const T *a = row_ptr<T>(P.a, 0, n, h, 0), *b = row_ptr<T>(P.b, 0, n, h, 0);
-        const float c = as_float<T>(row_ptr<T>(P.c, 0, n, h, 0)[col]);
+        const T *a = base_of<T>(P.a, false, n, h), *b = base_of<T>(P.b, false, n, h);
+        const float c = as_float<T>(base_of<T>(P.c, false, n, h)[col]);
         float *S = P.state_out + (int64_t)blockIdx.x * P.da * P.dc + col;
         for (int i = half; i < P.da; i += 2) {
             const float s = g * S[(int64_t)i * P.dc] + as_float<T>(b[i]) * c;
@@ -200,14 +107,39 @@ int check_config(const td_decay_config *c) {
     TD_REQUIRE(c->heads >= 1 && c->q_heads >= 1 && c->k_heads >= 1 && c->v_heads >= 1 && c->heads % c->q_heads == 0 &&
                    c->heads % c->k_heads == 0 && c->heads % c->v_heads == 0,
                "q_heads, k_heads and v_heads must divide heads, got %d, %d, %d and %d", c->q_heads, c->k_heads, c->v_heads, c->heads);
-    TD_REQUIRE((int64_t)c->n_seq * c->heads <= (1 << 30), "n_seq * heads must be at most 2^30");
+    TD_REQUIRE(((int64_t)c->n_seq + c->rows / CHUNK) * c->heads * ((c->dk * c->dv + 255) / 256) < (1LL << 31) &&
+                   (int64_t)c->n_seq * (c->rows / 256 + 1) * c->heads < (1LL << 31),
+               "too many sequences, rows and heads for one launch: n_seq %d, rows %d, heads %d", c->n_seq, c->rows, c->heads);
     return TD_OK;
 }
 
 int64_t total_rows(const td_decay_config *c) { return c->packed ? c->rows : (int64_t)c->n_seq * c->rows; }
 size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 
-View view(const void *p, const int64_t *s, int heads, int own) { return View{p, s[0], s[1], s[2], heads / own}; }
+int esize(const td_decay_config *c) { return c->dtype == TD_BF16 ? 2 : 4; }
+
+View view(const td_decay_config *c, const void *p, const int64_t *s, int own, int d) {
+    const int64_t per = 16 / esize(c);
+    const int vec = (uintptr_t)p % 16 == 0 && d % per == 0 && s[0] % per == 0 && s[1] % per == 0 && s[2] % per == 0;
+    return View{p, s[0], s[1], s[2], c->heads / own, d, vec};
+}
+
+// Segments: enough workgroups to fill the chip (1024: four a compute unit), each of 256 rows at least
+void split(const td_decay_config *c, int &len, int &segs, int64_t &slots) {
+    const int64_t rows = total_rows(c), want = rows * c->heads / 1024;
+    int64_t l = (want > 256 ? want : 256) + CHUNK - 1;
+    l -= l % CHUNK;
+    const int64_t longest = c->rows;
+    if (l >= longest) {
+        len = (int)(longest > 1 ? longest : 1);
+        segs = 1;
+        slots = c->n_seq;
+    } else {
+        len = (int)l;
+        segs = c->packed ? 0 : (int)((longest + l - 1) / l);
+        slots = c->packed ? c->rows / l + c->n_seq : (int64_t)c->n_seq * segs;
+    }
+}
 
 Pass base_pass(const td_decay_config *c, const float *log_decay, const int32_t *offsets) {
     Pass P = {};
@@ -217,15 +149,39 @@ Pass base_pass(const td_decay_config *c, const float *log_decay, const int32_t *
     P.rows = c->rows;
     P.heads = c->heads;
     P.out_scale = P.upd_scale = 1.0f;
+    int64_t slots;
+    split(c, P.seg_len, P.segs, slots);
+    P.slots = (int)slots;
     return P;
 }
 
-template <bool TANGENT> int launch_pass(const td_decay_config *c, const Pass &P, hipStream_t st) {
-    const dim3 grid(c->n_seq * c->heads);
-    if (c->dtype == TD_BF16) hipLaunchKernelGGL((td_decay_serial_kernel<__bf16, TANGENT>), grid, dim3(256), 0, st, P);
-    else hipLaunchKernelGGL((td_decay_serial_kernel<float, TANGENT>), grid, dim3(256), 0, st, P);
+template <typename T, int DP, int NW, int CT, bool TAN, bool SUM> int launch(const Pass &P, hipStream_t st) {
+    hipLaunchKernelGGL((td_decay_chunk_kernel<T, DP, NW, CT, TAN, SUM>), dim3((unsigned)(P.slots * P.heads)), dim3(64 * NW), 0, st, P);
     TD_LAUNCH_CHECK();
     return TD_OK;
+}
+
+template <typename T, bool TAN, bool SUM> int launch_d(const Pass &P, hipStream_t st) {
+    const int d = P.da > P.dc ? P.da : P.dc;
+    if (d <= 32) return launch<T, 32, 2, 1, TAN, SUM>(P, st);
+    if (d <= 64) return launch<T, 64, 4, 1, TAN, SUM>(P, st);
+    return launch<T, 128, 4, 2, TAN, SUM>(P, st);
+}
+
+// What the segments add, and the state that enters each of them (nothing to do where every sequence is one segment)
+template <bool TAN> int enter_states(const td_decay_config *c, const Pass &P, hipStream_t st) {
+    if (P.segs == 1) return TD_OK;
+    const int rc = c->dtype == TD_BF16 ? launch_d<__bf16, TAN, true>(P, st) : launch_d<float, TAN, true>(P, st);
+    if (rc != TD_OK) return rc;
+    const int64_t blocks = (int64_t)P.n_seq * P.heads * ((P.da * P.dc + 255) / 256);
+    hipLaunchKernelGGL(td_decay_scan_kernel<TAN>, dim3((unsigned)blocks), dim3(256), 0, st, P);
+    TD_LAUNCH_CHECK();
+    return TD_OK;
+}
+
+template <bool TAN> int launch_pass(const td_decay_config *c, Pass P, hipStream_t st) {
+    P.out_vec = P.dc % 4 == 0 && (uintptr_t)P.out % 16 == 0;
+    return c->dtype == TD_BF16 ? launch_d<__bf16, TAN, false>(P, st) : launch_d<float, TAN, false>(P, st);
 }
 
 int clear_rows(const td_decay_config *c, const int32_t *offsets, int width, void *out, hipStream_t st) {
@@ -257,14 +213,20 @@ int grad_pass(const td_decay_config *c, Pass P, int own_heads, int d, void *grad
     return clear_rows(c, P.offsets, own_heads * d, grad, st);
 }
 
-struct Layout { size_t slope, parts, total; };
-Layout backward_layout(const td_decay_config *c) {
-    Layout w;
-    w.slope = 0;
-    w.parts = up256((size_t)c->n_seq * c->heads * sizeof(double));
-    const int d = c->dk > c->dv ? c->dk : c->dv;
+struct Layout { size_t seg, seg_tan, slope, parts, total; };
+Layout layout(const td_decay_config *c, bool backward) {
+    int len, segs;
+    int64_t slots;
+    split(c, len, segs, slots);
+    const size_t states = segs == 1 ? 0 : up256((size_t)slots * c->heads * c->dk * c->dv * sizeof(float));
     const bool shared = c->q_heads != c->heads || c->k_heads != c->heads || c->v_heads != c->heads;
-    w.total = w.parts + (shared ? up256((size_t)total_rows(c) * c->heads * d * sizeof(float)) : 0);
+    const int d = c->dk > c->dv ? c->dk : c->dv;
+    Layout w;
+    w.seg = 0;
+    w.seg_tan = states;
+    w.slope = w.seg_tan + (backward ? states : 0);
+    w.parts = w.slope + (backward ? up256((size_t)slots * c->heads * sizeof(double)) : 0);
+    w.total = w.parts + (backward && shared ? up256((size_t)total_rows(c) * c->heads * d * sizeof(float)) : 256);
     return w;
 }
 
@@ -272,7 +234,7 @@ Layout backward_layout(const td_decay_config *c) {
 
 extern "C" size_t td_decay_workspace_bytes(const td_decay_config *cfg, int32_t backward) {
     if (check_config(cfg) != TD_OK) return 0;
-    return backward ? backward_layout(cfg).total : 256;
+    return layout(cfg, backward != 0).total;
 }
 
 extern "C" int td_decay_forward(const td_decay_config *cfg, const void *q, const void *k, const void *v, const float *log_decay,
@@ -282,12 +244,14 @@ extern "C" int td_decay_forward(const td_decay_config *cfg, const void *q, const
     TD_REQUIRE(!cfg->packed || offsets, "packed sequences need offsets");
     TD_REQUIRE(!state_out || state_out != state_in, "state_in and state_out must not be the same memory");
     Pass P = base_pass(cfg, log_decay, offsets);
-    P.a = view(q, cfg->q_stride, cfg->heads, cfg->q_heads);
-    P.b = view(k, cfg->k_stride, cfg->heads, cfg->k_heads);
-    P.c = view(v, cfg->v_stride, cfg->heads, cfg->v_heads);
+    P.a = view(cfg, q, cfg->q_stride, cfg->q_heads, cfg->dk);
+    P.b = view(cfg, k, cfg->k_stride, cfg->k_heads, cfg->dk);
+    P.c = view(cfg, v, cfg->v_stride, cfg->v_heads, cfg->dv);
     P.da = cfg->dk; P.dc = cfg->dv; P.st_a = cfg->dv; P.st_c = 1;
     P.state_in = state_in; P.state_out = state_out;
     P.out = o; P.out_scale = cfg->scale;
+    P.seg = (float *)workspace;
+    if (int rc = enter_states<false>(cfg, P, (hipStream_t)stream)) return rc;
     if (int rc = launch_pass<false>(cfg, P, (hipStream_t)stream)) return rc;
     return clear_rows(cfg, offsets, cfg->heads * cfg->dv, o, (hipStream_t)stream);
 }
@@ -299,37 +263,42 @@ extern "C" int td_decay_backward(const td_decay_config *cfg, const void *q, cons
     TD_REQUIRE(log_decay && workspace && (cfg->rows == 0 || (q && k && v && grad_o)), "null pointer");
     TD_REQUIRE(!cfg->packed || offsets, "packed sequences need offsets");
     hipStream_t st = (hipStream_t)stream;
-    const Layout w = backward_layout(cfg);
+    const Layout w = layout(cfg, true);
     float *parts = (float *)((char *)workspace + w.parts);
-    const View vq = view(q, cfg->q_stride, cfg->heads, cfg->q_heads), vk = view(k, cfg->k_stride, cfg->heads, cfg->k_heads),
-               vv = view(v, cfg->v_stride, cfg->heads, cfg->v_heads), vo = view(grad_o, cfg->grad_o_stride, cfg->heads, cfg->heads);
+    const View vq = view(cfg, q, cfg->q_stride, cfg->q_heads, cfg->dk), vk = view(cfg, k, cfg->k_stride, cfg->k_heads, cfg->dk),
+               vv = view(cfg, v, cfg->v_stride, cfg->v_heads, cfg->dv), vo = view(cfg, grad_o, cfg->grad_o_stride, cfg->heads, cfg->dv);
     if (grad_q || grad_log_decay) {
         Pass P = base_pass(cfg, log_decay, offsets);
         P.a = vo; P.b = vv; P.c = vk; P.e = vq;
         P.da = cfg->dv; P.dc = cfg->dk; P.st_a = 1; P.st_c = cfg->dv;
         P.state_in = state_in; P.grad_state = grad_state_out; P.slope = (double *)((char *)workspace + w.slope);
         P.out_scale = cfg->scale;
+        P.seg = (float *)((char *)workspace + w.seg); P.seg_tan = (float *)((char *)workspace + w.seg_tan);
+        if (int rc = grad_log_decay ? enter_states<true>(cfg, P, st) : enter_states<false>(cfg, P, st)) return rc;
         if (int rc = grad_pass(cfg, P, cfg->q_heads, cfg->dk, grad_q, parts, grad_log_decay != nullptr, st)) return rc;
         if (grad_log_decay) {
-            hipLaunchKernelGGL(td_decay_slope_kernel, dim3(cfg->heads), dim3(256), 0, st, P.slope, cfg->n_seq, cfg->heads, grad_log_decay);
+            hipLaunchKernelGGL(td_decay_slope_kernel, dim3(cfg->heads), dim3(256), 0, st, P.slope, P.slots, cfg->heads, grad_log_decay);
             TD_LAUNCH_CHECK();
         }
     }
-    if (grad_v || grad_state_in) {
+    if (grad_v || grad_k || grad_state_in) {
         Pass P = base_pass(cfg, log_decay, offsets);
         P.reverse = 1;
         P.a = vk; P.b = vq; P.c = vo;
         P.da = cfg->dk; P.dc = cfg->dv; P.st_a = cfg->dv; P.st_c = 1;
-        P.state_in = grad_state_out; P.state_out = grad_state_in; P.upd_scale = cfg->scale;
-        if (int rc = grad_pass(cfg, P, cfg->v_heads, cfg->dv, grad_v, parts, false, st)) return rc;
-    }
-    if (grad_k) {
-        Pass P = base_pass(cfg, log_decay, offsets);
-        P.reverse = 1;
-        P.a = vv; P.b = vo; P.c = vq;
-        P.da = cfg->dv; P.dc = cfg->dk; P.st_a = 1; P.st_c = cfg->dv;
         P.state_in = grad_state_out; P.upd_scale = cfg->scale;
-        if (int rc = grad_pass(cfg, P, cfg->k_heads, cfg->dk, grad_k, parts, false, st)) return rc;
+        P.seg = (float *)((char *)workspace + w.seg);
+        if (int rc = enter_states<false>(cfg, P, st)) return rc;
+        if (grad_v || grad_state_in) {
+            P.state_out = grad_state_in;
+            if (int rc = grad_pass(cfg, P, cfg->v_heads, cfg->dv, grad_v, parts, false, st)) return rc;
+        }
+        if (grad_k) {
+            P.state_out = nullptr;
+            P.a = vv; P.b = vo; P.c = vq;
+            P.da = cfg->dv; P.dc = cfg->dk; P.st_a = 1; P.st_c = cfg->dv;
+            if (int rc = grad_pass(cfg, P, cfg->k_heads, cfg->dk, grad_k, parts, false, st)) return rc;
+        }
     }
     return TD_OK;
 }
@@ -340,9 +309,9 @@ extern "C" int td_decay_step(const td_decay_config *cfg, const void *q, const vo
     TD_REQUIRE(cfg->rows == 1 && !cfg->packed, "td_decay_step takes one row of each sequence (rows = 1, packed = 0)");
     TD_REQUIRE(q && k && v && log_decay && state && o, "null pointer");
     Pass P = base_pass(cfg, log_decay, nullptr);
-    P.a = view(q, cfg->q_stride, cfg->heads, cfg->q_heads);
-    P.b = view(k, cfg->k_stride, cfg->heads, cfg->k_heads);
-    P.c = view(v, cfg->v_stride, cfg->heads, cfg->v_heads);
+    P.a = view(cfg, q, cfg->q_stride, cfg->q_heads, cfg->dk);
+    P.b = view(cfg, k, cfg->k_stride, cfg->k_heads, cfg->dk);
+    P.c = view(cfg, v, cfg->v_stride, cfg->v_heads, cfg->dv);
     P.da = cfg->dk; P.dc = cfg->dv;
     P.state_out = state; P.out = o; P.out_scale = cfg->scale;
     const dim3 grid(cfg->n_seq * cfg->heads);
