@@ -110,6 +110,7 @@ int check_config(const td_decay_config *c) {
     TD_REQUIRE(((int64_t)c->n_seq + c->rows / CHUNK) * c->heads * ((c->dk * c->dv + 255) / 256) < (1LL << 31) &&
                    (int64_t)c->n_seq * (c->rows / 256 + 1) * c->heads < (1LL << 31),
                "too many sequences, rows and heads for one launch: n_seq %d, rows %d, heads %d", c->n_seq, c->rows, c->heads);
+    TD_REQUIRE((int64_t)c->heads * TD_DECAY_MAX_DIM * CHUNK * 4 < (1LL << 31), "heads must be below 65536, got %d", c->heads);
     return TD_OK;
 }
 
@@ -118,10 +119,13 @@ size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 
 int esize(const td_decay_config *c) { return c->dtype == TD_BF16 ? 2 : 4; }
 
-View view(const td_decay_config *c, const void *p, const int64_t *s, int own, int d) {
+View view(const td_decay_config *c, const void *p, const int64_t *s, int own, int d) { return View{p, s[0], s[1], s[2], c->heads / own, d}; }
+
+// Whether a tensor can be read 16 bytes at a time, a chunk's rows at 32-bit offsets from its first
+bool wide(const td_decay_config *c, const View &v) {
     const int64_t per = 16 / esize(c);
-    const int vec = (uintptr_t)p % 16 == 0 && d % per == 0 && s[0] % per == 0 && s[1] % per == 0 && s[2] % per == 0;
-    return View{p, s[0], s[1], s[2], c->heads / own, d, vec};
+    return (uintptr_t)v.p % 16 == 0 && v.d % per == 0 && v.seq % per == 0 && v.row % per == 0 && v.head % per == 0 && v.row >= 0 &&
+           v.row < (1LL << 31) / CHUNK / 4;
 }
 
 // Segments: enough workgroups to fill the chip (1024: four a compute unit), each of 256 rows at least
@@ -155,33 +159,35 @@ Pass base_pass(const td_decay_config *c, const float *log_decay, const int32_t *
     return P;
 }
 
-template <typename T, int DP, int NW, int CT, bool TAN, bool SUM> int launch(const Pass &P, hipStream_t st) {
-    hipLaunchKernelGGL((td_decay_chunk_kernel<T, DP, NW, CT, TAN, SUM>), dim3((unsigned)(P.slots * P.heads)), dim3(64 * NW), 0, st, P);
+template <typename T, int DP, int NW, int CT, bool VEC, Form FORM, int WAVES> int launch(const Pass &P, hipStream_t st) {
+    hipLaunchKernelGGL((td_decay_chunk_kernel<T, DP, NW, CT, VEC, FORM, WAVES>), dim3((unsigned)(P.slots * P.heads)), dim3(64 * NW), 0, st, P);
     TD_LAUNCH_CHECK();
     return TD_OK;
 }
 
-template <typename T, bool TAN, bool SUM> int launch_d(const Pass &P, hipStream_t st) {
+template <typename T, bool VEC, Form FORM> int launch_d(const Pass &P, hipStream_t st) {
+    constexpr bool tan = FORM == OUT_TANGENT || FORM == SUM_TANGENT;
     const int d = P.da > P.dc ? P.da : P.dc;
-    if (d <= 32) return launch<T, 32, 2, 1, TAN, SUM>(P, st);
-    if (d <= 64) return launch<T, 64, 4, 1, TAN, SUM>(P, st);
-    return launch<T, 128, 4, 2, TAN, SUM>(P, st);
+    if (d <= 32) return launch<T, 32, 2, 1, VEC, FORM, 3>(P, st);
+    if (d <= 64) return launch<T, 64, 4, 1, VEC, FORM, tan ? 2 : 3>(P, st);
+    return launch<T, 128, 4, 2, VEC, FORM, tan ? 1 : 2>(P, st);
+}
+
+template <Form FORM> int launch_form(const td_decay_config *c, const Pass &P, hipStream_t st) {
+    constexpr bool add = FORM == SUM || FORM == SUM_TANGENT;
+    const bool vec = wide(c, P.b) && wide(c, P.c) && (add || (wide(c, P.a) && (uintptr_t)P.out % 16 == 0)) && (FORM != OUT_TANGENT || wide(c, P.e));
+    if (c->dtype == TD_BF16) return vec ? launch_d<__bf16, true, FORM>(P, st) : launch_d<__bf16, false, FORM>(P, st);
+    return vec ? launch_d<float, true, FORM>(P, st) : launch_d<float, false, FORM>(P, st);
 }
 
 // What the segments add, and the state that enters each of them (nothing to do where every sequence is one segment)
 template <bool TAN> int enter_states(const td_decay_config *c, const Pass &P, hipStream_t st) {
     if (P.segs == 1) return TD_OK;
-    const int rc = c->dtype == TD_BF16 ? launch_d<__bf16, TAN, true>(P, st) : launch_d<float, TAN, true>(P, st);
-    if (rc != TD_OK) return rc;
+    if (int rc = launch_form<TAN ? SUM_TANGENT : SUM>(c, P, st)) return rc;
     const int64_t blocks = (int64_t)P.n_seq * P.heads * ((P.da * P.dc + 255) / 256);
     hipLaunchKernelGGL(td_decay_scan_kernel<TAN>, dim3((unsigned)blocks), dim3(256), 0, st, P);
     TD_LAUNCH_CHECK();
     return TD_OK;
-}
-
-template <bool TAN> int launch_pass(const td_decay_config *c, Pass P, hipStream_t st) {
-    P.out_vec = P.dc % 4 == 0 && (uintptr_t)P.out % 16 == 0;
-    return c->dtype == TD_BF16 ? launch_d<__bf16, TAN, false>(P, st) : launch_d<float, TAN, false>(P, st);
 }
 
 int clear_rows(const td_decay_config *c, const int32_t *offsets, int width, void *out, hipStream_t st) {
@@ -198,7 +204,7 @@ int grad_pass(const td_decay_config *c, Pass P, int own_heads, int d, void *grad
     const bool shared = own_heads != c->heads;
     P.out = !grad ? nullptr : shared ? (void *)parts : grad;
     P.out_f32 = shared;
-    int rc = tangent ? launch_pass<true>(c, P, st) : launch_pass<false>(c, P, st);
+    int rc = tangent ? launch_form<OUT_TANGENT>(c, P, st) : launch_form<OUT>(c, P, st);
     if (rc != TD_OK || !grad) return rc;
     const int64_t n = total_rows(c) * own_heads * d;
     if (shared && n > 0) {
@@ -252,7 +258,7 @@ extern "C" int td_decay_forward(const td_decay_config *cfg, const void *q, const
     P.out = o; P.out_scale = cfg->scale;
     P.seg = (float *)workspace;
     if (int rc = enter_states<false>(cfg, P, (hipStream_t)stream)) return rc;
-    if (int rc = launch_pass<false>(cfg, P, (hipStream_t)stream)) return rc;
+    if (int rc = launch_form<OUT>(cfg, P, (hipStream_t)stream)) return rc;
     return clear_rows(cfg, offsets, cfg->heads * cfg->dv, o, (hipStream_t)stream);
 }
 
