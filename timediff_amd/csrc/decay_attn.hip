@@ -5,36 +5,60 @@
 // is the forward pass for (a, b, c) = (q, k, v); the gradient of q for (grad_o, v, k) with the state transposed; and, run from
 // the last row to the first, the gradient of v for (k, q, grad_o) and that of k for (v, grad_o, q), where M is the gradient of
 // the state BEHIND a row: it enters a row undecayed and decays when it leaves it.
-// The decay's gradient is sum_t <grad_o_t, d o_t / d log g>, and d M_t / d log g = g (M'_{t-1} + M_{t-1}) is carried beside M in the
-// pass that computes grad_q: a sum without cancellation, where sum_t t (q.grad_q - k.grad_k) would lose everything for fast decays.
+//
+// The gradient by log g is sum over t >= s of (t - s) g^(t-s) (q_t . k_s)(v_s . grad_o_t) and the entering state's like terms.  The number
+// of rows from s to t is cut where chunks begin: rows of t's chunk up to t (from grad_q's part that the state entering that chunk made, row
+// by row), rows of s's chunk behind s (from grad_k's part that the chunks behind it made), and the n rows of every chunk between (n times
+// the product of the state entering it and the gradient of the state leaving it).  Nothing cancels, where the shorter
+// sum_t t (q_t . grad_q_t - k_t . grad_k_t) would lose everything for decays that forget within a few rows.
 #include "decay_chunk.h"
 
 using namespace decay;
+
+// decay_inst.hip: one launcher per (element type, kernel)
+#define TD_LAUNCHERS(b)                                                                                                              \
+    int td_decay_launch_##b##_0(const Pass &, int, hipStream_t); int td_decay_launch_##b##_1(const Pass &, int, hipStream_t);       \
+    int td_decay_launch_##b##_2(const Pass &, int, hipStream_t); int td_decay_launch_##b##_3(const Pass &, int, hipStream_t);       \
+    int td_decay_launch_##b##_4(const Pass &, int, hipStream_t); int td_decay_launch_##b##_5(const Pass &, int, hipStream_t);
+TD_LAUNCHERS(0)
+TD_LAUNCHERS(1)
 
 namespace {
 
 template <typename T> __device__ __forceinline__ float as_float(T x) { return (float)x; }
 
-// The state entering each segment from what each segment adds: in place, one thread an element
-template <bool TAN> __global__ __launch_bounds__(256) void td_decay_scan_kernel(Pass P) {
+// The state entering each segment (REV: its gradient behind each segment) from what each segment adds: in place, one thread an element
+template <bool REV> __global__ __launch_bounds__(256) void td_decay_scan_kernel(Pass P) {
     const int size = P.da * P.dc, blocks = (size + 255) / 256, el = blockIdx.x % blocks * 256 + threadIdx.x;
     const int h = blockIdx.x / blocks % P.heads, n = blockIdx.x / blocks / P.heads;
     int lo, hi;
     row_range(P.offsets, P.rows, n, lo, hi);
     const int segments = (hi - lo + P.seg_len - 1) / P.seg_len;
     if (segments < 2 || el >= size) return;
-    const double whole_d = exp((double)P.log_decay[h] * P.seg_len);
-    const float whole = (float)whole_d;
-    const int64_t first = P.offsets ? first_slot(P, n) : (int64_t)n * P.segs, by = (int64_t)P.heads * size;
-    float *seg = P.seg + (first * P.heads + h) * size + el, *tan = TAN ? P.seg_tan + (first * P.heads + h) * size + el : nullptr;
-    float F = P.state_in ? P.state_in[((int64_t)n * P.heads + h) * size + el] : 0.0f, H = 0.0f;
-    float add = seg[0], add_tan = TAN ? tan[0] : 0.0f;
-    for (int p = 1; p < segments; ++p) {
-        const float next = p < segments - 1 ? seg[p * by] : 0.0f, next_tan = TAN && p < segments - 1 ? tan[p * by] : 0.0f;
-        if (TAN) tan[p * by] = H = whole * (H + (float)P.seg_len * F) + add_tan;
-        seg[p * by] = F = whole * F + add;
-        add = next;
-        add_tan = next_tan;
+    const float ld = P.log_decay[h];
+    const Factor whole = factor(ld, P.seg_len);
+    const int64_t first = P.offsets ? first_place(P, n, P.seg_len) : (int64_t)n * P.segs, by = (int64_t)P.heads * size;
+    float *seg = P.seg + (first * P.heads + h) * size + el;
+    float F = P.state_in ? P.state_in[((int64_t)n * P.heads + h) * size + el] : 0.0f;
+    if (REV) {
+        seg += (segments - 1) * by;
+        float add = seg[0];
+        seg[0] = F;
+        F = times(factor(ld, hi - lo - (segments - 1) * P.seg_len), F) + add;
+    } else {
+        F = times(whole, F) + seg[0];
+    }
+    constexpr int AHEAD = 8;          // the loads do not wait for the sums
+    for (int p = 1; p < segments; p += AHEAD) {
+        float add[AHEAD];
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) add[k] = p + k < segments - 1 ? seg[(REV ? -(p + k) : p + k) * by] : 0.0f;
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k)
+            if (p + k < segments) {
+                seg[(REV ? -(p + k) : p + k) * by] = F;
+                F = times(whole, F) + add[k];
+            }
     }
 }
 
@@ -62,15 +86,6 @@ __global__ __launch_bounds__(256) void td_decay_share_sum_kernel(const float *__
         for (int j = 0; j < share; ++j) s += p[(int64_t)j * d];
         out[i] = (T)s;
     }
-}
-
-// Rows of no sequence: zeros
-template <typename T>
-__global__ __launch_bounds__(256) void td_decay_clear_kernel(const int32_t *offsets, int n_seq, int rows, int width, T *out) {
-    const int lo = min(max(offsets[0], 0), rows), hi = min(max(offsets[n_seq], lo), rows);
-    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x)
-        if (row < lo || row >= hi)
-            for (int i = threadIdx.x; i < width; i += 256) out[row * width + i] = (T)0.0f;
 }
 
 template <typename T>
@@ -128,13 +143,14 @@ bool wide(const td_decay_config *c, const View &v) {
            v.row < (1LL << 31) / CHUNK / 4;
 }
 
-// Segments: enough workgroups to fill the chip (1024: four a compute unit), each of 256 rows at least
+// Segments: a sequence on its own is one after another, chunk by chunk, so few long ones are cut until there are workgroups for the chip (512: two
+// a compute unit), into segments of 256 rows at least; up to 512 rows a cut costs more (two launches and a second reading of k and v)
+// than it saves.
 void split(const td_decay_config *c, int &len, int &segs, int64_t &slots) {
-    const int64_t rows = total_rows(c), want = rows * c->heads / 1024;
+    const int64_t rows = total_rows(c), want = rows * c->heads / 512, longest = c->rows;
     int64_t l = (want > 256 ? want : 256) + CHUNK - 1;
     l -= l % CHUNK;
-    const int64_t longest = c->rows;
-    if (l >= longest) {
+    if (l >= longest || longest <= 512) {
         len = (int)(longest > 1 ? longest : 1);
         segs = 1;
         slots = c->n_seq;
@@ -159,82 +175,61 @@ Pass base_pass(const td_decay_config *c, const float *log_decay, const int32_t *
     return P;
 }
 
-template <typename T, int DP, int NW, int CT, bool VEC, Form FORM, int WAVES> int launch(const Pass &P, hipStream_t st) {
-    hipLaunchKernelGGL((td_decay_chunk_kernel<T, DP, NW, CT, VEC, FORM, WAVES>), dim3((unsigned)(P.slots * P.heads)), dim3(64 * NW), 0, st, P);
-    TD_LAUNCH_CHECK();
-    return TD_OK;
-}
-
-template <typename T, bool VEC, Form FORM> int launch_d(const Pass &P, hipStream_t st) {
-    constexpr bool tan = FORM == OUT_TANGENT || FORM == SUM_TANGENT;
-    const int d = P.da > P.dc ? P.da : P.dc;
-    if (d <= 32) return launch<T, 32, 2, 1, VEC, FORM, 3>(P, st);
-    if (d <= 64) return launch<T, 64, 4, 1, VEC, FORM, tan ? 2 : 3>(P, st);
-    return launch<T, 128, 4, 2, VEC, FORM, tan ? 1 : 2>(P, st);
-}
-
-template <Form FORM> int launch_form(const td_decay_config *c, const Pass &P, hipStream_t st) {
-    constexpr bool add = FORM == SUM || FORM == SUM_TANGENT;
-    const bool vec = wide(c, P.b) && wide(c, P.c) && (add || (wide(c, P.a) && (uintptr_t)P.out % 16 == 0)) && (FORM != OUT_TANGENT || wide(c, P.e));
-    if (c->dtype == TD_BF16) return vec ? launch_d<__bf16, true, FORM>(P, st) : launch_d<__bf16, false, FORM>(P, st);
-    return vec ? launch_d<float, true, FORM>(P, st) : launch_d<float, false, FORM>(P, st);
+int launch(const td_decay_config *c, Kind kind, const Pass &P, bool vec, hipStream_t st) {
+    typedef int (*Launcher)(const Pass &, int, hipStream_t);
+    static const Launcher table[2][6] = {
+        {td_decay_launch_0_0, td_decay_launch_0_1, td_decay_launch_0_2, td_decay_launch_0_3, td_decay_launch_0_4, td_decay_launch_0_5},
+        {td_decay_launch_1_0, td_decay_launch_1_1, td_decay_launch_1_2, td_decay_launch_1_3, td_decay_launch_1_4, td_decay_launch_1_5}};
+    return table[c->dtype == TD_BF16][kind](P, vec, st);
 }
 
 // What the segments add, and the state that enters each of them (nothing to do where every sequence is one segment)
-template <bool TAN> int enter_states(const td_decay_config *c, const Pass &P, hipStream_t st) {
+template <bool REV> int enter_states(const td_decay_config *c, const Pass &P, bool vec, hipStream_t st) {
     if (P.segs == 1) return TD_OK;
-    if (int rc = launch_form<TAN ? SUM_TANGENT : SUM>(c, P, st)) return rc;
+    if (int rc = launch(c, REV ? SUM_REVERSED : SUM, P, vec, st)) return rc;
     const int64_t blocks = (int64_t)P.n_seq * P.heads * ((P.da * P.dc + 255) / 256);
-    hipLaunchKernelGGL(td_decay_scan_kernel<TAN>, dim3((unsigned)blocks), dim3(256), 0, st, P);
+    hipLaunchKernelGGL(td_decay_scan_kernel<REV>, dim3((unsigned)blocks), dim3(256), 0, st, P);
     TD_LAUNCH_CHECK();
     return TD_OK;
 }
 
-int clear_rows(const td_decay_config *c, const int32_t *offsets, int width, void *out, hipStream_t st) {
-    if (!c->packed || c->rows == 0) return TD_OK;
-    const dim3 grid(c->rows < 256 ? c->rows : 256);
-    if (c->dtype == TD_BF16) hipLaunchKernelGGL(td_decay_clear_kernel<__bf16>, grid, dim3(256), 0, st, offsets, c->n_seq, c->rows, width, (__bf16 *)out);
-    else hipLaunchKernelGGL(td_decay_clear_kernel<float>, grid, dim3(256), 0, st, offsets, c->n_seq, c->rows, width, (float *)out);
+// The gradient of a tensor whose heads are shared, from float32 parts of every head
+int share_sum(const td_decay_config *c, const float *parts, void *grad, int own_heads, int d, hipStream_t st) {
+    const int64_t n = total_rows(c) * own_heads * d, blocks = (n + 255) / 256;
+    if (n == 0) return TD_OK;
+    const dim3 grid((unsigned)(blocks > 8192 ? 8192 : blocks));
+    if (c->dtype == TD_BF16)
+        hipLaunchKernelGGL(td_decay_share_sum_kernel<__bf16>, grid, dim3(256), 0, st, parts, (__bf16 *)grad, n, c->heads / own_heads, d);
+    else
+        hipLaunchKernelGGL(td_decay_share_sum_kernel<float>, grid, dim3(256), 0, st, parts, (float *)grad, n, c->heads / own_heads, d);
     TD_LAUNCH_CHECK();
     return TD_OK;
 }
 
-// One gradient: straight into `grad` where every head has its own, else into float32 `parts` and their sum
-int grad_pass(const td_decay_config *c, Pass P, int own_heads, int d, void *grad, float *parts, bool tangent, hipStream_t st) {
-    const bool shared = own_heads != c->heads;
-    P.out = !grad ? nullptr : shared ? (void *)parts : grad;
-    P.out_f32 = shared;
-    int rc = tangent ? launch_form<OUT_TANGENT>(c, P, st) : launch_form<OUT>(c, P, st);
-    if (rc != TD_OK || !grad) return rc;
-    const int64_t n = total_rows(c) * own_heads * d;
-    if (shared && n > 0) {
-        const int64_t blocks = (n + 255) / 256;
-        const dim3 grid((unsigned)(blocks > 8192 ? 8192 : blocks));
-        if (c->dtype == TD_BF16)
-            hipLaunchKernelGGL(td_decay_share_sum_kernel<__bf16>, grid, dim3(256), 0, st, parts, (__bf16 *)grad, n, c->heads / own_heads, d);
-        else
-            hipLaunchKernelGGL(td_decay_share_sum_kernel<float>, grid, dim3(256), 0, st, parts, (float *)grad, n, c->heads / own_heads, d);
-        TD_LAUNCH_CHECK();
-    }
-    return clear_rows(c, P.offsets, own_heads * d, grad, st);
-}
-
-struct Layout { size_t seg, seg_tan, slope, parts, total; };
+struct Layout { size_t seg, chunks, slope, parts, parts2, total; };
 Layout layout(const td_decay_config *c, bool backward) {
     int len, segs;
     int64_t slots;
     split(c, len, segs, slots);
-    const size_t states = segs == 1 ? 0 : up256((size_t)slots * c->heads * c->dk * c->dv * sizeof(float));
-    const bool shared = c->q_heads != c->heads || c->k_heads != c->heads || c->v_heads != c->heads;
-    const int d = c->dk > c->dv ? c->dk : c->dv;
+    const size_t state = (size_t)c->heads * c->dk * c->dv * sizeof(float), rows = (size_t)total_rows(c) * c->heads * sizeof(float);
+    // the waves hold states of whole tiles: at most 32 x 32, else multiples of 64
+    const auto pad = [](int d, int most) { return most <= 32 ? 32 : d <= 64 ? 64 : 128; };
+    const int most = c->dk > c->dv ? c->dk : c->dv;
+    const bool square = most > 64;        // unaligned tensors take the larger side for both
+    const size_t held = (size_t)c->heads * (square ? 128 : pad(c->dk, most)) * (square ? 128 : pad(c->dv, most)) * sizeof(float);
+    const size_t chunks = c->packed ? (size_t)c->rows / CHUNK + c->n_seq : (size_t)c->n_seq * ((c->rows + CHUNK - 1) / CHUNK);
     Layout w;
     w.seg = 0;
-    w.seg_tan = states;
-    w.slope = w.seg_tan + (backward ? states : 0);
-    w.parts = w.slope + (backward ? up256((size_t)slots * c->heads * sizeof(double)) : 0);
-    w.total = w.parts + (backward && shared ? up256((size_t)total_rows(c) * c->heads * d * sizeof(float)) : 256);
+    w.chunks = segs == 1 ? 0 : up256(slots * state);
+    w.slope = w.chunks + (backward ? chunks * held : 0);
+    w.parts = w.slope + (backward ? up256(2 * (size_t)slots * c->heads * sizeof(double)) : 0);
+    const bool qv = c->q_heads != c->heads || c->v_heads != c->heads, k = c->k_heads != c->heads;
+    w.parts2 = w.parts + (backward && qv ? up256(rows * most) : 0);
+    w.total = w.parts2 + (backward && k ? up256(rows * c->dk) : 0) + 256;
     return w;
 }
+
+bool aligned(const void *p) { return (uintptr_t)p % 16 == 0; }
 
 }  // namespace
 
@@ -249,6 +244,7 @@ extern "C" int td_decay_forward(const td_decay_config *cfg, const void *q, const
     TD_REQUIRE(log_decay && workspace && (cfg->rows == 0 || (q && k && v && o)), "null pointer");
     TD_REQUIRE(!cfg->packed || offsets, "packed sequences need offsets");
     TD_REQUIRE(!state_out || state_out != state_in, "state_in and state_out must not be the same memory");
+    hipStream_t st = (hipStream_t)stream;
     Pass P = base_pass(cfg, log_decay, offsets);
     P.a = view(cfg, q, cfg->q_stride, cfg->q_heads, cfg->dk);
     P.b = view(cfg, k, cfg->k_stride, cfg->k_heads, cfg->dk);
@@ -257,9 +253,9 @@ extern "C" int td_decay_forward(const td_decay_config *cfg, const void *q, const
     P.state_in = state_in; P.state_out = state_out;
     P.out = o; P.out_scale = cfg->scale;
     P.seg = (float *)workspace;
-    if (int rc = enter_states<false>(cfg, P, (hipStream_t)stream)) return rc;
-    if (int rc = launch_form<OUT>(cfg, P, (hipStream_t)stream)) return rc;
-    return clear_rows(cfg, offsets, cfg->heads * cfg->dv, o, (hipStream_t)stream);
+    const bool vec = wide(cfg, P.a) && wide(cfg, P.b) && wide(cfg, P.c) && aligned(o);
+    if (int rc = enter_states<false>(cfg, P, vec, st)) return rc;
+    return launch(cfg, OUT, P, vec, st);
 }
 
 extern "C" int td_decay_backward(const td_decay_config *cfg, const void *q, const void *k, const void *v, const float *log_decay,
@@ -270,41 +266,50 @@ extern "C" int td_decay_backward(const td_decay_config *cfg, const void *q, cons
     TD_REQUIRE(!cfg->packed || offsets, "packed sequences need offsets");
     hipStream_t st = (hipStream_t)stream;
     const Layout w = layout(cfg, true);
-    float *parts = (float *)((char *)workspace + w.parts);
+    char *ws = (char *)workspace;
+    float *parts = (float *)(ws + w.parts), *parts2 = (float *)(ws + w.parts2);
     const View vq = view(cfg, q, cfg->q_stride, cfg->q_heads, cfg->dk), vk = view(cfg, k, cfg->k_stride, cfg->k_heads, cfg->dk),
                vv = view(cfg, v, cfg->v_stride, cfg->v_heads, cfg->dv), vo = view(cfg, grad_o, cfg->grad_o_stride, cfg->heads, cfg->dv);
-    if (grad_q || grad_log_decay) {
-        Pass P = base_pass(cfg, log_decay, offsets);
-        P.a = vo; P.b = vv; P.c = vk; P.e = vq;
-        P.da = cfg->dv; P.dc = cfg->dk; P.st_a = 1; P.st_c = cfg->dv;
-        P.state_in = state_in; P.grad_state = grad_state_out; P.slope = (double *)((char *)workspace + w.slope);
-        P.out_scale = cfg->scale;
-        P.seg = (float *)((char *)workspace + w.seg); P.seg_tan = (float *)((char *)workspace + w.seg_tan);
-        if (int rc = grad_log_decay ? enter_states<true>(cfg, P, st) : enter_states<false>(cfg, P, st)) return rc;
-        if (int rc = grad_pass(cfg, P, cfg->q_heads, cfg->dk, grad_q, parts, grad_log_decay != nullptr, st)) return rc;
-        if (grad_log_decay) {
-            hipLaunchKernelGGL(td_decay_slope_kernel, dim3(cfg->heads), dim3(256), 0, st, P.slope, P.slots, cfg->heads, grad_log_decay);
-            TD_LAUNCH_CHECK();
-        }
+    // one answer for every kernel of the call: the states that one leaves for another are laid out by it
+    const bool vec = wide(cfg, vq) && wide(cfg, vk) && wide(cfg, vv) && wide(cfg, vo) && aligned(grad_q) && aligned(grad_k) && aligned(grad_v);
+    const bool slope = grad_log_decay != nullptr, q_shared = cfg->q_heads != cfg->heads, k_shared = cfg->k_heads != cfg->heads,
+               v_shared = cfg->v_heads != cfg->heads;
+    Pass P = base_pass(cfg, log_decay, offsets);
+    double *parts_of_slope = (double *)(ws + w.slope);
+    P.seg = (float *)(ws + w.seg);
+    P.chunk_states = (float *)(ws + w.chunks);
+    if (grad_q || slope) {
+        Pass Q = P;
+        Q.a = vo; Q.b = vv; Q.c = vk; Q.e = vq;
+        Q.da = cfg->dv; Q.dc = cfg->dk; Q.st_a = 1; Q.st_c = cfg->dv;
+        Q.state_in = state_in; Q.slope = parts_of_slope; Q.out_scale = cfg->scale;
+        Q.out = !grad_q ? nullptr : q_shared ? (void *)parts : grad_q;
+        Q.out_f32 = q_shared;
+        if (int rc = enter_states<false>(cfg, Q, vec, st)) return rc;
+        if (int rc = launch(cfg, slope ? OUT_SLOPE : OUT, Q, vec, st)) return rc;
+        if (grad_q && q_shared)
+            if (int rc = share_sum(cfg, parts, grad_q, cfg->q_heads, cfg->dk, st)) return rc;
     }
-    if (grad_v || grad_k || grad_state_in) {
-        Pass P = base_pass(cfg, log_decay, offsets);
-        P.reverse = 1;
-        P.a = vk; P.b = vq; P.c = vo;
-        P.da = cfg->dk; P.dc = cfg->dv; P.st_a = cfg->dv; P.st_c = 1;
-        P.state_in = grad_state_out; P.upd_scale = cfg->scale;
-        P.seg = (float *)((char *)workspace + w.seg);
-        if (int rc = enter_states<false>(cfg, P, st)) return rc;
-        if (grad_v || grad_state_in) {
-            P.state_out = grad_state_in;
-            if (int rc = grad_pass(cfg, P, cfg->v_heads, cfg->dv, grad_v, parts, false, st)) return rc;
-        }
-        if (grad_k) {
-            P.state_out = nullptr;
-            P.a = vv; P.b = vo; P.c = vq;
-            P.da = cfg->dv; P.dc = cfg->dk; P.st_a = 1; P.st_c = cfg->dv;
-            if (int rc = grad_pass(cfg, P, cfg->k_heads, cfg->dk, grad_k, parts, false, st)) return rc;
-        }
+    if (grad_v || grad_k || grad_state_in || slope) {
+        Pass R = P;
+        R.a = vk; R.b = vq; R.c = vo; R.e = vv;
+        R.da = cfg->dk; R.dc = cfg->dv; R.st_a = cfg->dv; R.st_c = 1;
+        R.state_in = grad_state_out; R.state_out = grad_state_in; R.upd_scale = cfg->scale;
+        R.slope = parts_of_slope + (size_t)P.slots * cfg->heads;
+        R.out = !grad_v ? nullptr : v_shared ? (void *)parts : grad_v;
+        R.out_f32 = v_shared;
+        R.out2 = !grad_k ? nullptr : k_shared ? (void *)parts2 : grad_k;
+        R.out2_f32 = k_shared;
+        if (int rc = enter_states<true>(cfg, R, vec, st)) return rc;
+        if (int rc = launch(cfg, slope ? PAIR_SLOPE : PAIR, R, vec, st)) return rc;
+        if (grad_v && v_shared)
+            if (int rc = share_sum(cfg, parts, grad_v, cfg->v_heads, cfg->dv, st)) return rc;
+        if (grad_k && k_shared)
+            if (int rc = share_sum(cfg, parts2, grad_k, cfg->k_heads, cfg->dk, st)) return rc;
+    }
+    if (slope) {
+        hipLaunchKernelGGL(td_decay_slope_kernel, dim3(cfg->heads), dim3(256), 0, st, parts_of_slope, 2 * P.slots, cfg->heads, grad_log_decay);
+        TD_LAUNCH_CHECK();
     }
     return TD_OK;
 }

@@ -1,9 +1,10 @@
-// The chunked kernel of decay attention (decay_attn.hip has the formulas): a workgroup takes one sequence (or a segment of one) and
+// The chunked kernels of decay attention (decay_attn.hip has the formulas): a workgroup takes one sequence (or a segment of one) and
 // head, 64 rows at a time, and keeps the state in registers between the chunks.  With i, j rows of a chunk of n, F the state
 // entering it and X^T standing for a matrix with its columns in lanes,
 //     out_i = os (g^(i+1) F^T a_i + sum_{j<=i} g^(i-j) (b_j . a_i) us c_j),       F' = g^n F + sum_j g^(n-1-j) us b_j c_j^T
-// (reversed passes: out's exponent is one less, F's terms' one more).  Everything is 16 x 16 matrix tiles, and the order of an operand's
-// inner index is free as long as both operands share it, so that no product's result is ever moved between lanes:
+// (reversed passes: rows counted from the chunk's end, out's exponent one less, F's terms' one more).  Everything is 16 x 16 matrix
+// tiles, and the order of an operand's inner index is free as long as both operands share it, so that no product's result is ever
+// moved between lanes:
 //   * a wave owns 16 CT columns of c and of the state; the state's accumulators (rows = da in a lane's registers, lane = column) ARE
 //     the operand of F^T a, and the scores' accumulators (rows j in registers, lane = row i) the operand of the sum over j: the waves
 //     share out the ten score tiles on and below the diagonal and pass them on through LDS as operands, lane by lane;
@@ -18,6 +19,8 @@ namespace decay {
 
 constexpr int CHUNK = 64;
 
+enum Kind { OUT, OUT_SLOPE, SUM, SUM_REVERSED, PAIR, PAIR_SLOPE };      // td_decay_out_kernel, td_decay_sum_kernel, td_decay_pair_kernel
+
 struct View {                 // rows of one tensor; head h of the recurrence reads head h / share
     const void *p;
     int64_t seq, row, head;
@@ -25,18 +28,18 @@ struct View {                 // rows of one tensor; head h of the recurrence re
 };
 
 struct Pass {
-    View a, b, c, e;          // e: what the tangent's output is dotted with (tangent form only)
+    View a, b, c, e;          // OUT: out from (a, b, c), e: what the slope of out is dotted with.  PAIR: out from (a, b, c), out2 from (e, c, b)
     const float *log_decay;
     const int32_t *offsets;   // packed: n_seq + 1, else NULL
     const float *state_in;    // (n_seq, heads, ..): element (i, j) of (da, dc) at i * st_a + j * st_c, NULL: zeros
     float *state_out;         // NULL: not wanted
-    const float *grad_state;  // tangent form: the gradient of the state left behind, NULL: none
-    float *seg, *seg_tan;     // (slots, heads, ..) as state_in: the state (its tangent) entering each segment; SUM form: what each one adds
-    double *slope;            // tangent form: one sum for each (slot, head)
+    float *seg;               // (slots, heads, ..) as state_in: the state entering each segment; SUM: what each one adds
+    float *chunk_states;      // (chunks, heads, ..): the state entering each chunk, as the waves hold it; left by OUT_SLOPE for PAIR_SLOPE
+    double *slope;            // one sum for each (slot, head)
     int64_t st_a, st_c;
-    void *out;                // (rows, heads, dc), float32 (out_f32) or the tensors' type; NULL: not wanted
-    int out_f32;
-    int n_seq, rows, heads, da, dc, reverse;
+    void *out, *out2;         // (rows, heads, dc), (rows, heads, da), float32 (out_f32, out2_f32) or the tensors' type; NULL: not wanted
+    int out_f32, out2_f32;
+    int n_seq, rows, heads, da, dc;
     int seg_len, segs, slots; // rows of a segment (a multiple of CHUNK), segments of a dense sequence (1: seg_len covers all), slots in all
     float out_scale, upd_scale;
 };
@@ -51,9 +54,9 @@ __device__ __forceinline__ void row_range(const int32_t *offsets, int rows, int 
     }
 }
 
-// Packed sequence n owns the slots from lo(n) / seg_len + n on: a sequence of any length has as many as it has segments (one at least), no
-// two share one, and there are rows / seg_len + n_seq in all, whatever the lengths are.
-__device__ __forceinline__ int first_slot(const Pass &P, int n) { return min(max(P.offsets[n], 0), P.rows) / P.seg_len + n; }
+// Packed sequence n owns the places from lo(n) / size + n on, for segments (size = seg_len) as for chunks: a sequence of any length has as
+// many as it needs (one at least), no two share one, and there are rows / size + n_seq in all, whatever the lengths are.
+__device__ __forceinline__ int first_place(const Pass &P, int n, int size) { return min(max(P.offsets[n], 0), P.rows) / size + n; }
 
 // -> the sequence and segment of a slot; segment < 0 where it has none
 __device__ __forceinline__ void slot_owner(const Pass &P, int slot, int &n, int &segment) {
@@ -65,15 +68,24 @@ __device__ __forceinline__ void slot_owner(const Pass &P, int slot, int &n, int 
     int lo = 0, hi = P.n_seq - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
-        if (first_slot(P, mid) <= slot) lo = mid;
+        if (first_place(P, mid, P.seg_len) <= slot) lo = mid;
         else hi = mid - 1;
     }
     n = lo;
-    segment = slot - first_slot(P, lo);
+    segment = slot - first_place(P, lo, P.seg_len);
 }
 
 // g^e for a whole number e: 1 for e = 0, also where log g is -inf
 __device__ __forceinline__ float power(float lg2, int e) { return e == 0 ? 1.0f : __builtin_amdgcn_exp2f(lg2 * (float)e); }
+
+// g^e as two floats: it multiplies a state again and again, and its own rounding would add up over a long memory
+struct Factor { float hi, lo; };
+__device__ __forceinline__ Factor factor(float log_g, int e) {
+    const double x = e == 0 ? 1.0 : exp((double)log_g * e);
+    const float hi = (float)x;
+    return Factor{hi, isinf(hi) || hi == 0.0f ? 0.0f : (float)(x - (double)hi)};
+}
+__device__ __forceinline__ float times(Factor f, float x) { return f.hi * x + f.lo * x; }
 
 typedef __attribute__((__vector_size__(4 * sizeof(__bf16)))) __bf16 bf16x4;
 
@@ -145,19 +157,22 @@ template <> struct Mat<float> {
 
 // One chunk's rows of one tensor on their way from memory to LDS.  Memory is read in the order of its rows (n of them from `low` on), a
 // reversed pass turns them round in LDS.  VEC: 16 bytes a load, at 32-bit offsets from the chunk's first row, into registers that are filled
-// while the chunk before it is computed; else (odd sizes, strides or addresses) element by element when the chunk begins.
-template <typename T, int DP, int NT, bool VEC> struct Stage {
-    static constexpr int PER = Mat<T>::VEC, PIECES = DP / PER, N = VEC ? CHUNK * PIECES / NT : 1, LD = DP + PER;
+// while the chunk before it is computed (unless there are too many); else (odd sizes, strides or addresses) element by element when the
+// chunk begins.
+template <typename T, int D, int NT, bool VEC, bool REV> struct Stage {
+    static constexpr int PER = Mat<T>::VEC, PIECES = D / PER, N = VEC ? CHUNK * PIECES / NT : 1, LD = D + PER;
+    static constexpr bool AHEAD = VEC && N <= 4;
     static_assert(NT % PIECES == 0, "a thread's pieces share their columns");
-    uint4 r[N];
+    uint4 r[AHEAD ? N : 1];
     uint32_t at;              // byte offset of the first piece; the others are whole rows further on
     __device__ __forceinline__ void init(const View &v, int tid) {
         at = (uint32_t)(tid / PIECES) * (uint32_t)(v.row * sizeof(T)) + tid % PIECES * 16;
+        if (AHEAD)
 #pragma unroll
-        for (int c = 0; c < N; ++c) r[c] = uint4{0, 0, 0, 0};
+            for (int c = 0; c < N; ++c) r[c] = uint4{0, 0, 0, 0};
     }
     template <bool FULL> __device__ __forceinline__ void load(const T *base, const View &v, int low, int n, int tid) {
-        if (!VEC || tid % PIECES * PER >= v.d) return;
+        if (!AHEAD || tid % PIECES * PER >= v.d) return;
         const char *p = (const char *)(base + (int64_t)low * v.row);
         const int64_t by = NT / PIECES * v.row * (int64_t)sizeof(T);
 #pragma unroll
@@ -166,24 +181,29 @@ template <typename T, int DP, int NT, bool VEC> struct Stage {
             if (FULL || (tid + c * NT) / PIECES < n) r[c] = *(const uint4 *)(p + c * by + at);
         }
     }
-    template <bool FULL> __device__ __forceinline__ void store(T *lds, const T *base, const View &v, int low, int n, int reverse, int tid) const {
+    template <bool FULL> __device__ __forceinline__ void store(T *lds, const T *base, const View &v, int low, int n, int tid) const {
         if (!VEC) {
             const T *p = base + (int64_t)low * v.row;
 #pragma unroll 4
-            for (int i = tid; i < CHUNK * DP; i += NT) {
-                const int row = i / DP, col = i % DP, to = reverse && row < n ? n - 1 - row : row;
+            for (int i = tid; i < CHUNK * D; i += NT) {
+                const int row = i / D, col = i % D, to = REV && row < n ? n - 1 - row : row;
                 lds[to * LD + Mat<T>::place(col >> 2) + (col & 3)] = row < n && col < v.d ? p[row * v.row + col] : (T)0.0f;
             }
             return;
         }
+        const char *p = (const char *)(base + (int64_t)low * v.row);
+        const int64_t by = NT / PIECES * v.row * (int64_t)sizeof(T);
 #pragma unroll
         for (int c = 0; c < N; ++c) {
-            const int i = tid + c * NT, row = i / PIECES, piece = i % PIECES, to = reverse && (FULL || row < n) ? (FULL ? CHUNK : n) - 1 - row : row;
+            const int i = tid + c * NT, row = i / PIECES, piece = i % PIECES, to = REV && (FULL || row < n) ? (FULL ? CHUNK : n) - 1 - row : row;
+            uint4 x = uint4{0, 0, 0, 0};
+            if (AHEAD) x = r[AHEAD ? c : 0];
+            else if ((FULL || row < n) && piece * PER < v.d) x = *(const uint4 *)(p + c * by + at);
             if constexpr (PER == 8) {
-                *(uint2 *)(lds + to * LD + Mat<T>::place(2 * piece)) = uint2{r[c].x, r[c].y};
-                *(uint2 *)(lds + to * LD + Mat<T>::place(2 * piece + 1)) = uint2{r[c].z, r[c].w};
+                *(uint2 *)(lds + to * LD + Mat<T>::place(2 * piece)) = uint2{x.x, x.y};
+                *(uint2 *)(lds + to * LD + Mat<T>::place(2 * piece + 1)) = uint2{x.z, x.w};
             } else {
-                *(uint4 *)(lds + to * LD + Mat<T>::place(piece)) = r[c];
+                *(uint4 *)(lds + to * LD + Mat<T>::place(piece)) = x;
             }
         }
     }
@@ -193,27 +213,215 @@ template <typename T> __device__ __forceinline__ const T *base_of(const View &v,
     return (const T *)v.p + (packed ? 0 : n * v.seq) + (h / v.share) * v.head;
 }
 
-struct Yes { static constexpr bool value = true; };
-struct No { static constexpr bool value = false; };
+// Waits until the matrix instructions before it have written their results.  It stands wherever a branch (a loop's end, a store of some
+// lanes) comes between a matrix instruction and the first reader of its result: the compiler places the waits that the hardware
+// needs itself, but on some paths through a branch it has left them out (results of v_mfma_f32_16x16x4_f32 were read 1 instruction behind it
+// instead of 10).
+__device__ __forceinline__ void settle() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_nop 15");
+    __builtin_amdgcn_sched_barrier(0);
+}
 
-enum Form { OUT, OUT_TANGENT, SUM, SUM_TANGENT };   // an output (with the state's derivative by log g carried beside it); only what a segment adds
+// A chunk's rows: a whole chunk, or the last rows of a sequence, of which tiles of 16 there are at most LIVE.  (How many tiles a product covers is
+// a constant in each form: a branch on it would stand between a matrix instruction and the readers of its result.)
+template <int LIVE_, bool FULL_> struct Rows {
+    static constexpr int LIVE = LIVE_;
+    static constexpr bool FULL = FULL_;
+};
+typedef Rows<CHUNK / 16, true> Whole;
+typedef Rows<CHUNK / 16, false> Most;
+typedef Rows<CHUNK / 32, false> Half;
 
-// DP: da and dc padded to 32, 64 or 128.  NW waves of CT column tiles each: NW * CT * 16 = DP.  VEC: every tensor is read and written
-// 16 bytes (outputs: four values) at a time.
-template <typename T, int DP, int NW, int CT, bool VEC, Form FORM> struct Sweep {
+// Which segment of which sequence a workgroup has
+struct Place {
+    int n_seq, segment, lo, t0, t1;      // rows lo + t0 .. lo + t1 - 1
+    bool last;
+    __device__ __forceinline__ bool find(const Pass &P, int slot) {
+        int hi;
+        slot_owner(P, slot, n_seq, segment);
+        row_range(P.offsets, P.rows, n_seq, lo, hi);
+        t0 = segment * P.seg_len;
+        if (segment < 0 || (segment > 0 && t0 >= hi - lo)) return false;
+        last = hi - lo - t0 <= P.seg_len;
+        t1 = last ? hi - lo : t0 + P.seg_len;
+        return true;
+    }
+};
+
+// The weights of a head that every chunk uses
+template <int NW> struct Weights {
+    static constexpr int RT = CHUNK / 16, SCORES = RT * (RT + 1) / 2, MINE = (SCORES + NW - 1) / NW;   // score tiles; at most so many a wave
+    float lg2, wo, wu[4], wa[MINE][4], tiles[RT];
+    int it[MINE], jt[MINE];
+    Factor whole;
+    // late: 1 in reversed passes
+    __device__ __forceinline__ void init(float log_g, float scale, int late, int wave, int g, int li) {
+        lg2 = log_g * 1.44269504f;
+        whole = factor(log_g, CHUNK);
+        wo = power(lg2, li + 1 - late);                                             // of row i: g^(its place in its tile + 1), times
+#pragma unroll
+        for (int k = 0; k < RT; ++k) tiles[k] = power(lg2, 16 * k);                 // g^(16 tiles before its own)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) wu[r] = power(lg2, 15 - (g * 4 + r) + late) * scale;   // of row j in the state, likewise from the chunk's end
+#pragma unroll
+        for (int m = 0; m < MINE; ++m) {                                            // of this wave's score tiles: g^(i-j)
+            const int id = wave + NW * m;
+            it[m] = id >= SCORES ? RT : id < 1 ? 0 : id < 3 ? 1 : id < 6 ? 2 : 3;
+            jt[m] = id - it[m] * (it[m] + 1) / 2;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) wa[m][r] = apart(m, r, g, li) < 0 ? 0.0f : power(lg2, apart(m, r, g, li)) * scale;
+        }
+    }
+    __device__ __forceinline__ int apart(int m, int r, int g, int li) const { return (it[m] - jt[m]) * 16 + li - (g * 4 + r); }
+};
+
+// One product stream: the state M (DA x DC) and what a chunk does with it.  TA x CT tiles of the state a wave.
+template <typename T, int DA, int DC, int NW, bool VEC, int TERMS> struct Stream {
     typedef Mat<T> M;
     typedef typename M::Op Op;
-    static constexpr bool TAN = FORM == OUT_TANGENT || FORM == SUM_TANGENT, ADD = FORM == SUM || FORM == SUM_TANGENT;
-    static constexpr int NT = 64 * NW, LD = DP + M::VEC, TILES = DP / 16, KS = TILES / M::KT, RT = CHUNK / 16, KR = RT / M::KT;
-    static constexpr int S2 = M::SPLIT ? (TAN ? 3 : 2) : 1, S3 = M::SPLIT ? 3 : 1;
-    static constexpr int SCORES = RT * (RT + 1) / 2, MINE = (SCORES + NW - 1) / NW;             // score tiles; at most so many a wave
-    static constexpr int PAIRS = M::KT == 2 ? RT / 2 * (RT / 2 + 1) : SCORES;                     // score operands: (it, kr), kr <= it / KT
-    static constexpr int PIECE = CHUNK * LD;                                                      // one tensor's chunk in LDS
-    static constexpr size_t BYTES = (ADD ? 2 : TAN ? 4 : 3) * PIECE * sizeof(T) + (ADD ? 0 : PAIRS * 64 * 16 * S2 * (TAN ? 2 : 1));
-    static_assert(NW * CT == TILES, "every column tile has a wave");
+    static constexpr int LA = DA + M::VEC, LC = DC + M::VEC, TA = DA / 16, CT = DC / 16 / NW, KS = TA / M::KT, RT = CHUNK / 16, KR = RT / M::KT;
+    static constexpr int S2 = M::SPLIT ? 2 : 1, S3 = M::SPLIT ? 3 : 1, SF = M::SPLIT ? TERMS : 1;      // terms of scores, of decayed rows, of the state
+    static constexpr int PAIRS = M::KT == 2 ? RT / 2 * (RT / 2 + 1) : RT * (RT + 1) / 2;               // score operands: (it, kr), kr <= it / KT
+    static_assert(CT * NW * 16 == DC && CT > 0, "every column tile has a wave");
+    f32x4 S[TA][CT], o[RT][CT];
+    Op vt[CT][KR];
 
     static __device__ __forceinline__ int pair(int it, int kr) { return M::KT == 2 ? (it >> 1) * ((it >> 1) + 1) + (it & 1) * ((it >> 1) + 1) + kr : it * (it + 1) / 2 + kr; }
 
+    // the halves of score operands above the diagonal
+    static __device__ __forceinline__ void clear_scores(Op *scores, int lane) {
+        const Op zero = {};
+        if (M::KT == 2)
+#pragma unroll
+            for (int it = 0; it < RT; it += 2)
+#pragma unroll
+                for (int k = 0; k < S2; ++k) scores[(pair(it, it / 2) * S2 + k) * 64 + lane] = zero;
+    }
+    // (b_j . a_i) of tile (it, jt)
+    static __device__ __forceinline__ f32x4 score(const T *la, const T *lb, int it, int jt, int g, int li) {
+        f32x4 w = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int s = 0; s < KS; ++s) w = M::mma(M::row_op(lb, LA, jt * 16 + li, s, g), M::row_op(la, LA, it * 16 + li, s, g), w);
+        return w;
+    }
+    static __device__ __forceinline__ void keep(f32x4 w, Op *scores, int it, int jt, int lane) {
+        M::template keep<S2>(w, scores + pair(it, jt / M::KT) * S2 * 64 + lane, jt % M::KT);
+    }
+    __device__ __forceinline__ void enter(const float *from, int64_t st_a, int64_t st_c, int da, int dc, int wave, int g, int li) {
+#pragma unroll
+        for (int mt = 0; mt < TA; ++mt)
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) S[mt][ct] = f32x4{0, 0, 0, 0};
+        if (!from) return;
+#pragma unroll
+        for (int mt = 0; mt < TA; ++mt)
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int i = mt * 16 + g * 4 + r, j = (wave * CT + ct) * 16 + li;
+                    if (i < da && j < dc) S[mt][ct][r] = from[i * st_a + j * st_c];
+                }
+    }
+    __device__ __forceinline__ void leave(float *to, int64_t st_a, int64_t st_c, int da, int dc, int wave, int g, int li) const {
+        if (!to) return;
+#pragma unroll
+        for (int mt = 0; mt < TA; ++mt)
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int i = mt * 16 + g * 4 + r, j = (wave * CT + ct) * 16 + li;
+                    if (i < da && j < dc) to[i * st_a + j * st_c] = S[mt][ct][r];
+                }
+    }
+    // o = g^(i+1) F^T a
+    template <typename R, typename W> __device__ __forceinline__ void from_state(const T *la, int n, const W &w, int g, int li) {
+#pragma unroll
+        for (int it = 0; it < R::LIVE; ++it)
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) o[it][ct] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            Op f[CT][SF];
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) {
+                f32x4 part[M::KT];
+#pragma unroll
+                for (int k = 0; k < M::KT; ++k) part[k] = S[s * M::KT + k][ct];
+                M::template split<SF>(part, f[ct]);
+            }
+#pragma unroll
+            for (int it = 0; it < R::LIVE; ++it) {
+                const Op q = M::row_op(la, LA, it * 16 + li, s, g);
+#pragma unroll
+                for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+                    for (int k = 0; k < SF; ++k) o[it][ct] = M::mma(f[ct][k], q, o[it][ct]);
+            }
+        }
+#pragma unroll
+        for (int it = 0; it < R::LIVE; ++it)
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) o[it][ct] = o[it][ct] * (w.wo * w.tiles[it]);
+    }
+    // sum of (first + i) o_i . e_i over this lane's entries
+    template <typename R> __device__ __forceinline__ float dot(const T *le, int n, int first, int wave, int g, int li) const {
+        float sum = 0.0f;
+#pragma unroll
+        for (int it = 0; it < R::LIVE; ++it) {
+            float part = 0.0f;
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) {
+                const T *e = le + (it * 16 + li) * LC + M::place((wave * CT + ct) * 4 + g);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) part += o[it][ct][r] * (float)e[r];
+            }
+            sum += (float)(first + it * 16 + li) * part;
+        }
+        return sum;
+    }
+    __device__ __forceinline__ void columns(const T *lc, int wave, int g, int li) {
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+            for (int kr = 0; kr < KR; ++kr) vt[ct][kr] = M::col_op(lc, LC, wave * CT + ct, kr, g, li);
+    }
+    // o += the rows of this chunk; rows of o to memory
+    template <typename R, bool REV> __device__ __forceinline__ void from_rows(const Op *scores, int n, float scale, void *out, int out_f32, int64_t row0, int heads, int h, int dc,
+                                                                             int wave, int lane) {
+        if (!out) return;
+        const int g = lane >> 4, li = lane & 15;
+        const uint32_t by = (uint32_t)heads * dc;
+        const int64_t first = row0 * by + (int64_t)h * dc;
+#pragma unroll
+        for (int it = 0; it < R::LIVE; ++it)
+#pragma unroll
+            for (int kr = 0; kr <= it / M::KT; ++kr)
+#pragma unroll
+                for (int k = 0; k < S2; ++k) {
+                    const Op f = scores[(pair(it, kr) * S2 + k) * 64 + lane];
+#pragma unroll
+                    for (int ct = 0; ct < CT; ++ct) o[it][ct] = M::mma(vt[ct][kr], f, o[it][ct]);
+                }
+#pragma unroll
+        for (int it = 0; it < R::LIVE; ++it)
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) o[it][ct] = o[it][ct] * scale;
+#pragma unroll
+        for (int it = 0; it < R::LIVE; ++it) {
+            const int i = it * 16 + li;
+            if (!R::FULL && i >= n) continue;
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) {
+                const int col = (wave * CT + ct) * 16 + g * 4;
+                const uint32_t at = (uint32_t)(REV ? n - 1 - i : i) * by + col;
+                if (out_f32) put((float *)out + first, at, o[it][ct], dc - col);
+                else put((T *)out + first, at, o[it][ct], dc - col);
+            }
+        }
+    }
     // four columns of a row, `left` of them there
     template <typename U> static __device__ __forceinline__ void put(U *base, uint32_t at, f32x4 v, int left) {
         typedef __attribute__((__vector_size__(4 * sizeof(U)))) U U4;
@@ -226,334 +434,325 @@ template <typename T, int DP, int NW, int CT, bool VEC, Form FORM> struct Sweep 
                 if (r < left) to[r] = (U)v[r];
         }
     }
-
-    static __device__ __forceinline__ void run(const Pass &P, char *lds) {
-        T *const lb = (T *)lds, *const lc = lb + PIECE, *const la = lc + PIECE, *const le = la + PIECE;
-        Op *const scores = (Op *)(lb + (TAN ? 4 : 3) * PIECE), *const slopes = scores + PAIRS * 64 * S2;      // [pair][term][lane]
-        const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, li = lane & 15;
-        const int h = blockIdx.x % P.heads, slot = blockIdx.x / P.heads;
-        const bool packed = P.offsets != nullptr;
-        int n_seq, segment, lo, hi;
-        slot_owner(P, slot, n_seq, segment);
-        row_range(P.offsets, P.rows, n_seq, lo, hi);
-        const int len = hi - lo, t0 = segment * P.seg_len;
-        if (segment < 0 || (segment > 0 && t0 >= len)) {
-            if (FORM == OUT_TANGENT && tid == 0) P.slope[blockIdx.x] = 0.0;
-            return;
-        }
-        const bool last = len - t0 <= P.seg_len;
-        if (ADD && last) return;
-        const int t1 = last ? len : t0 + P.seg_len;
-        // row t of the recurrence is row lo + t, or hi - 1 - t of a reversed pass; so a chunk of n begins at row low(t, n) of memory
-        const auto low = [&](int t, int n) { return P.reverse ? hi - t - n : lo + t; };
-        const T *pa = base_of<T>(P.a, packed, n_seq, h), *pb = base_of<T>(P.b, packed, n_seq, h), *pc = base_of<T>(P.c, packed, n_seq, h);
-        const T *pe = FORM == OUT_TANGENT ? base_of<T>(P.e, packed, n_seq, h) : nullptr;
-        Stage<T, DP, NT, VEC> sa, sb, sc, se;
-        sb.init(P.b, tid);
-        sc.init(P.c, tid);
-        if (!ADD) sa.init(P.a, tid);
-        if (FORM == OUT_TANGENT) se.init(P.e, tid);
-        const auto fetch_as = [&](auto full, int t, int n) __attribute__((always_inline)) {
-            constexpr bool FULL = decltype(full)::value;
-            sb.template load<FULL>(pb, P.b, low(t, n), n, tid);
-            if (!ADD) sa.template load<FULL>(pa, P.a, low(t, n), n, tid);
-            sc.template load<FULL>(pc, P.c, low(t, n), n, tid);
-            if (FORM == OUT_TANGENT) se.template load<FULL>(pe, P.e, low(t, n), n, tid);
-        };
-        const auto fetch = [&](int t) __attribute__((always_inline)) {
-            if (t1 - t >= CHUNK) fetch_as(Yes(), t, CHUNK);
-            else if (t < t1) fetch_as(No(), t, t1 - t);
-        };
-        fetch(t0);
-
-        const float ld = P.log_decay[h], lg2 = ld * 1.44269504f;
-        const int late = P.reverse ? 1 : 0;
-        // g^64 as two floats: it multiplies the state once a chunk, and its own rounding would add up over a long memory
-        const double whole_d = exp((double)ld * CHUNK);
-        const float whole = (float)whole_d, whole_lo = isinf(whole) || whole == 0.0f ? 0.0f : (float)(whole_d - (double)whole);
-        // weights: g^(i-j) us of this wave's score tiles; of row j of a full chunk in the state, g^(15 - its place in its tile) us, its tile's
-        // factor beside it; g^(place of row i in its tile + 1), likewise
-        float wa[MINE][4], wu[4];
-        const float wo = power(lg2, li + 1 - late);
-        float tiles[RT];                         // g^(16 k)
+    // F' = g^n F + sum_j g^(n-1-j+late) us b_j c_j^T
+    template <typename R, typename W> __device__ __forceinline__ void advance(const T *lb, int n, const W &w, float scale, int late, int g, int li) {
+        const Factor f = R::FULL ? w.whole : Factor{power(w.lg2, n), 0.0f};
 #pragma unroll
-        for (int k = 0; k < RT; ++k) tiles[k] = power(lg2, 16 * k);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) wu[r] = power(lg2, 15 - (g * 4 + r) + late) * P.upd_scale;
-        int my_it[MINE], my_jt[MINE];
-#pragma unroll
-        for (int m = 0; m < MINE; ++m) {
-            const int id = wave + NW * m;
-            my_it[m] = id >= SCORES ? RT : id < 1 ? 0 : id < 3 ? 1 : id < 6 ? 2 : 3;
-            my_jt[m] = id - my_it[m] * (my_it[m] + 1) / 2;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int apart = (my_it[m] - my_jt[m]) * 16 + li - (g * 4 + r);
-                wa[m][r] = apart < 0 ? 0.0f : power(lg2, apart) * P.upd_scale;
-            }
-        }
-        if (!ADD && M::KT == 2 && wave == 0) {      // the halves of operands above the diagonal
-            const Op zero = {};
-#pragma unroll
-            for (int it = 0; it < RT; it += 2)
-#pragma unroll
-                for (int k = 0; k < S2; ++k) {
-                    scores[(pair(it, it / 2) * S2 + k) * 64 + lane] = zero;
-                    if (TAN) slopes[(pair(it, it / 2) * S2 + k) * 64 + lane] = zero;
-                }
-        }
-
-        f32x4 S[TILES][CT], H[TAN ? TILES : 1][CT];
-        const int64_t state_at = ((int64_t)n_seq * P.heads + h) * P.da * P.dc, seg_at = (int64_t)blockIdx.x * P.da * P.dc;
-        const float *enter = ADD ? nullptr : segment > 0 ? P.seg + seg_at : P.state_in ? P.state_in + state_at : nullptr;
-        const float *enter_tan = FORM == OUT_TANGENT && segment > 0 ? P.seg_tan + seg_at : nullptr;
-#pragma unroll
-        for (int mt = 0; mt < TILES; ++mt)
-#pragma unroll
-            for (int ct = 0; ct < CT; ++ct) {
-                S[mt][ct] = f32x4{0, 0, 0, 0};
-                if (TAN) H[mt][ct] = f32x4{0, 0, 0, 0};
-            }
-        if (enter) {
-#pragma unroll
-            for (int mt = 0; mt < TILES; ++mt)
-#pragma unroll
-                for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int i = mt * 16 + g * 4 + r, j = (wave * CT + ct) * 16 + li;
-                        if (i < P.da && j < P.dc) {
-                            S[mt][ct][r] = enter[i * P.st_a + j * P.st_c];
-                            if (TAN && enter_tan) H[mt][ct][r] = enter_tan[i * P.st_a + j * P.st_c];
-                        }
-                    }
-        }
-
-        double slope = 0.0;
-        const int64_t out_at = ((int64_t)(packed ? 0 : n_seq) * P.rows * P.heads + h) * P.dc;
-        T *const out = (T *)P.out + out_at;
-        float *const out_f32 = (float *)P.out + out_at;
-        const auto chunk = [&](auto full, int t, int n_) __attribute__((always_inline)) {
-            constexpr bool FULL = decltype(full)::value;
-            const int n = FULL ? CHUNK : n_;
-            sb.template store<FULL>(lb, pb, P.b, low(t, n), n, P.reverse, tid);
-            sc.template store<FULL>(lc, pc, P.c, low(t, n), n, P.reverse, tid);
-            if (!ADD) sa.template store<FULL>(la, pa, P.a, low(t, n), n, P.reverse, tid);
-            if (FORM == OUT_TANGENT) se.template store<FULL>(le, pe, P.e, low(t, n), n, P.reverse, tid);
-            __syncthreads();
-            if (FULL) fetch(t + CHUNK);
-
-            f32x4 o[RT][CT], x[TAN ? RT : 1][CT];
-            if constexpr (!ADD) {
-                // this wave's score tiles
-#pragma unroll
-                for (int m = 0; m < MINE; ++m) {
-                    const int it = my_it[m], jt = my_jt[m];
-                    if (it >= RT || (!FULL && it * 16 >= n)) continue;
-                    f32x4 w = f32x4{0, 0, 0, 0}, wx;
-#pragma unroll
-                    for (int s = 0; s < KS; ++s) w = M::mma(M::row_op(lb, LD, jt * 16 + li, s, g), M::row_op(la, LD, it * 16 + li, s, g), w);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        w[r] *= wa[m][r];
-                        if (TAN) wx[r] = w[r] * (float)((it - jt) * 16 + li - (g * 4 + r));
-                    }
-                    const int at = pair(it, jt / M::KT) * S2;
-                    M::template keep<S2>(w, scores + at * 64 + lane, jt % M::KT);
-                    if constexpr (TAN) M::template keep<S2>(wx, slopes + at * 64 + lane, jt % M::KT);
-                }
-                // F^T a
-#pragma unroll
-                for (int it = 0; it < RT; ++it)
-#pragma unroll
-                    for (int ct = 0; ct < CT; ++ct) {
-                        o[it][ct] = f32x4{0, 0, 0, 0};
-                        if (TAN) x[it][ct] = f32x4{0, 0, 0, 0};
-                    }
-#pragma unroll
-                for (int s = 0; s < KS; ++s) {
-                    Op f[CT][S2], ft[TAN ? CT : 1][S2];
-#pragma unroll
-                    for (int ct = 0; ct < CT; ++ct) {
-                        f32x4 part[M::KT];
-#pragma unroll
-                        for (int k = 0; k < M::KT; ++k) part[k] = S[s * M::KT + k][ct];
-                        M::template split<S2>(part, f[ct]);
-                        if constexpr (TAN) {
-#pragma unroll
-                            for (int k = 0; k < M::KT; ++k) part[k] = H[s * M::KT + k][ct];
-                            M::template split<S2>(part, ft[ct]);
-                        }
-                    }
-#pragma unroll
-                    for (int it = 0; it < RT; ++it) {
-                        if (!FULL && it * 16 >= n) break;
-                        const Op q = M::row_op(la, LD, it * 16 + li, s, g);
-#pragma unroll
-                        for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-                            for (int k = 0; k < S2; ++k) {
-                                o[it][ct] = M::mma(f[ct][k], q, o[it][ct]);
-                                if constexpr (TAN) x[it][ct] = M::mma(ft[ct][k], q, x[it][ct]);
-                            }
-                    }
-                }
-                __syncthreads();
-            }
-
-            Op vt[CT][KR];
+        for (int mt = 0; mt < TA; ++mt)
 #pragma unroll
             for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
-                for (int kr = 0; kr < KR; ++kr) vt[ct][kr] = M::col_op(lc, LD, wave * CT + ct, kr, g, li);
-
-            if constexpr (!ADD) {
-                // their weights, and the rows of this chunk
-                float dot = 0.0f;
+                for (int r = 0; r < 4; ++r) S[mt][ct][r] = times(f, S[mt][ct][r]);
 #pragma unroll
-                for (int it = 0; it < RT; ++it) {
-                    if (!FULL && it * 16 >= n) break;
-                    const float into = wo * tiles[it];
+        for (int kr = 0; kr < (R::LIVE + M::KT - 1) / M::KT; ++kr) {
+            float wr[M::KT][4];
 #pragma unroll
-                    for (int ct = 0; ct < CT; ++ct) {
-                        if constexpr (TAN) x[it][ct] = (x[it][ct] + o[it][ct] * (float)(it * 16 + li + 1)) * into;
-                        o[it][ct] = o[it][ct] * into;
-                    }
+            for (int k = 0; k < M::KT; ++k)
 #pragma unroll
-                    for (int kr = 0; kr <= it / M::KT; ++kr)
-#pragma unroll
-                        for (int k = 0; k < S2; ++k) {
-                            const int at = (pair(it, kr) * S2 + k) * 64 + lane;
-                            const Op f = scores[at];
-#pragma unroll
-                            for (int ct = 0; ct < CT; ++ct) o[it][ct] = M::mma(vt[ct][kr], f, o[it][ct]);
-                            if constexpr (TAN) {
-                                const Op fx = slopes[at];
-#pragma unroll
-                                for (int ct = 0; ct < CT; ++ct) x[it][ct] = M::mma(vt[ct][kr], fx, x[it][ct]);
-                            }
-                        }
-                    const int i = it * 16 + li;
-#pragma unroll
-                    for (int ct = 0; ct < CT; ++ct) {
-                        const int tile = wave * CT + ct, col = tile * 16 + g * 4;
-                        if constexpr (TAN) {
-                            const T *e = le + i * LD + M::place(tile * 4 + g);
-#pragma unroll
-                            for (int r = 0; r < 4; ++r) dot += x[it][ct][r] * (float)e[r];
-                        }
-                        if (!P.out || (!FULL && i >= n)) continue;
-                        const uint32_t by = (uint32_t)P.heads * P.dc, at = (P.reverse ? n - 1 - i : i) * by + col;
-                        const f32x4 v = o[it][ct] * P.out_scale;
-                        if (P.out_f32) put(out_f32 + (int64_t)low(t, n) * by, at, v, P.dc - col);
-                        else put(out + (int64_t)low(t, n) * by, at, v, P.dc - col);
-                    }
+                for (int r = 0; r < 4; ++r) {
+                    const int tile = kr * M::KT + k, j = tile * 16 + g * 4 + r;
+                    wr[k][r] = R::FULL ? w.wu[r] * w.tiles[RT - 1 - tile] : j < n ? power(w.lg2, n - 1 - j + late) * scale : 0.0f;
                 }
-                if (TAN) slope += (double)(dot * P.out_scale);
-            }
-
-            // F' = g^n F + sum_j g^(n-1-j) b_j c_j^T
-            const float decay = FULL ? whole : power(lg2, n), decay_lo = FULL ? whole_lo : 0.0f;
+            Op u[CT][S3];
 #pragma unroll
-            for (int mt = 0; mt < TILES; ++mt)
+            for (int ct = 0; ct < CT; ++ct) {
+                f32x4 y[M::KT];
+#pragma unroll
+                for (int k = 0; k < M::KT; ++k)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) y[k][r] = M::elem(vt[ct][kr], k, r) * wr[k][r];
+                M::template split<S3>(y, u[ct]);
+            }
+#pragma unroll
+            for (int mt = 0; mt < TA; ++mt) {
+                const Op b = M::col_op(lb, LA, mt, kr, g, li);
 #pragma unroll
                 for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        if (TAN) {
-                            const float y = H[mt][ct][r] + (float)n * S[mt][ct][r];
-                            H[mt][ct][r] = decay * y + decay_lo * y;
-                        }
-                        S[mt][ct][r] = decay * S[mt][ct][r] + decay_lo * S[mt][ct][r];
-                    }
-#pragma unroll
-            for (int kr = 0; kr < KR; ++kr) {
-                if (!FULL && kr * M::KT * 16 >= n) break;
-                float w[M::KT][4];
-                if (FULL) {
-#pragma unroll
-                    for (int k = 0; k < M::KT; ++k) {
-                        const float tile = tiles[RT - 1 - (kr * M::KT + k)];
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) w[k][r] = wu[r] * tile;
-                    }
-                } else {
-#pragma unroll
-                    for (int k = 0; k < M::KT; ++k)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const int j = (kr * M::KT + k) * 16 + g * 4 + r;
-                            w[k][r] = j < n ? power(lg2, n - 1 - j + late) * P.upd_scale : 0.0f;
-                        }
-                }
-                Op u[CT][S3], ux[TAN ? CT : 1][S3];
-#pragma unroll
-                for (int ct = 0; ct < CT; ++ct) {
-                    f32x4 y[M::KT], z[M::KT];
-#pragma unroll
-                    for (int k = 0; k < M::KT; ++k)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const int j = (kr * M::KT + k) * 16 + g * 4 + r;
-                            y[k][r] = M::elem(vt[ct][kr], k, r) * w[k][r];
-                            if (TAN) z[k][r] = y[k][r] * (float)(n - 1 - j);
-                        }
-                    M::template split<S3>(y, u[ct]);
-                    if constexpr (TAN) M::template split<S3>(z, ux[ct]);
-                }
-#pragma unroll
-                for (int mt = 0; mt < TILES; ++mt) {
-                    const Op b = M::col_op(lb, LD, mt, kr, g, li);
-#pragma unroll
-                    for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-                        for (int k = 0; k < S3; ++k) {
-                            S[mt][ct] = M::mma(b, u[ct][k], S[mt][ct]);
-                            if constexpr (TAN) H[mt][ct] = M::mma(b, ux[ct][k], H[mt][ct]);
-                        }
-                }
+                    for (int k = 0; k < S3; ++k) S[mt][ct] = M::mma(b, u[ct][k], S[mt][ct]);
             }
-            __syncthreads();
-        };
-        int t = t0;
-        for (; t1 - t >= CHUNK; t += CHUNK) chunk(Yes(), t, CHUNK);
-        if (t < t1) chunk(No(), t, t1 - t);
-
-        float *leave = ADD ? P.seg + seg_at : last && P.state_out ? P.state_out + state_at : nullptr;
-        float *leave_tan = FORM == SUM_TANGENT ? P.seg_tan + seg_at : nullptr;
-        const float *grad = FORM == OUT_TANGENT && last && P.grad_state ? P.grad_state + state_at : nullptr;
-        if (leave || grad) {
-#pragma unroll
-            for (int mt = 0; mt < TILES; ++mt)
-#pragma unroll
-                for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int i = mt * 16 + g * 4 + r, j = (wave * CT + ct) * 16 + li;
-                        if (i >= P.da || j >= P.dc) continue;
-                        const int64_t at = i * P.st_a + j * P.st_c;
-                        if (leave) leave[at] = S[mt][ct][r];
-                        if (TAN && leave_tan) leave_tan[at] = H[mt][ct][r];
-                        if (TAN && grad) slope += (double)(H[mt][ct][r] * grad[at]);
-                    }
         }
-        if constexpr (FORM == OUT_TANGENT) {
-            double *red = (double *)lds;
-            __syncthreads();
-            red[tid] = slope;
-            __syncthreads();
-            for (int o = NT / 2; o > 0; o >>= 1) {
-                if (tid < o) red[tid] += red[tid + o];
-                __syncthreads();
-            }
-            if (tid == 0) P.slope[blockIdx.x] = red[0];
-        }
+        settle();
     }
 };
 
-template <typename T, int DP, int NW, int CT, bool VEC, Form FORM, int WAVES> __global__ __launch_bounds__(64 * NW, WAVES) void td_decay_chunk_kernel(Pass P) {
-    __shared__ __align__(16) char lds[Sweep<T, DP, NW, CT, VEC, FORM>::BYTES];
-    Sweep<T, DP, NW, CT, VEC, FORM>::run(P, lds);
+// Rows of no sequence: zeros in head h's columns, shared out over the slots
+template <typename U> __device__ __forceinline__ void clear_rows(const Pass &P, U *out, int dc, int slot, int h, int tid, int nt) {
+    const int lo = min(max(P.offsets[0], 0), P.rows), hi = min(max(P.offsets[P.n_seq], lo), P.rows);
+    for (int i = slot; i < lo + P.rows - hi; i += P.slots)
+        for (int c = tid; c < dc; c += nt) out[((int64_t)(i < lo ? i : hi + i - lo) * P.heads + h) * dc + c] = (U)0.0f;
+}
+template <typename T> __device__ __forceinline__ void clear_rows_of(const Pass &P, void *out, int f32, int dc, int slot, int h, int tid, int nt) {
+    if (!out) return;
+    if (f32) clear_rows(P, (float *)out, dc, slot, h, tid, nt);
+    else clear_rows(P, (T *)out, dc, slot, h, tid, nt);
+}
+
+// The sum of a workgroup's values, in a fixed order
+template <int NT> __device__ __forceinline__ void workgroup_sum(double x, double *red, double *to, int tid) {
+    __syncthreads();
+    red[tid] = x;
+    __syncthreads();
+    for (int o = NT / 2; o > 0; o >>= 1) {
+        if (tid < o) red[tid] += red[tid + o];
+        __syncthreads();
+    }
+    if (tid == 0) *to = red[0];
+}
+
+__device__ __forceinline__ int64_t chunk_place(const Pass &P, int n_seq) {
+    return P.offsets ? first_place(P, n_seq, CHUNK) : (int64_t)n_seq * ((P.rows + CHUNK - 1) / CHUNK);
+}
+
+// What a segment adds to the state
+template <typename T, int DA, int DC, int NW, bool VEC, bool REV, int WAVES> __global__ __launch_bounds__(64 * NW, WAVES) void td_decay_sum_kernel(Pass P) {
+    typedef Stream<T, DA, DC, NW, VEC, 2> X;
+    constexpr int NT = 64 * NW;
+    __shared__ __align__(16) T lb[CHUNK * X::LA];
+    __shared__ __align__(16) T lc[CHUNK * X::LC];
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = (tid & 63) >> 4, li = tid & 15;
+    const int h = blockIdx.x % P.heads, slot = blockIdx.x / P.heads;
+    Place at;
+    if (!at.find(P, slot) || (REV ? at.segment == 0 : at.last)) return;      // nothing enters a segment from these
+    const T *pb = base_of<T>(P.b, P.offsets, at.n_seq, h) + (int64_t)at.lo * P.b.row, *pc = base_of<T>(P.c, P.offsets, at.n_seq, h) + (int64_t)at.lo * P.c.row;
+    Stage<T, DA, NT, VEC, REV> sb;
+    Stage<T, DC, NT, VEC, REV> sc;
+    sb.init(P.b, tid);
+    sc.init(P.c, tid);
+    const auto fetch = [&](auto rows, int t, int n) __attribute__((always_inline)) {
+        constexpr bool FULL = decltype(rows)::FULL;
+        sb.template load<FULL>(pb, P.b, t, n, tid);
+        sc.template load<FULL>(pc, P.c, t, n, tid);
+    };
+    const int whole = (at.t1 - at.t0) / CHUNK, tail = (at.t1 - at.t0) % CHUNK;
+    if (REV && tail) fetch(Most(), at.t1 - tail, tail);
+    else fetch(Whole(), REV ? at.t1 - CHUNK : at.t0, CHUNK);
+    Weights<NW> w;
+    w.init(P.log_decay[h], P.upd_scale, REV, wave, g, li);
+    X x;
+    x.enter(nullptr, 0, 0, 0, 0, wave, g, li);
+    const auto chunk = [&](auto rows, int t, int n, int next) __attribute__((always_inline)) {
+        typedef decltype(rows) R;
+        constexpr bool FULL = R::FULL;
+        sb.template store<FULL>(lb, pb, P.b, t, n, tid);
+        sc.template store<FULL>(lc, pc, P.c, t, n, tid);
+        __syncthreads();
+        if (next >= 0) fetch(Whole(), next, CHUNK);
+        x.columns(lc, wave, g, li);
+        x.template advance<R>(lb, n, w, P.upd_scale, REV, g, li);
+        __syncthreads();
+    };
+    const int before = whole ? at.t1 - tail - CHUNK : -1;
+    if (REV && tail > CHUNK / 2) chunk(Most(), at.t1 - tail, tail, before);
+    else if (REV && tail) chunk(Half(), at.t1 - tail, tail, before);
+    for (int c = 0; c < whole; ++c) {        // (a segment that is not the last has no tail)
+        const int t = REV ? at.t0 + (whole - 1 - c) * CHUNK : at.t0 + c * CHUNK;
+        chunk(Whole(), t, CHUNK, c + 1 < whole ? (REV ? t - CHUNK : t + CHUNK) : -1);
+    }
+    x.leave(P.seg + (int64_t)blockIdx.x * P.da * P.dc, P.st_a, P.st_c, P.da, P.dc, wave, g, li);
+}
+
+// out from (a, b, c), rows ascending.  SLOPE: the part of the derivative by log g that rows owe to the states entering their chunks, dotted with
+// e, and those states for the pass over the other gradients.
+template <typename T, int DA, int DC, int NW, bool VEC, bool SLOPE, int WAVES> __global__ __launch_bounds__(64 * NW, WAVES) void td_decay_out_kernel(Pass P) {
+    typedef Stream<T, DA, DC, NW, VEC, SLOPE ? 3 : 2> X;
+    typedef typename X::Op Op;
+    constexpr int NT = 64 * NW;
+    __shared__ __align__(16) T la[CHUNK * X::LA];
+    __shared__ __align__(16) T lb[CHUNK * X::LA];
+    __shared__ __align__(16) T lc[CHUNK * X::LC];
+    __shared__ __align__(16) T le[SLOPE ? CHUNK * X::LC : 8];
+    __shared__ __align__(16) Op scores[X::PAIRS * X::S2 * 64];
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, li = lane & 15;
+    const int h = blockIdx.x % P.heads, slot = blockIdx.x / P.heads;
+    const bool packed = P.offsets != nullptr;
+    if (packed) clear_rows_of<T>(P, P.out, P.out_f32, P.dc, slot, h, tid, NT);
+    Place at;
+    if (!at.find(P, slot)) {
+        if (SLOPE && tid == 0) P.slope[blockIdx.x] = 0.0;
+        return;
+    }
+    const T *pa = base_of<T>(P.a, packed, at.n_seq, h) + (int64_t)at.lo * P.a.row, *pb = base_of<T>(P.b, packed, at.n_seq, h) + (int64_t)at.lo * P.b.row;
+    const T *pc = base_of<T>(P.c, packed, at.n_seq, h) + (int64_t)at.lo * P.c.row;
+    const T *pe = SLOPE ? base_of<T>(P.e, packed, at.n_seq, h) + (int64_t)at.lo * P.e.row : nullptr;
+    Stage<T, DA, NT, VEC, false> sa, sb;
+    Stage<T, DC, NT, VEC, false> sc, se;
+    sa.init(P.a, tid);
+    sb.init(P.b, tid);
+    sc.init(P.c, tid);
+    if (SLOPE) se.init(P.e, tid);
+    const auto fetch = [&](int t) __attribute__((always_inline)) {
+        const auto load = [&](auto rows, int n) __attribute__((always_inline)) {
+            constexpr bool FULL = decltype(rows)::FULL;
+            sb.template load<FULL>(pb, P.b, t, n, tid);
+            sa.template load<FULL>(pa, P.a, t, n, tid);
+            sc.template load<FULL>(pc, P.c, t, n, tid);
+            if (SLOPE) se.template load<FULL>(pe, P.e, t, n, tid);
+        };
+        if (at.t1 - t >= CHUNK) load(Whole(), CHUNK);
+        else if (t < at.t1) load(Most(), at.t1 - t);
+    };
+    fetch(at.t0);
+    Weights<NW> w;
+    w.init(P.log_decay[h], P.upd_scale, 0, wave, g, li);
+    if (wave == 0) X::clear_scores(scores, lane);
+    const int64_t state_at = ((int64_t)at.n_seq * P.heads + h) * P.da * P.dc;
+    X x;
+    x.enter(at.segment > 0 ? P.seg + (int64_t)blockIdx.x * P.da * P.dc : P.state_in ? P.state_in + state_at : nullptr, P.st_a, P.st_c, P.da, P.dc, wave, g, li);
+    double slope = 0.0;
+    const auto chunk = [&](auto rows, int t, int n) __attribute__((always_inline)) {
+        typedef decltype(rows) R;
+        constexpr bool FULL = R::FULL;
+        sb.template store<FULL>(lb, pb, P.b, t, n, tid);
+        sa.template store<FULL>(la, pa, P.a, t, n, tid);
+        sc.template store<FULL>(lc, pc, P.c, t, n, tid);
+        if (SLOPE) se.template store<FULL>(le, pe, P.e, t, n, tid);
+        __syncthreads();
+        if (FULL) fetch(t + CHUNK);
+#pragma unroll
+        for (int m = 0; m < w.MINE; ++m) {
+            const int it = w.it[m], jt = w.jt[m];
+            if (it >= R::LIVE) continue;
+            f32x4 s = X::score(la, lb, it, jt, g, li);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[r] *= w.wa[m][r];
+            X::keep(s, scores, it, jt, lane);
+        }
+        if (SLOPE) {
+            f32x4 *to = (f32x4 *)P.chunk_states + ((((chunk_place(P, at.n_seq) + t / CHUNK) * P.heads + h) * NW + wave) * X::TA * X::CT) * 64 + lane;
+#pragma unroll
+            for (int mt = 0; mt < X::TA; ++mt)
+#pragma unroll
+                for (int ct = 0; ct < X::CT; ++ct) to[(mt * X::CT + ct) * 64] = x.S[mt][ct];
+        }
+        x.template from_state<R>(la, n, w, g, li);
+        if (SLOPE) slope += (double)(x.template dot<R>(le, n, 1, wave, g, li) * P.out_scale);
+        __syncthreads();
+        x.columns(lc, wave, g, li);
+        x.template from_rows<R, false>(scores, n, P.out_scale, P.out, P.out_f32, (packed ? 0 : (int64_t)at.n_seq * P.rows) + at.lo + t, P.heads, h, P.dc, wave, lane);
+        x.template advance<R>(lb, n, w, P.upd_scale, 0, g, li);
+        __syncthreads();
+    };
+    int t = at.t0;
+    for (; at.t1 - t >= CHUNK; t += CHUNK) chunk(Whole(), t, CHUNK);
+    if (at.t1 - t > CHUNK / 2) chunk(Most(), t, at.t1 - t);
+    else if (t < at.t1) chunk(Half(), t, at.t1 - t);
+    x.leave(at.last && P.state_out ? P.state_out + state_at : nullptr, P.st_a, P.st_c, P.da, P.dc, wave, g, li);
+    if (SLOPE) workgroup_sum<NT>(slope, (double *)scores, P.slope + blockIdx.x, tid);
+}
+
+// out from (a, b, c) and out2 from (e, c, b), rows descending: the gradients of v and k from (k, q, grad_o) and (v, grad_o, q).  SLOPE: the rest of
+// the derivative by log g: pairs of rows of one chunk; what a chunk's rows owe to the chunks behind it; and the chunk's own n rows, for every pair with one
+// row before and one behind it, which is n g^n <state entering the chunk, its gradient when it leaves>.
+template <typename T, int DK, int DV, int NW, bool VEC, bool SLOPE, int WAVES> __global__ __launch_bounds__(64 * NW, WAVES) void td_decay_pair_kernel(Pass P) {
+    typedef Stream<T, DK, DV, NW, VEC, 2> V;
+    typedef Stream<T, DV, DK, NW, VEC, SLOPE ? 3 : 2> K;
+    typedef typename V::Op Op;
+    constexpr int NT = 64 * NW;
+    __shared__ __align__(16) T lk[CHUNK * V::LA];
+    __shared__ __align__(16) T lq[CHUNK * V::LA];
+    __shared__ __align__(16) T lo[CHUNK * V::LC];
+    __shared__ __align__(16) T lv[CHUNK * V::LC];
+    __shared__ __align__(16) Op scores[2][V::PAIRS * V::S2 * 64];
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, li = lane & 15;
+    const int h = blockIdx.x % P.heads, slot = blockIdx.x / P.heads;
+    const bool packed = P.offsets != nullptr;
+    if (packed) {
+        clear_rows_of<T>(P, P.out, P.out_f32, P.dc, slot, h, tid, NT);
+        clear_rows_of<T>(P, P.out2, P.out2_f32, P.da, slot, h, tid, NT);
+    }
+    Place at;
+    if (!at.find(P, slot)) {
+        if (SLOPE && tid == 0) P.slope[blockIdx.x] = 0.0;
+        return;
+    }
+    const T *pk = base_of<T>(P.a, packed, at.n_seq, h) + (int64_t)at.lo * P.a.row, *pq = base_of<T>(P.b, packed, at.n_seq, h) + (int64_t)at.lo * P.b.row;
+    const T *po = base_of<T>(P.c, packed, at.n_seq, h) + (int64_t)at.lo * P.c.row, *pv = base_of<T>(P.e, packed, at.n_seq, h) + (int64_t)at.lo * P.e.row;
+    Stage<T, DK, NT, VEC, true> sk, sq;
+    Stage<T, DV, NT, VEC, true> so, sv;
+    sk.init(P.a, tid);
+    sq.init(P.b, tid);
+    so.init(P.c, tid);
+    sv.init(P.e, tid);
+    const auto fetch = [&](auto rows, int t, int n) __attribute__((always_inline)) {
+        constexpr bool FULL = decltype(rows)::FULL;
+        sk.template load<FULL>(pk, P.a, t, n, tid);
+        sq.template load<FULL>(pq, P.b, t, n, tid);
+        so.template load<FULL>(po, P.c, t, n, tid);
+        sv.template load<FULL>(pv, P.e, t, n, tid);
+    };
+    const int whole = (at.t1 - at.t0) / CHUNK, tail = (at.t1 - at.t0) % CHUNK;
+    if (tail) fetch(Most(), at.t1 - tail, tail);
+    else if (whole) fetch(Whole(), at.t1 - CHUNK, CHUNK);
+    Weights<NW> w;
+    w.init(P.log_decay[h], P.upd_scale, 1, wave, g, li);
+    if (wave == 0) {
+        V::clear_scores(scores[0], lane);
+        V::clear_scores(scores[1], lane);
+    }
+    const int64_t state_at = ((int64_t)at.n_seq * P.heads + h) * P.da * P.dc;
+    const float *from = !at.last ? P.seg + (int64_t)blockIdx.x * P.da * P.dc : P.state_in ? P.state_in + state_at : nullptr;
+    V xv;
+    K xk;
+    xv.enter(from, P.st_a, P.st_c, P.da, P.dc, wave, g, li);
+    xk.enter(from, P.st_c, P.st_a, P.dc, P.da, wave, g, li);
+    double slope = 0.0;
+    const auto chunk = [&](auto rows, int t, int n, int next) __attribute__((always_inline)) {
+        typedef decltype(rows) R;
+        constexpr bool FULL = R::FULL;
+        sk.template store<FULL>(lk, pk, P.a, t, n, tid);
+        sq.template store<FULL>(lq, pq, P.b, t, n, tid);
+        so.template store<FULL>(lo, po, P.c, t, n, tid);
+        sv.template store<FULL>(lv, pv, P.e, t, n, tid);
+        __syncthreads();
+        if (next >= 0) fetch(Whole(), next, CHUNK);
+        float sum = 0.0f;
+#pragma unroll
+        for (int m = 0; m < w.MINE; ++m) {
+            const int it = w.it[m], jt = w.jt[m];
+            if (it >= R::LIVE) continue;
+            f32x4 s1 = V::score(lk, lq, it, jt, g, li), s2 = K::score(lv, lo, it, jt, g, li);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                s1[r] *= w.wa[m][r];
+                if (SLOPE) sum += (float)w.apart(m, r, g, li) * s1[r] * s2[r];
+                s2[r] *= w.wa[m][r];
+            }
+            V::keep(s1, scores[0], it, jt, lane);
+            V::keep(s2, scores[1], it, jt, lane);
+        }
+        if (SLOPE) {
+            const f32x4 *from = (const f32x4 *)P.chunk_states + ((((chunk_place(P, at.n_seq) + t / CHUNK) * P.heads + h) * NW + wave) * K::TA * K::CT) * 64 + lane;
+            float cross = 0.0f;
+#pragma unroll
+            for (int mt = 0; mt < K::TA; ++mt)
+#pragma unroll
+                for (int ct = 0; ct < K::CT; ++ct) {
+                    const f32x4 F = from[(mt * K::CT + ct) * 64];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) cross += F[r] * xk.S[mt][ct][r];
+                }
+            sum += (float)n * power(w.lg2, n) * cross;
+        }
+        const int64_t row0 = (packed ? 0 : (int64_t)at.n_seq * P.rows) + at.lo + t;
+        xk.template from_state<R>(lv, n, w, g, li);
+        if (SLOPE) slope += (double)(sum + xk.template dot<R>(lk, n, 0, wave, g, li));
+        __syncthreads();
+        xk.columns(lq, wave, g, li);
+        xk.template from_rows<R, true>(scores[1], n, 1.0f, P.out2, P.out2_f32, row0, P.heads, h, P.da, wave, lane);
+        xk.template advance<R>(lo, n, w, P.upd_scale, 1, g, li);
+        xv.template from_state<R>(lk, n, w, g, li);
+        xv.columns(lo, wave, g, li);
+        xv.template from_rows<R, true>(scores[0], n, 1.0f, P.out, P.out_f32, row0, P.heads, h, P.dc, wave, lane);
+        xv.template advance<R>(lq, n, w, P.upd_scale, 1, g, li);
+        __syncthreads();
+    };
+    const int before = whole ? at.t1 - tail - CHUNK : -1;
+    if (tail > CHUNK / 2) chunk(Most(), at.t1 - tail, tail, before);
+    else if (tail) chunk(Half(), at.t1 - tail, tail, before);
+    for (int c = whole - 1; c >= 0; --c) chunk(Whole(), at.t0 + c * CHUNK, CHUNK, c > 0 ? at.t0 + (c - 1) * CHUNK : -1);
+    xv.leave(at.segment == 0 && P.state_out ? P.state_out + state_at : nullptr, P.st_a, P.st_c, P.da, P.dc, wave, g, li);
+    if (SLOPE) workgroup_sum<NT>(slope, (double *)scores, P.slope + blockIdx.x, tid);
 }
 
 }  // namespace decay

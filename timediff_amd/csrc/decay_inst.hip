@@ -1,0 +1,54 @@
+// One object per (element type, kernel) of decay attention: TD_INST_BF16 0 or 1, TD_INST_KIND as decay::Kind.
+#include "decay_chunk.h"
+
+using namespace decay;
+
+#define TD_CAT_(a, b, c) a##b##_##c
+#define TD_CAT(a, b, c) TD_CAT_(a, b, c)
+
+namespace {
+
+#if TD_INST_BF16
+typedef __bf16 T;
+#else
+typedef float T;
+#endif
+
+// waves a SIMD is to hold: what the registers of each size allow without spilling
+template <bool VEC, int DA, int DC> int launch(const Pass &P, hipStream_t st) {
+    constexpr int NW = DA == 32 ? 2 : 4, size = DA + DC;
+    const dim3 grid((unsigned)(P.slots * P.heads)), block(64 * NW);
+#if TD_INST_KIND == 0
+    hipLaunchKernelGGL((td_decay_out_kernel<T, DA, DC, NW, VEC, false, size <= 128 ? 3 : 2>), grid, block, 0, st, P);
+#elif TD_INST_KIND == 1
+    hipLaunchKernelGGL((td_decay_out_kernel<T, DA, DC, NW, VEC, true, size <= 64 ? 3 : size <= 128 ? 2 : 1>), grid, block, 0, st, P);
+#elif TD_INST_KIND == 2
+    hipLaunchKernelGGL((td_decay_sum_kernel<T, DA, DC, NW, VEC, false, size <= 128 ? 4 : 2>), grid, block, 0, st, P);
+#elif TD_INST_KIND == 3
+    hipLaunchKernelGGL((td_decay_sum_kernel<T, DA, DC, NW, VEC, true, size <= 128 ? 4 : 2>), grid, block, 0, st, P);
+#elif TD_INST_KIND == 4
+    hipLaunchKernelGGL((td_decay_pair_kernel<T, DA, DC, NW, VEC, false, size <= 128 ? 2 : 1>), grid, block, 0, st, P);
+#else
+    hipLaunchKernelGGL((td_decay_pair_kernel<T, DA, DC, NW, VEC, true, size <= 128 ? 2 : 1>), grid, block, 0, st, P);
+#endif
+    TD_LAUNCH_CHECK();
+    return TD_OK;
+}
+
+}  // namespace
+
+// (sizes that are not a multiple of 16 bytes take the nearest square: what they gain from fewer kernels they do not lose to padding, their
+// loads are the bound)
+int TD_CAT(td_decay_launch_, TD_INST_BF16, TD_INST_KIND)(const Pass &P, int vec, hipStream_t st) {
+    const int most = P.da > P.dc ? P.da : P.dc;
+    if (vec) {
+        if (most <= 32) return launch<true, 32, 32>(P, st);
+        if (most <= 64) return launch<true, 64, 64>(P, st);
+        if (P.da <= 64) return launch<true, 64, 128>(P, st);
+        if (P.dc <= 64) return launch<true, 128, 64>(P, st);
+        return launch<true, 128, 128>(P, st);
+    }
+    if (most <= 32) return launch<false, 32, 32>(P, st);
+    if (most <= 64) return launch<false, 64, 64>(P, st);
+    return launch<false, 128, 128>(P, st);
+}
