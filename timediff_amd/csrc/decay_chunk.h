@@ -87,8 +87,6 @@ __device__ __forceinline__ Factor factor(float log_g, int e) {
 }
 __device__ __forceinline__ float times(Factor f, float x) { return f.hi * x + f.lo * x; }
 
-typedef __attribute__((__vector_size__(4 * sizeof(__bf16)))) __bf16 bf16x4;
-
 template <typename T> struct Mat;
 template <> struct Mat<__bf16> {
     typedef bf16x8 Op;
@@ -108,29 +106,36 @@ template <> struct Mat<__bf16> {
         x.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)(void *)(p + 16 * ld));
         return x.o;
     }
+    // two values to bf16 (one instruction); what is left of them behind
+    static __device__ __forceinline__ uint32_t term(float &a, float &b, bool last) {
+        typedef __attribute__((ext_vector_type(2))) float f32x2;
+        typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+        const uint32_t bits = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf16x2));
+        if (!last) {
+            a -= __uint_as_float(bits << 16);
+            b -= __uint_as_float(bits & 0xFFFF0000u);
+        }
+        return bits;
+    }
     // the operand whose elements are x[tile][register]
     template <int N> static __device__ __forceinline__ void split(const f32x4 *x, Op *p) {
+        union { uint32_t u[4]; Op o; } y[N];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            float v = x[j >> 2][j & 3];
+        for (int j = 0; j < 4; ++j) {
+            float a = x[j >> 1][2 * j & 3], b = x[j >> 1][(2 * j & 3) + 1];
 #pragma unroll
-            for (int k = 0; k < N; ++k) {
-                p[k][j] = (__bf16)v;
-                v -= (float)p[k][j];
-            }
+            for (int k = 0; k < N; ++k) y[k].u[j] = term(a, b, k == N - 1);
         }
+#pragma unroll
+        for (int k = 0; k < N; ++k) p[k] = y[k].o;
     }
     // one tile's terms into its half of the operands at to, to + 64, ..
     template <int N> static __device__ __forceinline__ void keep(f32x4 x, Op *to, int half) {
+        float a = x[0], b = x[1], c = x[2], d = x[3];
 #pragma unroll
         for (int k = 0; k < N; ++k) {
-            bf16x4 y;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                y[r] = (__bf16)x[r];
-                x[r] -= (float)y[r];
-            }
-            *((bf16x4 *)(to + 64 * k) + half) = y;
+            const uint32_t low = term(a, b, k == N - 1), high = term(c, d, k == N - 1);
+            *((uint2 *)(to + 64 * k) + half) = uint2{low, high};
         }
     }
     static __device__ __forceinline__ float elem(Op o, int tile, int r) { return (float)o[tile * 4 + r]; }
@@ -212,6 +217,16 @@ template <typename T, int D, int NT, bool VEC, bool REV> struct Stage {
 template <typename T> __device__ __forceinline__ const T *base_of(const View &v, bool packed, int n, int h) {
     return (const T *)v.p + (packed ? 0 : n * v.seq) + (h / v.share) * v.head;
 }
+
+// The thread's number as if read anew: what is computed from it (addresses in LDS and in memory, places in a tile) is computed again where it
+// is used.  Kept from chunk to chunk, as the compiler would, it fills the registers twice over.
+__device__ __forceinline__ int here(int tid) {
+    asm volatile("" : "+v"(tid));
+    return tid;
+}
+
+// Loads of what comes behind stay behind: the registers of two steps at once do not fit
+__device__ __forceinline__ void phase() { __builtin_amdgcn_sched_barrier(0); }
 
 // Waits until the matrix instructions before it have written their results.  It stands wherever a branch (a loop's end, a store of some
 // lanes) comes between a matrix instruction and the first reader of its result: the compiler places the waits that the hardware
@@ -510,7 +525,7 @@ template <typename T, int DA, int DC, int NW, bool VEC, bool REV, int WAVES> __g
     constexpr int NT = 64 * NW;
     __shared__ __align__(16) T lb[CHUNK * X::LA];
     __shared__ __align__(16) T lc[CHUNK * X::LC];
-    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = (tid & 63) >> 4, li = tid & 15;
+    const int tid_ = threadIdx.x, tid = tid_, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = (tid & 63) >> 4, li = tid & 15;
     const int h = blockIdx.x % P.heads, slot = blockIdx.x / P.heads;
     Place at;
     if (!at.find(P, slot) || (REV ? at.segment == 0 : at.last)) return;      // nothing enters a segment from these
@@ -534,6 +549,7 @@ template <typename T, int DA, int DC, int NW, bool VEC, bool REV, int WAVES> __g
     const auto chunk = [&](auto rows, int t, int n, int next) __attribute__((always_inline)) {
         typedef decltype(rows) R;
         constexpr bool FULL = R::FULL;
+        const int tid = here(tid_), lane = tid & 63, g = lane >> 4, li = lane & 15;
         sb.template store<FULL>(lb, pb, P.b, t, n, tid);
         sc.template store<FULL>(lc, pc, P.c, t, n, tid);
         __syncthreads();
@@ -563,7 +579,7 @@ template <typename T, int DA, int DC, int NW, bool VEC, bool SLOPE, int WAVES> _
     __shared__ __align__(16) T lc[CHUNK * X::LC];
     __shared__ __align__(16) T le[SLOPE ? CHUNK * X::LC : 8];
     __shared__ __align__(16) Op scores[X::PAIRS * X::S2 * 64];
-    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, li = lane & 15;
+    const int tid_ = threadIdx.x, tid = tid_, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, li = lane & 15;
     const int h = blockIdx.x % P.heads, slot = blockIdx.x / P.heads;
     const bool packed = P.offsets != nullptr;
     if (packed) clear_rows_of<T>(P, P.out, P.out_f32, P.dc, slot, h, tid, NT);
@@ -603,6 +619,7 @@ template <typename T, int DA, int DC, int NW, bool VEC, bool SLOPE, int WAVES> _
     const auto chunk = [&](auto rows, int t, int n) __attribute__((always_inline)) {
         typedef decltype(rows) R;
         constexpr bool FULL = R::FULL;
+        const int tid = here(tid_), lane = tid & 63, g = lane >> 4, li = lane & 15;
         sb.template store<FULL>(lb, pb, P.b, t, n, tid);
         sa.template store<FULL>(la, pa, P.a, t, n, tid);
         sc.template store<FULL>(lc, pc, P.c, t, n, tid);
@@ -625,11 +642,14 @@ template <typename T, int DA, int DC, int NW, bool VEC, bool SLOPE, int WAVES> _
 #pragma unroll
                 for (int ct = 0; ct < X::CT; ++ct) to[(mt * X::CT + ct) * 64] = x.S[mt][ct];
         }
+        phase();
         x.template from_state<R>(la, n, w, g, li);
         if (SLOPE) slope += (double)(x.template dot<R>(le, n, 1, wave, g, li) * P.out_scale);
         __syncthreads();
+        phase();
         x.columns(lc, wave, g, li);
         x.template from_rows<R, false>(scores, n, P.out_scale, P.out, P.out_f32, (packed ? 0 : (int64_t)at.n_seq * P.rows) + at.lo + t, P.heads, h, P.dc, wave, lane);
+        phase();
         x.template advance<R>(lb, n, w, P.upd_scale, 0, g, li);
         __syncthreads();
     };
@@ -654,7 +674,7 @@ template <typename T, int DK, int DV, int NW, bool VEC, bool SLOPE, int WAVES> _
     __shared__ __align__(16) T lo[CHUNK * V::LC];
     __shared__ __align__(16) T lv[CHUNK * V::LC];
     __shared__ __align__(16) Op scores[2][V::PAIRS * V::S2 * 64];
-    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, li = lane & 15;
+    const int tid_ = threadIdx.x, tid = tid_, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, li = lane & 15;
     const int h = blockIdx.x % P.heads, slot = blockIdx.x / P.heads;
     const bool packed = P.offsets != nullptr;
     if (packed) {
@@ -700,6 +720,7 @@ template <typename T, int DK, int DV, int NW, bool VEC, bool SLOPE, int WAVES> _
     const auto chunk = [&](auto rows, int t, int n, int next) __attribute__((always_inline)) {
         typedef decltype(rows) R;
         constexpr bool FULL = R::FULL;
+        const int tid = here(tid_), lane = tid & 63, g = lane >> 4, li = lane & 15;
         sk.template store<FULL>(lk, pk, P.a, t, n, tid);
         sq.template store<FULL>(lq, pq, P.b, t, n, tid);
         so.template store<FULL>(lo, po, P.c, t, n, tid);
@@ -721,6 +742,7 @@ template <typename T, int DK, int DV, int NW, bool VEC, bool SLOPE, int WAVES> _
             V::keep(s1, scores[0], it, jt, lane);
             V::keep(s2, scores[1], it, jt, lane);
         }
+        phase();
         if (SLOPE) {
             const f32x4 *from = (const f32x4 *)P.chunk_states + ((((chunk_place(P, at.n_seq) + t / CHUNK) * P.heads + h) * NW + wave) * K::TA * K::CT) * 64 + lane;
             float cross = 0.0f;
@@ -735,15 +757,20 @@ template <typename T, int DK, int DV, int NW, bool VEC, bool SLOPE, int WAVES> _
             sum += (float)n * power(w.lg2, n) * cross;
         }
         const int64_t row0 = (packed ? 0 : (int64_t)at.n_seq * P.rows) + at.lo + t;
+        phase();
         xk.template from_state<R>(lv, n, w, g, li);
         if (SLOPE) slope += (double)(sum + xk.template dot<R>(lk, n, 0, wave, g, li));
         __syncthreads();
+        phase();
         xk.columns(lq, wave, g, li);
         xk.template from_rows<R, true>(scores[1], n, 1.0f, P.out2, P.out2_f32, row0, P.heads, h, P.da, wave, lane);
+        phase();
         xk.template advance<R>(lo, n, w, P.upd_scale, 1, g, li);
         xv.template from_state<R>(lk, n, w, g, li);
+        phase();
         xv.columns(lo, wave, g, li);
         xv.template from_rows<R, true>(scores[0], n, 1.0f, P.out, P.out_f32, row0, P.heads, h, P.dc, wave, lane);
+        phase();
         xv.template advance<R>(lq, n, w, P.upd_scale, 1, g, li);
         __syncthreads();
     };
