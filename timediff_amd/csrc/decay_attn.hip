@@ -17,9 +17,9 @@ using namespace decay;
 
 // decay_inst.hip: one launcher per (element type, kernel)
 #define TD_LAUNCHERS(b)                                                                                                              \
-    int td_decay_launch_##b##_0(const Pass &, int, hipStream_t); int td_decay_launch_##b##_1(const Pass &, int, hipStream_t);       \
-    int td_decay_launch_##b##_2(const Pass &, int, hipStream_t); int td_decay_launch_##b##_3(const Pass &, int, hipStream_t);       \
-    int td_decay_launch_##b##_4(const Pass &, int, hipStream_t); int td_decay_launch_##b##_5(const Pass &, int, hipStream_t);
+    int td_decay_launch_##b##_0(const Work &, int, hipStream_t); int td_decay_launch_##b##_1(const Work &, int, hipStream_t);       \
+    int td_decay_launch_##b##_2(const Work &, int, hipStream_t); int td_decay_launch_##b##_3(const Work &, int, hipStream_t);       \
+    int td_decay_launch_##b##_4(const Work &, int, hipStream_t);
 TD_LAUNCHERS(0)
 TD_LAUNCHERS(1)
 
@@ -136,11 +136,11 @@ int esize(const td_decay_config *c) { return c->dtype == TD_BF16 ? 2 : 4; }
 
 View view(const td_decay_config *c, const void *p, const int64_t *s, int own, int d) { return View{p, s[0], s[1], s[2], c->heads / own, d}; }
 
-// Whether a tensor can be read 16 bytes at a time, a chunk's rows at 32-bit offsets from its first
+// Whether a tensor can be read 16 bytes at a time, a chunk's rows at 32-bit offsets from its first (24 bits of row stride)
 bool wide(const td_decay_config *c, const View &v) {
     const int64_t per = 16 / esize(c);
     return (uintptr_t)v.p % 16 == 0 && v.d % per == 0 && v.seq % per == 0 && v.row % per == 0 && v.head % per == 0 && v.row >= 0 &&
-           v.row < (1LL << 31) / CHUNK / 4;
+           v.row * esize(c) < (1 << 24);
 }
 
 // Segments: a sequence on its own is one after another, chunk by chunk, so few long ones are cut until there are workgroups for the chip (512: two
@@ -175,13 +175,21 @@ Pass base_pass(const td_decay_config *c, const float *log_decay, const int32_t *
     return P;
 }
 
-int launch(const td_decay_config *c, Kind kind, const Pass &P, bool vec, hipStream_t st) {
-    typedef int (*Launcher)(const Pass &, int, hipStream_t);
-    static const Launcher table[2][6] = {
-        {td_decay_launch_0_0, td_decay_launch_0_1, td_decay_launch_0_2, td_decay_launch_0_3, td_decay_launch_0_4, td_decay_launch_0_5},
-        {td_decay_launch_1_0, td_decay_launch_1_1, td_decay_launch_1_2, td_decay_launch_1_3, td_decay_launch_1_4, td_decay_launch_1_5}};
-    return table[c->dtype == TD_BF16][kind](P, vec, st);
+int launch(const td_decay_config *c, Kind kind, const Work &w, bool vec, hipStream_t st) {
+    typedef int (*Launcher)(const Work &, int, hipStream_t);
+    static const Launcher table[2][5] = {
+        {td_decay_launch_0_0, td_decay_launch_0_1, td_decay_launch_0_2, td_decay_launch_0_3, td_decay_launch_0_4},
+        {td_decay_launch_1_0, td_decay_launch_1_1, td_decay_launch_1_2, td_decay_launch_1_3, td_decay_launch_1_4}};
+    return table[c->dtype == TD_BF16][kind](w, vec, st);
 }
+int launch(const td_decay_config *c, Kind kind, const Pass &P, bool vec, hipStream_t st) {
+    Work w = {};
+    w.p = P;
+    return launch(c, kind, w, vec, st);
+}
+
+// Workgroups of the backward pass: as many as the chip holds (two a compute unit), each with its own place for the states of a segment's chunks
+int backward_groups(int64_t slots, int heads) { return (int)(slots * heads < 512 ? slots * heads : 512); }
 
 // What the segments add, and the state that enters each of them (nothing to do where every sequence is one segment)
 template <bool REV> int enter_states(const td_decay_config *c, const Pass &P, bool vec, hipStream_t st) {
@@ -206,26 +214,23 @@ int share_sum(const td_decay_config *c, const float *parts, void *grad, int own_
     return TD_OK;
 }
 
-struct Layout { size_t seg, chunks, slope, parts, parts2, total; };
+struct Layout { size_t seg, seg2, chunks, slope, parts, parts2, total; };
 Layout layout(const td_decay_config *c, bool backward) {
     int len, segs;
     int64_t slots;
     split(c, len, segs, slots);
     const size_t state = (size_t)c->heads * c->dk * c->dv * sizeof(float), rows = (size_t)total_rows(c) * c->heads * sizeof(float);
-    // the waves hold states of whole tiles: at most 32 x 32, else multiples of 64
-    const auto pad = [](int d, int most) { return most <= 32 ? 32 : d <= 64 ? 64 : 128; };
-    const int most = c->dk > c->dv ? c->dk : c->dv;
-    const bool square = most > 64;        // unaligned tensors take the larger side for both
-    const size_t held = (size_t)c->heads * (square ? 128 : pad(c->dk, most)) * (square ? 128 : pad(c->dv, most)) * sizeof(float);
-    const size_t chunks = c->packed ? (size_t)c->rows / CHUNK + c->n_seq : (size_t)c->n_seq * ((c->rows + CHUNK - 1) / CHUNK);
+    const int most = c->dk > c->dv ? c->dk : c->dv, side = most <= 32 ? 32 : most <= 64 ? 64 : 128;
+    const size_t held = (size_t)side * side * sizeof(float) * ((len + CHUNK - 1) / CHUNK);
     Layout w;
     w.seg = 0;
-    w.chunks = segs == 1 ? 0 : up256(slots * state);
-    w.slope = w.chunks + (backward ? chunks * held : 0);
+    w.seg2 = segs == 1 ? 0 : up256(slots * state);
+    w.chunks = w.seg2 + (backward && segs != 1 ? up256(slots * state) : 0);
+    w.slope = w.chunks + (backward ? held * backward_groups(slots, c->heads) : 0);
     w.parts = w.slope + (backward ? up256(2 * (size_t)slots * c->heads * sizeof(double)) : 0);
-    const bool qv = c->q_heads != c->heads || c->v_heads != c->heads, k = c->k_heads != c->heads;
-    w.parts2 = w.parts + (backward && qv ? up256(rows * most) : 0);
-    w.total = w.parts2 + (backward && k ? up256(rows * c->dk) : 0) + 256;
+    const bool q = c->q_heads != c->heads, k = c->k_heads != c->heads, v = c->v_heads != c->heads;
+    w.parts2 = w.parts + (backward && q ? up256(rows * c->dk) : 0);
+    w.total = w.parts2 + (backward ? (k ? up256(rows * c->dk) : 0) + (v ? up256(rows * c->dv) : 0) : 0) + 256;
     return w;
 }
 
@@ -265,50 +270,52 @@ extern "C" int td_decay_backward(const td_decay_config *cfg, const void *q, cons
     TD_REQUIRE(log_decay && workspace && (cfg->rows == 0 || (q && k && v && grad_o)), "null pointer");
     TD_REQUIRE(!cfg->packed || offsets, "packed sequences need offsets");
     hipStream_t st = (hipStream_t)stream;
-    const Layout w = layout(cfg, true);
+    const Layout l = layout(cfg, true);
     char *ws = (char *)workspace;
-    float *parts = (float *)(ws + w.parts), *parts2 = (float *)(ws + w.parts2);
+    const bool q_shared = cfg->q_heads != cfg->heads, k_shared = cfg->k_heads != cfg->heads, v_shared = cfg->v_heads != cfg->heads;
+    float *parts_q = (float *)(ws + l.parts), *parts_k = (float *)(ws + l.parts2);
+    float *parts_v = (float *)(ws + l.parts2 + (k_shared ? up256((size_t)total_rows(cfg) * cfg->heads * cfg->dk * sizeof(float)) : 0));
     const View vq = view(cfg, q, cfg->q_stride, cfg->q_heads, cfg->dk), vk = view(cfg, k, cfg->k_stride, cfg->k_heads, cfg->dk),
                vv = view(cfg, v, cfg->v_stride, cfg->v_heads, cfg->dv), vo = view(cfg, grad_o, cfg->grad_o_stride, cfg->heads, cfg->dv);
-    // one answer for every kernel of the call: the states that one leaves for another are laid out by it
     const bool vec = wide(cfg, vq) && wide(cfg, vk) && wide(cfg, vv) && wide(cfg, vo) && aligned(grad_q) && aligned(grad_k) && aligned(grad_v);
-    const bool slope = grad_log_decay != nullptr, q_shared = cfg->q_heads != cfg->heads, k_shared = cfg->k_heads != cfg->heads,
-               v_shared = cfg->v_heads != cfg->heads;
-    Pass P = base_pass(cfg, log_decay, offsets);
-    double *parts_of_slope = (double *)(ws + w.slope);
-    P.seg = (float *)(ws + w.seg);
-    P.chunk_states = (float *)(ws + w.chunks);
-    if (grad_q || slope) {
-        Pass Q = P;
-        Q.a = vo; Q.b = vv; Q.c = vk; Q.e = vq;
-        Q.da = cfg->dv; Q.dc = cfg->dk; Q.st_a = 1; Q.st_c = cfg->dv;
-        Q.state_in = state_in; Q.slope = parts_of_slope; Q.out_scale = cfg->scale;
-        Q.out = !grad_q ? nullptr : q_shared ? (void *)parts : grad_q;
-        Q.out_f32 = q_shared;
+    const bool slope = grad_log_decay != nullptr;
+    Work w = {};
+    w.chunk_states = (float *)(ws + l.chunks);
+    w.ascending = grad_q || slope;
+    w.descending = grad_v || grad_k || grad_state_in || slope;
+    Pass &Q = w.p, &R = w.r;
+    Q = R = base_pass(cfg, log_decay, offsets);
+    w.groups = backward_groups(Q.slots, cfg->heads);
+    double *slopes = (double *)(ws + l.slope);
+    Q.a = vo; Q.b = vv; Q.c = vk; Q.e = vq;
+    Q.da = cfg->dv; Q.dc = cfg->dk; Q.st_a = 1; Q.st_c = cfg->dv;
+    Q.state_in = state_in; Q.slope = slopes; Q.out_scale = cfg->scale;
+    Q.out = !grad_q ? nullptr : q_shared ? (void *)parts_q : grad_q;
+    Q.out_f32 = q_shared;
+    Q.seg = (float *)(ws + l.seg);
+    R.a = vk; R.b = vq; R.c = vo; R.e = vv;
+    R.da = cfg->dk; R.dc = cfg->dv; R.st_a = cfg->dv; R.st_c = 1;
+    R.state_in = grad_state_out; R.state_out = grad_state_in; R.upd_scale = cfg->scale;
+    R.slope = slopes + (size_t)R.slots * cfg->heads;
+    R.out = !grad_v ? nullptr : v_shared ? (void *)parts_v : grad_v;
+    R.out_f32 = v_shared;
+    R.out2 = !grad_k ? nullptr : k_shared ? (void *)parts_k : grad_k;
+    R.out2_f32 = k_shared;
+    R.seg = (float *)(ws + l.seg2);
+    if (w.ascending)
         if (int rc = enter_states<false>(cfg, Q, vec, st)) return rc;
-        if (int rc = launch(cfg, slope ? OUT_SLOPE : OUT, Q, vec, st)) return rc;
-        if (grad_q && q_shared)
-            if (int rc = share_sum(cfg, parts, grad_q, cfg->q_heads, cfg->dk, st)) return rc;
-    }
-    if (grad_v || grad_k || grad_state_in || slope) {
-        Pass R = P;
-        R.a = vk; R.b = vq; R.c = vo; R.e = vv;
-        R.da = cfg->dk; R.dc = cfg->dv; R.st_a = cfg->dv; R.st_c = 1;
-        R.state_in = grad_state_out; R.state_out = grad_state_in; R.upd_scale = cfg->scale;
-        R.slope = parts_of_slope + (size_t)P.slots * cfg->heads;
-        R.out = !grad_v ? nullptr : v_shared ? (void *)parts : grad_v;
-        R.out_f32 = v_shared;
-        R.out2 = !grad_k ? nullptr : k_shared ? (void *)parts2 : grad_k;
-        R.out2_f32 = k_shared;
+    if (w.descending)
         if (int rc = enter_states<true>(cfg, R, vec, st)) return rc;
-        if (int rc = launch(cfg, slope ? PAIR_SLOPE : PAIR, R, vec, st)) return rc;
-        if (grad_v && v_shared)
-            if (int rc = share_sum(cfg, parts, grad_v, cfg->v_heads, cfg->dv, st)) return rc;
-        if (grad_k && k_shared)
-            if (int rc = share_sum(cfg, parts2, grad_k, cfg->k_heads, cfg->dk, st)) return rc;
-    }
+    if (w.ascending || w.descending)
+        if (int rc = launch(cfg, slope ? BACKWARD_SLOPE : BACKWARD, w, vec, st)) return rc;
+    if (grad_q && q_shared)
+        if (int rc = share_sum(cfg, parts_q, grad_q, cfg->q_heads, cfg->dk, st)) return rc;
+    if (grad_v && v_shared)
+        if (int rc = share_sum(cfg, parts_v, grad_v, cfg->v_heads, cfg->dv, st)) return rc;
+    if (grad_k && k_shared)
+        if (int rc = share_sum(cfg, parts_k, grad_k, cfg->k_heads, cfg->dk, st)) return rc;
     if (slope) {
-        hipLaunchKernelGGL(td_decay_slope_kernel, dim3(cfg->heads), dim3(256), 0, st, parts_of_slope, 2 * P.slots, cfg->heads, grad_log_decay);
+        hipLaunchKernelGGL(td_decay_slope_kernel, dim3(cfg->heads), dim3(256), 0, st, slopes, 2 * Q.slots, cfg->heads, grad_log_decay);
         TD_LAUNCH_CHECK();
     }
     return TD_OK;

@@ -19,7 +19,7 @@ namespace decay {
 
 constexpr int CHUNK = 64;
 
-enum Kind { OUT, OUT_SLOPE, SUM, SUM_REVERSED, PAIR, PAIR_SLOPE };      // td_decay_out_kernel, td_decay_sum_kernel, td_decay_pair_kernel
+enum Kind { OUT, SUM, SUM_REVERSED, BACKWARD, BACKWARD_SLOPE };      // td_decay_out_kernel, td_decay_sum_kernel, td_decay_backward_kernel
 
 struct View {                 // rows of one tensor; head h of the recurrence reads head h / share
     const void *p;
@@ -28,13 +28,12 @@ struct View {                 // rows of one tensor; head h of the recurrence re
 };
 
 struct Pass {
-    View a, b, c, e;          // OUT: out from (a, b, c), e: what the slope of out is dotted with.  PAIR: out from (a, b, c), out2 from (e, c, b)
+    View a, b, c, e;          // ascending: out from (a, b, c), e: what the slope of out is dotted with.  Descending: out from (a, b, c), out2 from (e, c, b)
     const float *log_decay;
     const int32_t *offsets;   // packed: n_seq + 1, else NULL
     const float *state_in;    // (n_seq, heads, ..): element (i, j) of (da, dc) at i * st_a + j * st_c, NULL: zeros
     float *state_out;         // NULL: not wanted
     float *seg;               // (slots, heads, ..) as state_in: the state entering each segment; SUM: what each one adds
-    float *chunk_states;      // (chunks, heads, ..): the state entering each chunk, as the waves hold it; left by OUT_SLOPE for PAIR_SLOPE
     double *slope;            // one sum for each (slot, head)
     int64_t st_a, st_c;
     void *out, *out2;         // (rows, heads, dc), (rows, heads, da), float32 (out_f32, out2_f32) or the tensors' type; NULL: not wanted
@@ -42,6 +41,13 @@ struct Pass {
     int n_seq, rows, heads, da, dc;
     int seg_len, segs, slots; // rows of a segment (a multiple of CHUNK), segments of a dense sequence (1: seg_len covers all), slots in all
     float out_scale, upd_scale;
+};
+
+// What a launcher takes.  Backward: p ascending, r descending, `groups` workgroups that share out the slots and heads
+struct Work {
+    Pass p, r;
+    float *chunk_states;
+    int groups, ascending, descending;
 };
 
 // The rows of sequence n: [lo, hi) of the packed tensors or of its own rows.  Whatever the offsets hold, 0 <= lo <= hi <= rows.
@@ -162,29 +168,29 @@ template <> struct Mat<float> {
 
 // One chunk's rows of one tensor on their way from memory to LDS.  Memory is read in the order of its rows (n of them from `low` on), a
 // reversed pass turns them round in LDS.  VEC: 16 bytes a load, at 32-bit offsets from the chunk's first row, into registers that are filled
-// while the chunk before it is computed (unless there are too many); else (odd sizes, strides or addresses) element by element when the
-// chunk begins.
+// while the chunk before it is computed (unless there are too many).  These loads are never skipped, so that their registers have one writer:
+// a lane without a row or a column of its own reads its neighbours', and nothing of that is stored.  Else (odd sizes, strides or addresses)
+// element by element when the chunk begins.
 template <typename T, int D, int NT, bool VEC, bool REV> struct Stage {
     static constexpr int PER = Mat<T>::VEC, PIECES = D / PER, N = VEC ? CHUNK * PIECES / NT : 1, LD = D + PER;
     static constexpr bool AHEAD = VEC && N <= 4;
     static_assert(NT % PIECES == 0, "a thread's pieces share their columns");
     uint4 r[AHEAD ? N : 1];
-    uint32_t at;              // byte offset of the first piece; the others are whole rows further on
-    __device__ __forceinline__ void init(const View &v, int tid) {
-        at = (uint32_t)(tid / PIECES) * (uint32_t)(v.row * sizeof(T)) + tid % PIECES * 16;
-        if (AHEAD)
-#pragma unroll
-            for (int c = 0; c < N; ++c) r[c] = uint4{0, 0, 0, 0};
+    // the columns behind the last are zeros from here on
+    static __device__ __forceinline__ void init(T *lds, const View &v, int tid) {
+        if (VEC && v.d < D)
+            for (int i = tid; i < CHUNK * LD; i += NT) lds[i] = (T)0.0f;
     }
-    template <bool FULL> __device__ __forceinline__ void load(const T *base, const View &v, int low, int n, int tid) {
-        if (!AHEAD || tid % PIECES * PER >= v.d) return;
-        const char *p = (const char *)(base + (int64_t)low * v.row);
-        const int64_t by = NT / PIECES * v.row * (int64_t)sizeof(T);
+    static __device__ __forceinline__ uint4 piece(const char *chunk, const View &v, int c, int n, int tid) {
+        const int row = min(tid / PIECES + c * (NT / PIECES), n - 1), col = min(tid % PIECES * PER, v.d - PER);
+        return *(const uint4 *)(chunk + (uint32_t)(__umul24(row, (uint32_t)v.row * sizeof(T)) + col * sizeof(T)));
+    }
+    // n >= 1
+    __device__ __forceinline__ void load(const T *base, const View &v, int low, int n, int tid) {
+        if (!AHEAD) return;
+        const char *chunk = (const char *)(base + (int64_t)low * v.row);
 #pragma unroll
-        for (int c = 0; c < N; ++c) {
-            if (!FULL) r[c] = uint4{0, 0, 0, 0};
-            if (FULL || (tid + c * NT) / PIECES < n) r[c] = *(const uint4 *)(p + c * by + at);
-        }
+        for (int c = 0; c < N; ++c) r[c] = piece(chunk, v, c, n, tid);
     }
     template <bool FULL> __device__ __forceinline__ void store(T *lds, const T *base, const View &v, int low, int n, int tid) const {
         if (!VEC) {
@@ -196,23 +202,25 @@ template <typename T, int D, int NT, bool VEC, bool REV> struct Stage {
             }
             return;
         }
-        const char *p = (const char *)(base + (int64_t)low * v.row);
-        const int64_t by = NT / PIECES * v.row * (int64_t)sizeof(T);
+        if (tid % PIECES * PER >= v.d) return;
+        const char *chunk = (const char *)(base + (int64_t)low * v.row);
 #pragma unroll
         for (int c = 0; c < N; ++c) {
-            const int i = tid + c * NT, row = i / PIECES, piece = i % PIECES, to = REV && (FULL || row < n) ? (FULL ? CHUNK : n) - 1 - row : row;
-            uint4 x = uint4{0, 0, 0, 0};
-            if (AHEAD) x = r[AHEAD ? c : 0];
-            else if ((FULL || row < n) && piece * PER < v.d) x = *(const uint4 *)(p + c * by + at);
+            const int row = tid / PIECES + c * (NT / PIECES), at = tid % PIECES, to = REV && (FULL || row < n) ? (FULL ? CHUNK : n) - 1 - row : row;
+            uint4 x = AHEAD ? r[AHEAD ? c : 0] : piece(chunk, v, c, FULL ? CHUNK : n, tid);
+            if (!FULL && row >= n) x = uint4{0, 0, 0, 0};
             if constexpr (PER == 8) {
-                *(uint2 *)(lds + to * LD + Mat<T>::place(2 * piece)) = uint2{x.x, x.y};
-                *(uint2 *)(lds + to * LD + Mat<T>::place(2 * piece + 1)) = uint2{x.z, x.w};
+                *(uint2 *)(lds + to * LD + Mat<T>::place(2 * at)) = uint2{x.x, x.y};
+                *(uint2 *)(lds + to * LD + Mat<T>::place(2 * at + 1)) = uint2{x.z, x.w};
             } else {
-                *(uint4 *)(lds + to * LD + Mat<T>::place(piece)) = x;
+                *(uint4 *)(lds + to * LD + Mat<T>::place(at)) = x;
             }
         }
     }
 };
+
+// The next chunk of a pass, for the loads ahead: its first row and how many it has (1 where there is none: a row that is there)
+struct Next { int t, n; };
 
 template <typename T> __device__ __forceinline__ const T *base_of(const View &v, bool packed, int n, int h) {
     return (const T *)v.p + (packed ? 0 : n * v.seq) + (h / v.share) * v.head;
@@ -223,6 +231,15 @@ template <typename T> __device__ __forceinline__ const T *base_of(const View &v,
 __device__ __forceinline__ int here(int tid) {
     asm volatile("" : "+v"(tid));
     return tid;
+}
+
+// A kernel's argument of type A at byte `at` of the argument list, read anew from memory where it is used: kept in scalar registers, the
+// two passes' arguments would be spilled lane by lane.
+template <typename A> __device__ __forceinline__ const A &argument(int at) {
+    typedef const __attribute__((address_space(4))) char *Args;
+    Args p = (Args)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return *(const A *)(const char *)(p + at);
 }
 
 // Loads of what comes behind stay behind: the registers of two steps at once do not fit
@@ -515,77 +532,75 @@ template <int NT> __device__ __forceinline__ void workgroup_sum(double x, double
     if (tid == 0) *to = red[0];
 }
 
-__device__ __forceinline__ int64_t chunk_place(const Pass &P, int n_seq) {
-    return P.offsets ? first_place(P, n_seq, CHUNK) : (int64_t)n_seq * ((P.rows + CHUNK - 1) / CHUNK);
-}
-
 // What a segment adds to the state
 template <typename T, int DA, int DC, int NW, bool VEC, bool REV, int WAVES> __global__ __launch_bounds__(64 * NW, WAVES) void td_decay_sum_kernel(Pass P) {
     typedef Stream<T, DA, DC, NW, VEC, 2> X;
     constexpr int NT = 64 * NW;
     __shared__ __align__(16) T lb[CHUNK * X::LA];
     __shared__ __align__(16) T lc[CHUNK * X::LC];
-    const int tid_ = threadIdx.x, tid = tid_, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = (tid & 63) >> 4, li = tid & 15;
+    const int tid_ = here(threadIdx.x), tid = tid_, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = (tid & 63) >> 4, li = tid & 15;
     const int h = blockIdx.x % P.heads, slot = blockIdx.x / P.heads;
     Place at;
     if (!at.find(P, slot) || (REV ? at.segment == 0 : at.last)) return;      // nothing enters a segment from these
     const T *pb = base_of<T>(P.b, P.offsets, at.n_seq, h) + (int64_t)at.lo * P.b.row, *pc = base_of<T>(P.c, P.offsets, at.n_seq, h) + (int64_t)at.lo * P.c.row;
     Stage<T, DA, NT, VEC, REV> sb;
     Stage<T, DC, NT, VEC, REV> sc;
-    sb.init(P.b, tid);
-    sc.init(P.c, tid);
-    const auto fetch = [&](auto rows, int t, int n) __attribute__((always_inline)) {
-        constexpr bool FULL = decltype(rows)::FULL;
-        sb.template load<FULL>(pb, P.b, t, n, tid);
-        sc.template load<FULL>(pc, P.c, t, n, tid);
+    sb.init(lb, P.b, tid);
+    sc.init(lc, P.c, tid);
+    const auto fetch = [&](Next next, int tid) __attribute__((always_inline)) {
+        sb.load(pb, P.b, next.t, next.n, tid);
+        sc.load(pc, P.c, next.t, next.n, tid);
     };
     const int whole = (at.t1 - at.t0) / CHUNK, tail = (at.t1 - at.t0) % CHUNK;
-    if (REV && tail) fetch(Most(), at.t1 - tail, tail);
-    else fetch(Whole(), REV ? at.t1 - CHUNK : at.t0, CHUNK);
+    fetch(REV && tail ? Next{at.t1 - tail, tail} : Next{REV ? at.t1 - CHUNK : at.t0, CHUNK}, tid);
+    __syncthreads();
     Weights<NW> w;
     w.init(P.log_decay[h], P.upd_scale, REV, wave, g, li);
     X x;
     x.enter(nullptr, 0, 0, 0, 0, wave, g, li);
-    const auto chunk = [&](auto rows, int t, int n, int next) __attribute__((always_inline)) {
+    const auto chunk = [&](auto rows, int t, int n, Next next) __attribute__((always_inline)) {
         typedef decltype(rows) R;
         constexpr bool FULL = R::FULL;
         const int tid = here(tid_), lane = tid & 63, g = lane >> 4, li = lane & 15;
         sb.template store<FULL>(lb, pb, P.b, t, n, tid);
         sc.template store<FULL>(lc, pc, P.c, t, n, tid);
         __syncthreads();
-        if (next >= 0) fetch(Whole(), next, CHUNK);
+        fetch(next, tid);
         x.columns(lc, wave, g, li);
         x.template advance<R>(lb, n, w, P.upd_scale, REV, g, li);
         __syncthreads();
     };
-    const int before = whole ? at.t1 - tail - CHUNK : -1;
+    const Next before = whole ? Next{at.t1 - tail - CHUNK, CHUNK} : Next{at.t0, 1};
     if (REV && tail > CHUNK / 2) chunk(Most(), at.t1 - tail, tail, before);
     else if (REV && tail) chunk(Half(), at.t1 - tail, tail, before);
     for (int c = 0; c < whole; ++c) {        // (a segment that is not the last has no tail)
         const int t = REV ? at.t0 + (whole - 1 - c) * CHUNK : at.t0 + c * CHUNK;
-        chunk(Whole(), t, CHUNK, c + 1 < whole ? (REV ? t - CHUNK : t + CHUNK) : -1);
+        chunk(Whole(), t, CHUNK, c + 1 < whole ? Next{REV ? t - CHUNK : t + CHUNK, CHUNK} : Next{t, 1});
     }
     x.leave(P.seg + (int64_t)blockIdx.x * P.da * P.dc, P.st_a, P.st_c, P.da, P.dc, wave, g, li);
 }
 
 // out from (a, b, c), rows ascending.  SLOPE: the part of the derivative by log g that rows owe to the states entering their chunks, dotted with
 // e, and those states for the pass over the other gradients.
-template <typename T, int DA, int DC, int NW, bool VEC, bool SLOPE, int WAVES> __global__ __launch_bounds__(64 * NW, WAVES) void td_decay_out_kernel(Pass P) {
+template <typename T, int DA, int DC, int NW, bool SLOPE> struct OutLds {
+    typedef Stream<T, DA, DC, NW, true, 2> X;
+    T a[CHUNK * X::LA], b[CHUNK * X::LA], c[CHUNK * X::LC], e[SLOPE ? CHUNK * X::LC : 8];
+    typename X::Op scores[X::PAIRS * X::S2 * 64];
+};
+template <typename T, int DA, int DC, int NW, bool VEC, bool SLOPE>
+__device__ __forceinline__ void out_sweep(const Pass &P, int item, OutLds<T, DA, DC, NW, SLOPE> &lds, float *chunk_states) {
     typedef Stream<T, DA, DC, NW, VEC, SLOPE ? 3 : 2> X;
     typedef typename X::Op Op;
     constexpr int NT = 64 * NW;
-    __shared__ __align__(16) T la[CHUNK * X::LA];
-    __shared__ __align__(16) T lb[CHUNK * X::LA];
-    __shared__ __align__(16) T lc[CHUNK * X::LC];
-    __shared__ __align__(16) T le[SLOPE ? CHUNK * X::LC : 8];
-    __shared__ __align__(16) Op scores[X::PAIRS * X::S2 * 64];
-    const int tid_ = threadIdx.x, tid = tid_, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, li = lane & 15;
-    const int h = blockIdx.x % P.heads, slot = blockIdx.x / P.heads;
+    T *const la = lds.a, *const lb = lds.b, *const lc = lds.c, *const le = lds.e;
+    Op *const scores = lds.scores;
+    const int tid_ = here(threadIdx.x), tid = tid_, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, li = lane & 15;
+    const int h = item % P.heads, slot = item / P.heads;
     const bool packed = P.offsets != nullptr;
     if (packed) clear_rows_of<T>(P, P.out, P.out_f32, P.dc, slot, h, tid, NT);
     Place at;
     if (!at.find(P, slot)) {
-        if (SLOPE && tid == 0) P.slope[blockIdx.x] = 0.0;
+        if (SLOPE && tid == 0) P.slope[item] = 0.0;
         return;
     }
     const T *pa = base_of<T>(P.a, packed, at.n_seq, h) + (int64_t)at.lo * P.a.row, *pb = base_of<T>(P.b, packed, at.n_seq, h) + (int64_t)at.lo * P.b.row;
@@ -593,28 +608,25 @@ template <typename T, int DA, int DC, int NW, bool VEC, bool SLOPE, int WAVES> _
     const T *pe = SLOPE ? base_of<T>(P.e, packed, at.n_seq, h) + (int64_t)at.lo * P.e.row : nullptr;
     Stage<T, DA, NT, VEC, false> sa, sb;
     Stage<T, DC, NT, VEC, false> sc, se;
-    sa.init(P.a, tid);
-    sb.init(P.b, tid);
-    sc.init(P.c, tid);
-    if (SLOPE) se.init(P.e, tid);
-    const auto fetch = [&](int t) __attribute__((always_inline)) {
-        const auto load = [&](auto rows, int n) __attribute__((always_inline)) {
-            constexpr bool FULL = decltype(rows)::FULL;
-            sb.template load<FULL>(pb, P.b, t, n, tid);
-            sa.template load<FULL>(pa, P.a, t, n, tid);
-            sc.template load<FULL>(pc, P.c, t, n, tid);
-            if (SLOPE) se.template load<FULL>(pe, P.e, t, n, tid);
-        };
-        if (at.t1 - t >= CHUNK) load(Whole(), CHUNK);
-        else if (t < at.t1) load(Most(), at.t1 - t);
+    sa.init(la, P.a, tid);
+    sb.init(lb, P.b, tid);
+    sc.init(lc, P.c, tid);
+    if (SLOPE) se.init(le, P.e, tid);
+    const auto fetch = [&](int t, int tid) __attribute__((always_inline)) {
+        const Next next = at.t1 - t >= CHUNK ? Next{t, CHUNK} : t < at.t1 ? Next{t, at.t1 - t} : Next{at.t0, 1};
+        sb.load(pb, P.b, next.t, next.n, tid);
+        sa.load(pa, P.a, next.t, next.n, tid);
+        sc.load(pc, P.c, next.t, next.n, tid);
+        if (SLOPE) se.load(pe, P.e, next.t, next.n, tid);
     };
-    fetch(at.t0);
+    if (at.t0 < at.t1) fetch(at.t0, tid);
+    __syncthreads();
     Weights<NW> w;
     w.init(P.log_decay[h], P.upd_scale, 0, wave, g, li);
     if (wave == 0) X::clear_scores(scores, lane);
     const int64_t state_at = ((int64_t)at.n_seq * P.heads + h) * P.da * P.dc;
     X x;
-    x.enter(at.segment > 0 ? P.seg + (int64_t)blockIdx.x * P.da * P.dc : P.state_in ? P.state_in + state_at : nullptr, P.st_a, P.st_c, P.da, P.dc, wave, g, li);
+    x.enter(at.segment > 0 ? P.seg + (int64_t)item * P.da * P.dc : P.state_in ? P.state_in + state_at : nullptr, P.st_a, P.st_c, P.da, P.dc, wave, g, li);
     double slope = 0.0;
     const auto chunk = [&](auto rows, int t, int n) __attribute__((always_inline)) {
         typedef decltype(rows) R;
@@ -625,7 +637,7 @@ template <typename T, int DA, int DC, int NW, bool VEC, bool SLOPE, int WAVES> _
         sc.template store<FULL>(lc, pc, P.c, t, n, tid);
         if (SLOPE) se.template store<FULL>(le, pe, P.e, t, n, tid);
         __syncthreads();
-        if (FULL) fetch(t + CHUNK);
+        if (FULL) fetch(t + CHUNK, tid);
 #pragma unroll
         for (int m = 0; m < w.MINE; ++m) {
             const int it = w.it[m], jt = w.jt[m];
@@ -636,7 +648,7 @@ template <typename T, int DA, int DC, int NW, bool VEC, bool SLOPE, int WAVES> _
             X::keep(s, scores, it, jt, lane);
         }
         if (SLOPE) {
-            f32x4 *to = (f32x4 *)P.chunk_states + ((((chunk_place(P, at.n_seq) + t / CHUNK) * P.heads + h) * NW + wave) * X::TA * X::CT) * 64 + lane;
+            f32x4 *to = (f32x4 *)chunk_states + (((t - at.t0) / CHUNK * NW + wave) * X::TA * X::CT) * 64 + lane;
 #pragma unroll
             for (int mt = 0; mt < X::TA; ++mt)
 #pragma unroll
@@ -658,24 +670,32 @@ template <typename T, int DA, int DC, int NW, bool VEC, bool SLOPE, int WAVES> _
     if (at.t1 - t > CHUNK / 2) chunk(Most(), t, at.t1 - t);
     else if (t < at.t1) chunk(Half(), t, at.t1 - t);
     x.leave(at.last && P.state_out ? P.state_out + state_at : nullptr, P.st_a, P.st_c, P.da, P.dc, wave, g, li);
-    if (SLOPE) workgroup_sum<NT>(slope, (double *)scores, P.slope + blockIdx.x, tid);
+    if (SLOPE) workgroup_sum<NT>(slope, (double *)&lds, P.slope + item, tid);
+}
+
+template <typename T, int DA, int DC, int NW, bool VEC, int WAVES> __global__ __launch_bounds__(64 * NW, WAVES) void td_decay_out_kernel(Pass P) {
+    __shared__ __align__(16) OutLds<T, DA, DC, NW, false> lds;
+    out_sweep<T, DA, DC, NW, VEC, false>(P, blockIdx.x, lds, nullptr);
 }
 
 // out from (a, b, c) and out2 from (e, c, b), rows descending: the gradients of v and k from (k, q, grad_o) and (v, grad_o, q).  SLOPE: the rest of
 // the derivative by log g: pairs of rows of one chunk; what a chunk's rows owe to the chunks behind it; and the chunk's own n rows, for every pair with one
 // row before and one behind it, which is n g^n <state entering the chunk, its gradient when it leaves>.
-template <typename T, int DK, int DV, int NW, bool VEC, bool SLOPE, int WAVES> __global__ __launch_bounds__(64 * NW, WAVES) void td_decay_pair_kernel(Pass P) {
+template <typename T, int DK, int DV, int NW> struct PairLds {
+    typedef Stream<T, DK, DV, NW, true, 2> V;
+    T k[CHUNK * V::LA], q[CHUNK * V::LA], o[CHUNK * V::LC], v[CHUNK * V::LC];
+    typename V::Op scores[2][V::PAIRS * V::S2 * 64];
+};
+template <typename T, int DK, int DV, int NW, bool VEC, bool SLOPE>
+__device__ __forceinline__ void pair_sweep(const Pass &P, int item, PairLds<T, DK, DV, NW> &lds, const float *chunk_states) {
     typedef Stream<T, DK, DV, NW, VEC, 2> V;
     typedef Stream<T, DV, DK, NW, VEC, SLOPE ? 3 : 2> K;
     typedef typename V::Op Op;
     constexpr int NT = 64 * NW;
-    __shared__ __align__(16) T lk[CHUNK * V::LA];
-    __shared__ __align__(16) T lq[CHUNK * V::LA];
-    __shared__ __align__(16) T lo[CHUNK * V::LC];
-    __shared__ __align__(16) T lv[CHUNK * V::LC];
-    __shared__ __align__(16) Op scores[2][V::PAIRS * V::S2 * 64];
-    const int tid_ = threadIdx.x, tid = tid_, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, li = lane & 15;
-    const int h = blockIdx.x % P.heads, slot = blockIdx.x / P.heads;
+    T *const lk = lds.k, *const lq = lds.q, *const lo = lds.o, *const lv = lds.v;
+    Op *const scores[2] = {lds.scores[0], lds.scores[1]};
+    const int tid_ = here(threadIdx.x), tid = tid_, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, li = lane & 15;
+    const int h = item % P.heads, slot = item / P.heads;
     const bool packed = P.offsets != nullptr;
     if (packed) {
         clear_rows_of<T>(P, P.out, P.out_f32, P.dc, slot, h, tid, NT);
@@ -683,27 +703,26 @@ template <typename T, int DK, int DV, int NW, bool VEC, bool SLOPE, int WAVES> _
     }
     Place at;
     if (!at.find(P, slot)) {
-        if (SLOPE && tid == 0) P.slope[blockIdx.x] = 0.0;
+        if (SLOPE && tid == 0) P.slope[item] = 0.0;
         return;
     }
     const T *pk = base_of<T>(P.a, packed, at.n_seq, h) + (int64_t)at.lo * P.a.row, *pq = base_of<T>(P.b, packed, at.n_seq, h) + (int64_t)at.lo * P.b.row;
     const T *po = base_of<T>(P.c, packed, at.n_seq, h) + (int64_t)at.lo * P.c.row, *pv = base_of<T>(P.e, packed, at.n_seq, h) + (int64_t)at.lo * P.e.row;
     Stage<T, DK, NT, VEC, true> sk, sq;
     Stage<T, DV, NT, VEC, true> so, sv;
-    sk.init(P.a, tid);
-    sq.init(P.b, tid);
-    so.init(P.c, tid);
-    sv.init(P.e, tid);
-    const auto fetch = [&](auto rows, int t, int n) __attribute__((always_inline)) {
-        constexpr bool FULL = decltype(rows)::FULL;
-        sk.template load<FULL>(pk, P.a, t, n, tid);
-        sq.template load<FULL>(pq, P.b, t, n, tid);
-        so.template load<FULL>(po, P.c, t, n, tid);
-        sv.template load<FULL>(pv, P.e, t, n, tid);
+    sk.init(lk, P.a, tid);
+    sq.init(lq, P.b, tid);
+    so.init(lo, P.c, tid);
+    sv.init(lv, P.e, tid);
+    const auto fetch = [&](Next next, int tid) __attribute__((always_inline)) {
+        sk.load(pk, P.a, next.t, next.n, tid);
+        sq.load(pq, P.b, next.t, next.n, tid);
+        so.load(po, P.c, next.t, next.n, tid);
+        sv.load(pv, P.e, next.t, next.n, tid);
     };
     const int whole = (at.t1 - at.t0) / CHUNK, tail = (at.t1 - at.t0) % CHUNK;
-    if (tail) fetch(Most(), at.t1 - tail, tail);
-    else if (whole) fetch(Whole(), at.t1 - CHUNK, CHUNK);
+    if (at.t0 < at.t1) fetch(tail ? Next{at.t1 - tail, tail} : Next{at.t1 - CHUNK, CHUNK}, tid);
+    __syncthreads();
     Weights<NW> w;
     w.init(P.log_decay[h], P.upd_scale, 1, wave, g, li);
     if (wave == 0) {
@@ -711,13 +730,13 @@ template <typename T, int DK, int DV, int NW, bool VEC, bool SLOPE, int WAVES> _
         V::clear_scores(scores[1], lane);
     }
     const int64_t state_at = ((int64_t)at.n_seq * P.heads + h) * P.da * P.dc;
-    const float *from = !at.last ? P.seg + (int64_t)blockIdx.x * P.da * P.dc : P.state_in ? P.state_in + state_at : nullptr;
+    const float *from = !at.last ? P.seg + (int64_t)item * P.da * P.dc : P.state_in ? P.state_in + state_at : nullptr;
     V xv;
     K xk;
     xv.enter(from, P.st_a, P.st_c, P.da, P.dc, wave, g, li);
     xk.enter(from, P.st_c, P.st_a, P.dc, P.da, wave, g, li);
     double slope = 0.0;
-    const auto chunk = [&](auto rows, int t, int n, int next) __attribute__((always_inline)) {
+    const auto chunk = [&](auto rows, int t, int n, Next next) __attribute__((always_inline)) {
         typedef decltype(rows) R;
         constexpr bool FULL = R::FULL;
         const int tid = here(tid_), lane = tid & 63, g = lane >> 4, li = lane & 15;
@@ -726,7 +745,7 @@ template <typename T, int DK, int DV, int NW, bool VEC, bool SLOPE, int WAVES> _
         so.template store<FULL>(lo, po, P.c, t, n, tid);
         sv.template store<FULL>(lv, pv, P.e, t, n, tid);
         __syncthreads();
-        if (next >= 0) fetch(Whole(), next, CHUNK);
+        fetch(next, tid);
         float sum = 0.0f;
 #pragma unroll
         for (int m = 0; m < w.MINE; ++m) {
@@ -744,7 +763,7 @@ template <typename T, int DK, int DV, int NW, bool VEC, bool SLOPE, int WAVES> _
         }
         phase();
         if (SLOPE) {
-            const f32x4 *from = (const f32x4 *)P.chunk_states + ((((chunk_place(P, at.n_seq) + t / CHUNK) * P.heads + h) * NW + wave) * K::TA * K::CT) * 64 + lane;
+            const f32x4 *from = (const f32x4 *)chunk_states + (((t - at.t0) / CHUNK * NW + wave) * K::TA * K::CT) * 64 + lane;
             float cross = 0.0f;
 #pragma unroll
             for (int mt = 0; mt < K::TA; ++mt)
@@ -774,12 +793,30 @@ template <typename T, int DK, int DV, int NW, bool VEC, bool SLOPE, int WAVES> _
         xv.template advance<R>(lq, n, w, P.upd_scale, 1, g, li);
         __syncthreads();
     };
-    const int before = whole ? at.t1 - tail - CHUNK : -1;
+    const Next before = whole ? Next{at.t1 - tail - CHUNK, CHUNK} : Next{at.t0, 1};
     if (tail > CHUNK / 2) chunk(Most(), at.t1 - tail, tail, before);
     else if (tail) chunk(Half(), at.t1 - tail, tail, before);
-    for (int c = whole - 1; c >= 0; --c) chunk(Whole(), at.t0 + c * CHUNK, CHUNK, c > 0 ? at.t0 + (c - 1) * CHUNK : -1);
+    for (int c = whole - 1; c >= 0; --c) chunk(Whole(), at.t0 + c * CHUNK, CHUNK, c > 0 ? Next{at.t0 + (c - 1) * CHUNK, CHUNK} : Next{at.t0, 1});
     xv.leave(at.segment == 0 && P.state_out ? P.state_out + state_at : nullptr, P.st_a, P.st_c, P.da, P.dc, wave, g, li);
-    if (SLOPE) workgroup_sum<NT>(slope, (double *)scores, P.slope + blockIdx.x, tid);
+    if (SLOPE) workgroup_sum<NT>(slope, (double *)&lds, P.slope + item, tid);
+}
+
+// The gradients of one (slot, head) after another: that of q with Q's rows ascending, those of k and v with R's descending, right behind each other
+// so that the second reading of q, k, v and grad_o (and, for the slope, of the states entering the chunks, in a place of the
+// workgroup's own: `held` floats) comes from the caches.
+template <typename T, int DK, int DV, int NW, bool VEC, bool SLOPE, int WAVES>
+__global__ __launch_bounds__(64 * NW, WAVES) void td_decay_backward_kernel(Pass Q, Pass R, float *chunk_states, int64_t held, int ascending, int descending) {
+    __shared__ __align__(16) union {
+        OutLds<T, DV, DK, NW, SLOPE> out;
+        PairLds<T, DK, DV, NW> pair;
+    } lds;
+    float *mine = chunk_states + blockIdx.x * held;
+    for (int item = blockIdx.x; item < Q.slots * Q.heads; item += gridDim.x) {
+        if (ascending) out_sweep<T, DV, DK, NW, VEC, SLOPE>(argument<Pass>(0), item, lds.out, mine);
+        __syncthreads();
+        if (descending) pair_sweep<T, DK, DV, NW, VEC, SLOPE>(argument<Pass>(sizeof(Pass)), item, lds.pair, mine);
+        __syncthreads();
+    }
 }
 
 }  // namespace decay

@@ -15,21 +15,20 @@ typedef float T;
 #endif
 
 // waves a SIMD is to hold: what the registers of each size allow without spilling
-template <bool VEC, int DA, int DC> int launch(const Pass &P, hipStream_t st) {
+template <bool VEC, int DA, int DC> int launch(const Work &w, hipStream_t st) {
     constexpr int NW = DA == 32 ? 2 : 4, size = DA + DC;
+    const Pass &P = w.p;
     const dim3 grid((unsigned)(P.slots * P.heads)), block(64 * NW);
 #if TD_INST_KIND == 0
-    hipLaunchKernelGGL((td_decay_out_kernel<T, DA, DC, NW, VEC, false, size <= 128 ? 3 : 2>), grid, block, 0, st, P);
+    hipLaunchKernelGGL((td_decay_out_kernel<T, DA, DC, NW, VEC, size <= 128 ? 3 : 2>), grid, block, 0, st, P);
 #elif TD_INST_KIND == 1
-    hipLaunchKernelGGL((td_decay_out_kernel<T, DA, DC, NW, VEC, true, size <= 64 ? 3 : size <= 128 ? 2 : 1>), grid, block, 0, st, P);
-#elif TD_INST_KIND == 2
     hipLaunchKernelGGL((td_decay_sum_kernel<T, DA, DC, NW, VEC, false, size <= 128 ? 4 : 2>), grid, block, 0, st, P);
-#elif TD_INST_KIND == 3
+#elif TD_INST_KIND == 2
     hipLaunchKernelGGL((td_decay_sum_kernel<T, DA, DC, NW, VEC, true, size <= 128 ? 4 : 2>), grid, block, 0, st, P);
-#elif TD_INST_KIND == 4
-    hipLaunchKernelGGL((td_decay_pair_kernel<T, DA, DC, NW, VEC, false, size <= 128 ? 2 : 1>), grid, block, 0, st, P);
 #else
-    hipLaunchKernelGGL((td_decay_pair_kernel<T, DA, DC, NW, VEC, true, size <= 128 ? 2 : 1>), grid, block, 0, st, P);
+    const int64_t held = (int64_t)((P.seg_len + CHUNK - 1) / CHUNK) * DA * DC;
+    hipLaunchKernelGGL((td_decay_backward_kernel<T, DA, DC, NW, VEC, TD_INST_KIND == 4, size <= 128 ? 2 : 1>), dim3((unsigned)w.groups), block, 0, st, w.p, w.r,
+                       w.chunk_states, held, w.ascending, w.descending);
 #endif
     TD_LAUNCH_CHECK();
     return TD_OK;
@@ -39,16 +38,17 @@ template <bool VEC, int DA, int DC> int launch(const Pass &P, hipStream_t st) {
 
 // (sizes that are not a multiple of 16 bytes take the nearest square: what they gain from fewer kernels they do not lose to padding, their
 // loads are the bound)
-int TD_CAT(td_decay_launch_, TD_INST_BF16, TD_INST_KIND)(const Pass &P, int vec, hipStream_t st) {
+int TD_CAT(td_decay_launch_, TD_INST_BF16, TD_INST_KIND)(const Work &w, int vec, hipStream_t st) {
+    const Pass &P = TD_INST_KIND < 3 ? w.p : w.r;          // backward: (da, dc) = (dk, dv)
     const int most = P.da > P.dc ? P.da : P.dc;
     if (vec) {
-        if (most <= 32) return launch<true, 32, 32>(P, st);
-        if (most <= 64) return launch<true, 64, 64>(P, st);
-        if (P.da <= 64) return launch<true, 64, 128>(P, st);
-        if (P.dc <= 64) return launch<true, 128, 64>(P, st);
-        return launch<true, 128, 128>(P, st);
+        if (most <= 32) return launch<true, 32, 32>(w, st);
+        if (most <= 64) return launch<true, 64, 64>(w, st);
+        if (P.da <= 64) return launch<true, 64, 128>(w, st);
+        if (P.dc <= 64) return launch<true, 128, 64>(w, st);
+        return launch<true, 128, 128>(w, st);
     }
-    if (most <= 32) return launch<false, 32, 32>(P, st);
-    if (most <= 64) return launch<false, 64, 64>(P, st);
-    return launch<false, 128, 128>(P, st);
+    if (most <= 32) return launch<false, 32, 32>(w, st);
+    if (most <= 64) return launch<false, 64, 64>(w, st);
+    return launch<false, 128, 128>(w, st);
 }
