@@ -100,18 +100,27 @@ template <> struct Mat<__bf16> {
     static constexpr int VEC = 8;       // elements of 16 bytes
     static constexpr bool SPLIT = true;
     static __device__ __forceinline__ f32x4 mma(Op a, Op b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
-    // columns are stored in the order of the inner index: of each 32, group g's four of the first 16, then its four of the second
-    static __device__ __forceinline__ int place(int four) { return (four >> 3) * 32 + (four & 3) * 8 + ((four >> 2) & 1) * 4; }
-    static __device__ __forceinline__ Op row_op(const __bf16 *t, int ld, int row, int ks, int g) { return *(const Op *)(t + row * ld + ks * 32 + g * 8); }
-    static __device__ __forceinline__ Op col_op(const __bf16 *t, int ld, int tile, int kr, int g, int li) {
+    static constexpr int pitch(int d) { return d; }          // elements between rows in LDS
+    static __device__ __forceinline__ Op row_op(const __bf16 *t, int d, int row, int ks, int g) { return *(const Op *)(t + lds_at(d, row, ks * 4 + g)); }
+    static __device__ __forceinline__ Op col_op(const __bf16 *t, int d, int tile, int kr, int g, int li) {
         typedef __attribute__((__vector_size__(4 * sizeof(short)))) short s16x4;
         typedef __attribute__((address_space(3))) s16x4 *lds;
-        const __bf16 *p = t + (kr * 32 + g * 4 + (li >> 2)) * ld + place(tile * 4 + (li & 3));
+        const int row = kr * 32 + g * 4 + (li >> 2);
+        const __bf16 *p = t + lds_at(d, row, (tile >> 1) * 4 + (li & 3)) + (tile & 1) * 4;
         union { s16x4 s[2]; Op o; } x;
         x.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)(void *)p);
-        x.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)(void *)(p + 16 * ld));
+        x.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)(void *)(p + 16 * d));
         return x.o;
     }
+    // A row in LDS: of each 32 columns, 16 bytes for each group g with its four of the first 16 and its four of the second (the order of an
+    // operand's inner index, so that one 16-byte load is an operand); no padding, a row's 16-byte pieces change places with
+    // bits of the row's number, so that eight rows' same piece and four rows' four neighbouring pieces both lie on different banks.
+    static __device__ __forceinline__ int lds_at(int d, int row, int piece) {
+        const int turn = d == 64 ? (row & 2) << 1 | (row & 4) >> 1 | (row & 1) : d > 64 ? (row & 3) << 2 | (row & 4) >> 2 : (row & 4) >> 2;
+        return row * d + (piece ^ turn) * 8;
+    }
+    // four columns from 4 * four on
+    static __device__ __forceinline__ int four_at(int d, int row, int four) { return lds_at(d, row, (four >> 3) * 4 + (four & 3)) + ((four >> 2) & 1) * 4; }
     // two values to bf16 (one instruction); what is left of them behind
     static __device__ __forceinline__ uint32_t term(float &a, float &b, bool last) {
         typedef __attribute__((ext_vector_type(2))) float f32x2;
@@ -155,12 +164,13 @@ template <> struct Mat<float> {
         for (int r = 0; r < 4; ++r) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[r], b[r], c, 0, 0, 0);
         return c;
     }
-    static __device__ __forceinline__ int place(int four) { return four * 4; }
-    static __device__ __forceinline__ Op row_op(const float *t, int ld, int row, int ks, int g) { return *(const Op *)(t + row * ld + ks * 16 + g * 4); }
-    static __device__ __forceinline__ Op col_op(const float *t, int ld, int tile, int kr, int g, int li) {
-        const float *p = t + (kr * 16 + g * 4) * ld + tile * 16 + li;
-        return Op{p[0], p[ld], p[2 * ld], p[3 * ld]};
+    static constexpr int pitch(int d) { return d + 4; }      // rows in LDS: 16 bytes between them
+    static __device__ __forceinline__ Op row_op(const float *t, int d, int row, int ks, int g) { return *(const Op *)(t + row * pitch(d) + ks * 16 + g * 4); }
+    static __device__ __forceinline__ Op col_op(const float *t, int d, int tile, int kr, int g, int li) {
+        const float *p = t + (kr * 16 + g * 4) * pitch(d) + tile * 16 + li;
+        return Op{p[0], p[pitch(d)], p[2 * pitch(d)], p[3 * pitch(d)]};
     }
+    static __device__ __forceinline__ int four_at(int d, int row, int four) { return row * pitch(d) + four * 4; }
     template <int N> static __device__ __forceinline__ void split(const f32x4 *x, Op *p) { p[0] = x[0]; }
     template <int N> static __device__ __forceinline__ void keep(f32x4 x, Op *to, int) { *to = x; }
     static __device__ __forceinline__ float elem(Op o, int, int r) { return o[r]; }
@@ -172,14 +182,14 @@ template <> struct Mat<float> {
 // a lane without a row or a column of its own reads its neighbours', and nothing of that is stored.  Else (odd sizes, strides or addresses)
 // element by element when the chunk begins.
 template <typename T, int D, int NT, bool VEC, bool REV> struct Stage {
-    static constexpr int PER = Mat<T>::VEC, PIECES = D / PER, N = VEC ? CHUNK * PIECES / NT : 1, LD = D + PER;
+    static constexpr int PER = Mat<T>::VEC, PIECES = D / PER, N = VEC ? CHUNK * PIECES / NT : 1;
     static constexpr bool AHEAD = VEC && N <= 4;
     static_assert(NT % PIECES == 0, "a thread's pieces share their columns");
     uint4 r[AHEAD ? N : 1];
     // the columns behind the last are zeros from here on
     static __device__ __forceinline__ void init(T *lds, const View &v, int tid) {
         if (VEC && v.d < D)
-            for (int i = tid; i < CHUNK * LD; i += NT) lds[i] = (T)0.0f;
+            for (int i = tid; i < CHUNK * Mat<T>::pitch(D); i += NT) lds[i] = (T)0.0f;
     }
     static __device__ __forceinline__ uint4 piece(const char *chunk, const View &v, int c, int n, int tid) {
         const int row = min(tid / PIECES + c * (NT / PIECES), n - 1), col = min(tid % PIECES * PER, v.d - PER);
@@ -198,7 +208,7 @@ template <typename T, int D, int NT, bool VEC, bool REV> struct Stage {
 #pragma unroll 4
             for (int i = tid; i < CHUNK * D; i += NT) {
                 const int row = i / D, col = i % D, to = REV && row < n ? n - 1 - row : row;
-                lds[to * LD + Mat<T>::place(col >> 2) + (col & 3)] = row < n && col < v.d ? p[row * v.row + col] : (T)0.0f;
+                lds[Mat<T>::four_at(D, to, col >> 2) + (col & 3)] = row < n && col < v.d ? p[row * v.row + col] : (T)0.0f;
             }
             return;
         }
@@ -210,10 +220,10 @@ template <typename T, int D, int NT, bool VEC, bool REV> struct Stage {
             uint4 x = AHEAD ? r[AHEAD ? c : 0] : piece(chunk, v, c, FULL ? CHUNK : n, tid);
             if (!FULL && row >= n) x = uint4{0, 0, 0, 0};
             if constexpr (PER == 8) {
-                *(uint2 *)(lds + to * LD + Mat<T>::place(2 * at)) = uint2{x.x, x.y};
-                *(uint2 *)(lds + to * LD + Mat<T>::place(2 * at + 1)) = uint2{x.z, x.w};
+                *(uint2 *)(lds + Mat<T>::four_at(D, to, 2 * at)) = uint2{x.x, x.y};
+                *(uint2 *)(lds + Mat<T>::four_at(D, to, 2 * at + 1)) = uint2{x.z, x.w};
             } else {
-                *(uint4 *)(lds + to * LD + Mat<T>::place(at)) = x;
+                *(uint4 *)(lds + Mat<T>::four_at(D, to, at)) = x;
             }
         }
     }
@@ -312,7 +322,7 @@ template <int NW> struct Weights {
 template <typename T, int DA, int DC, int NW, bool VEC, int TERMS> struct Stream {
     typedef Mat<T> M;
     typedef typename M::Op Op;
-    static constexpr int LA = DA + M::VEC, LC = DC + M::VEC, TA = DA / 16, CT = DC / 16 / NW, KS = TA / M::KT, RT = CHUNK / 16, KR = RT / M::KT;
+    static constexpr int LA = DA, LC = DC, PA = M::pitch(DA), PC = M::pitch(DC), TA = DA / 16, CT = DC / 16 / NW, KS = TA / M::KT, RT = CHUNK / 16, KR = RT / M::KT;
     static constexpr int S2 = M::SPLIT ? 2 : 1, S3 = M::SPLIT ? 3 : 1, SF = M::SPLIT ? TERMS : 1;      // terms of scores, of decayed rows, of the state
     static constexpr int PAIRS = M::KT == 2 ? RT / 2 * (RT / 2 + 1) : RT * (RT + 1) / 2;               // score operands: (it, kr), kr <= it / KT
     static_assert(CT * NW * 16 == DC && CT > 0, "every column tile has a wave");
@@ -406,7 +416,7 @@ template <typename T, int DA, int DC, int NW, bool VEC, int TERMS> struct Stream
             float part = 0.0f;
 #pragma unroll
             for (int ct = 0; ct < CT; ++ct) {
-                const T *e = le + (it * 16 + li) * LC + M::place((wave * CT + ct) * 4 + g);
+                const T *e = le + M::four_at(LC, it * 16 + li, (wave * CT + ct) * 4 + g);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) part += o[it][ct][r] * (float)e[r];
             }
@@ -536,8 +546,8 @@ template <int NT> __device__ __forceinline__ void workgroup_sum(double x, double
 template <typename T, int DA, int DC, int NW, bool VEC, bool REV, int WAVES> __global__ __launch_bounds__(64 * NW, WAVES) void td_decay_sum_kernel(Pass P) {
     typedef Stream<T, DA, DC, NW, VEC, 2> X;
     constexpr int NT = 64 * NW;
-    __shared__ __align__(16) T lb[CHUNK * X::LA];
-    __shared__ __align__(16) T lc[CHUNK * X::LC];
+    __shared__ __align__(16) T lb[CHUNK * X::PA];
+    __shared__ __align__(16) T lc[CHUNK * X::PC];
     const int tid_ = here(threadIdx.x), tid = tid_, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = (tid & 63) >> 4, li = tid & 15;
     const int h = blockIdx.x % P.heads, slot = blockIdx.x / P.heads;
     Place at;
@@ -584,7 +594,7 @@ template <typename T, int DA, int DC, int NW, bool VEC, bool REV, int WAVES> __g
 // e, and those states for the pass over the other gradients.
 template <typename T, int DA, int DC, int NW, bool SLOPE> struct OutLds {
     typedef Stream<T, DA, DC, NW, true, 2> X;
-    T a[CHUNK * X::LA], b[CHUNK * X::LA], c[CHUNK * X::LC], e[SLOPE ? CHUNK * X::LC : 8];
+    T a[CHUNK * X::PA], b[CHUNK * X::PA], c[CHUNK * X::PC], e[SLOPE ? CHUNK * X::PC : 8];
     typename X::Op scores[X::PAIRS * X::S2 * 64];
 };
 template <typename T, int DA, int DC, int NW, bool VEC, bool SLOPE>
@@ -683,7 +693,7 @@ template <typename T, int DA, int DC, int NW, bool VEC, int WAVES> __global__ __
 // row before and one behind it, which is n g^n <state entering the chunk, its gradient when it leaves>.
 template <typename T, int DK, int DV, int NW> struct PairLds {
     typedef Stream<T, DK, DV, NW, true, 2> V;
-    T k[CHUNK * V::LA], q[CHUNK * V::LA], o[CHUNK * V::LC], v[CHUNK * V::LC];
+    T k[CHUNK * V::PA], q[CHUNK * V::PA], o[CHUNK * V::PC], v[CHUNK * V::PC];
     typename V::Op scores[2][V::PAIRS * V::S2 * 64];
 };
 template <typename T, int DK, int DV, int NW, bool VEC, bool SLOPE>
@@ -693,7 +703,7 @@ __device__ __forceinline__ void pair_sweep(const Pass &P, int item, PairLds<T, D
     typedef typename V::Op Op;
     constexpr int NT = 64 * NW;
     T *const lk = lds.k, *const lq = lds.q, *const lo = lds.o, *const lv = lds.v;
-    Op *const scores[2] = {lds.scores[0], lds.scores[1]};
+    Op *const scores_k = lds.scores[0], *const scores_v = lds.scores[1];
     const int tid_ = here(threadIdx.x), tid = tid_, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, li = lane & 15;
     const int h = item % P.heads, slot = item / P.heads;
     const bool packed = P.offsets != nullptr;
@@ -726,8 +736,8 @@ __device__ __forceinline__ void pair_sweep(const Pass &P, int item, PairLds<T, D
     Weights<NW> w;
     w.init(P.log_decay[h], P.upd_scale, 1, wave, g, li);
     if (wave == 0) {
-        V::clear_scores(scores[0], lane);
-        V::clear_scores(scores[1], lane);
+        V::clear_scores(scores_k, lane);
+        V::clear_scores(scores_v, lane);
     }
     const int64_t state_at = ((int64_t)at.n_seq * P.heads + h) * P.da * P.dc;
     const float *from = !at.last ? P.seg + (int64_t)item * P.da * P.dc : P.state_in ? P.state_in + state_at : nullptr;
@@ -745,34 +755,38 @@ __device__ __forceinline__ void pair_sweep(const Pass &P, int item, PairLds<T, D
         so.template store<FULL>(lo, po, P.c, t, n, tid);
         sv.template store<FULL>(lv, pv, P.e, t, n, tid);
         __syncthreads();
+        f32x4 F[SLOPE ? K::TA : 1][K::CT];         // the state that entered this chunk ascending
+        if (SLOPE) {
+            const f32x4 *from = (const f32x4 *)chunk_states + (((t - at.t0) / CHUNK * NW + wave) * K::TA * K::CT) * 64 + lane;
+#pragma unroll
+            for (int mt = 0; mt < K::TA; ++mt)
+#pragma unroll
+                for (int ct = 0; ct < K::CT; ++ct) F[mt][ct] = from[(mt * K::CT + ct) * 64];
+        }
         fetch(next, tid);
         float sum = 0.0f;
 #pragma unroll
         for (int m = 0; m < w.MINE; ++m) {
             const int it = w.it[m], jt = w.jt[m];
             if (it >= R::LIVE) continue;
-            f32x4 s1 = V::score(lk, lq, it, jt, g, li), s2 = K::score(lv, lo, it, jt, g, li);
+            f32x4 sv = V::score(lk, lq, it, jt, g, li), sk = K::score(lv, lo, it, jt, g, li);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                s1[r] *= w.wa[m][r];
-                if (SLOPE) sum += (float)w.apart(m, r, g, li) * s1[r] * s2[r];
-                s2[r] *= w.wa[m][r];
+                sv[r] *= w.wa[m][r];
+                if (SLOPE) sum += (float)w.apart(m, r, g, li) * sv[r] * sk[r];
+                sk[r] *= w.wa[m][r];
             }
-            V::keep(s1, scores[0], it, jt, lane);
-            V::keep(s2, scores[1], it, jt, lane);
+            V::keep(sv, scores_v, it, jt, lane);
+            K::keep(sk, scores_k, it, jt, lane);
         }
-        phase();
         if (SLOPE) {
-            const f32x4 *from = (const f32x4 *)chunk_states + (((t - at.t0) / CHUNK * NW + wave) * K::TA * K::CT) * 64 + lane;
             float cross = 0.0f;
 #pragma unroll
             for (int mt = 0; mt < K::TA; ++mt)
 #pragma unroll
-                for (int ct = 0; ct < K::CT; ++ct) {
-                    const f32x4 F = from[(mt * K::CT + ct) * 64];
+                for (int ct = 0; ct < K::CT; ++ct)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) cross += F[r] * xk.S[mt][ct][r];
-                }
+                    for (int r = 0; r < 4; ++r) cross += F[mt][ct][r] * xk.S[mt][ct][r];
             sum += (float)n * power(w.lg2, n) * cross;
         }
         const int64_t row0 = (packed ? 0 : (int64_t)at.n_seq * P.rows) + at.lo + t;
@@ -782,13 +796,14 @@ __device__ __forceinline__ void pair_sweep(const Pass &P, int item, PairLds<T, D
         __syncthreads();
         phase();
         xk.columns(lq, wave, g, li);
-        xk.template from_rows<R, true>(scores[1], n, 1.0f, P.out2, P.out2_f32, row0, P.heads, h, P.da, wave, lane);
+        xk.template from_rows<R, true>(scores_k, n, 1.0f, P.out2, P.out2_f32, row0, P.heads, h, P.da, wave, lane);
         phase();
         xk.template advance<R>(lo, n, w, P.upd_scale, 1, g, li);
+        phase();
         xv.template from_state<R>(lk, n, w, g, li);
         phase();
         xv.columns(lo, wave, g, li);
-        xv.template from_rows<R, true>(scores[0], n, 1.0f, P.out, P.out_f32, row0, P.heads, h, P.dc, wave, lane);
+        xv.template from_rows<R, true>(scores_v, n, 1.0f, P.out, P.out_f32, row0, P.heads, h, P.dc, wave, lane);
         phase();
         xv.template advance<R>(lq, n, w, P.upd_scale, 1, g, li);
         __syncthreads();

@@ -27,7 +27,7 @@ template <bool VEC, int DA, int DC> int launch(const Work &w, hipStream_t st) {
     hipLaunchKernelGGL((td_decay_sum_kernel<T, DA, DC, NW, VEC, true, size <= 128 ? 4 : 2>), grid, block, 0, st, P);
 #else
     const int64_t held = (int64_t)((P.seg_len + CHUNK - 1) / CHUNK) * DA * DC;
-    hipLaunchKernelGGL((td_decay_backward_kernel<T, DA, DC, NW, VEC, TD_INST_KIND == 4, size <= 128 ? 2 : 1>), dim3((unsigned)w.groups), block, 0, st, w.p, w.r,
+    hipLaunchKernelGGL((td_decay_backward_kernel<T, DA, DC, NW, VEC, TD_INST_KIND == 4, size <= 64 || (size <= 128 && TD_INST_BF16) ? 2 : 1>), dim3((unsigned)w.groups), block, 0, st, w.p, w.r,
                        w.chunk_states, held, w.ascending, w.descending);
 #endif
     TD_LAUNCH_CHECK();
