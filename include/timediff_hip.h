@@ -360,7 +360,8 @@ typedef struct td_decay_config {
                                                                         dimension of every tensor is contiguous */
 } td_decay_config;
 
-/* Scratch of one forward (backward = 0) or backward (1) call; 0 with td_last_error() set for a bad configuration. */
+/* Scratch of one forward (backward = 0) or backward (1) call; 0 with td_last_error() set for a bad configuration.  A forward call
+ * that asks for 256 uses none and takes NULL. */
 TD_API size_t td_decay_workspace_bytes(const td_decay_config *cfg, int32_t backward);
 /* o: (.., rows, heads, dv) contiguous; state_in, state_out: (n_seq, heads, dk, dv) float32 or NULL (not the same memory). */
 TD_API int td_decay_forward(const td_decay_config *cfg, const void *q, const void *k, const void *v, const float *log_decay,

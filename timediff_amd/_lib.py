@@ -132,12 +132,13 @@ _SIGS = {
     "td_cls_workspace_bytes": (C.c_size_t, [C.POINTER(RnnConfig), _I, _I]),
     "td_cls_forward": (C.c_int, [C.POINTER(RnnConfig), _P, _P, _P, _P, _I, _I, _P, _P, _P]),
     "td_cls_backward": (C.c_int, [C.POINTER(RnnConfig), _P, _P, _P, _P, _P, _I, _I, _P, C.POINTER(_P), _P, _P, _P]),
-    "td_decay_workspace_bytes": (C.c_size_t, [C.POINTER(DecayConfig), _I]),
-    "td_decay_forward": (C.c_int, [C.POINTER(DecayConfig)] + [_P] * 10),
-    "td_decay_backward": (C.c_int, [C.POINTER(DecayConfig)] + [_P] * 15),
-    "td_decay_step": (C.c_int, [C.POINTER(DecayConfig)] + [_P] * 7),
-    "td_adamw": (C.c_int, [C.POINTER(AdamwConfig), C.POINTER(AdamwTensor), _I, _P]),
-    "td_adamw_record_set": (C.c_int, [_P, C.POINTER(AdamwConfig), _P]),
+    # (configurations and tensor lists by address: ctypes.byref of their structures, or their bytes)
+    "td_decay_workspace_bytes": (C.c_size_t, [_P, _I]),
+    "td_decay_forward": (C.c_int, [_P] * 11),
+    "td_decay_backward": (C.c_int, [_P] * 16),
+    "td_decay_step": (C.c_int, [_P] * 8),
+    "td_adamw": (C.c_int, [_P, _P, _I, _P]),
+    "td_adamw_record_set": (C.c_int, [_P, _P, _P]),
     "td_set_head_fusion": (C.c_int, [_I]),
     "td_set_side_gemm": (C.c_int, [_I]),
     "td_set_step_launch": (C.c_int, [_I]),

@@ -214,6 +214,7 @@ int share_sum(const td_decay_config *c, const float *parts, void *grad, int own_
     return TD_OK;
 }
 
+constexpr size_t NO_WORKSPACE = 256;      // what a call that uses none asks for: 0 says that the configuration is bad
 struct Layout { size_t seg, seg2, chunks, slope, parts, parts2, total; };
 Layout layout(const td_decay_config *c, bool backward) {
     int len, segs;
@@ -230,7 +231,7 @@ Layout layout(const td_decay_config *c, bool backward) {
     w.parts = w.slope + (backward ? up256(2 * (size_t)slots * c->heads * sizeof(double)) : 0);
     const bool q = c->q_heads != c->heads, k = c->k_heads != c->heads, v = c->v_heads != c->heads;
     w.parts2 = w.parts + (backward && q ? up256(rows * c->dk) : 0);
-    w.total = w.parts2 + (backward ? (k ? up256(rows * c->dk) : 0) + (v ? up256(rows * c->dv) : 0) : 0) + 256;
+    w.total = w.parts2 + (backward ? (k ? up256(rows * c->dk) : 0) + (v ? up256(rows * c->dv) : 0) : 0) + NO_WORKSPACE;
     return w;
 }
 
@@ -246,7 +247,7 @@ extern "C" size_t td_decay_workspace_bytes(const td_decay_config *cfg, int32_t b
 extern "C" int td_decay_forward(const td_decay_config *cfg, const void *q, const void *k, const void *v, const float *log_decay,
                                 const int32_t *offsets, const float *state_in, void *o, float *state_out, void *workspace, void *stream) {
     if (int rc = check_config(cfg)) return rc;
-    TD_REQUIRE(log_decay && workspace && (cfg->rows == 0 || (q && k && v && o)), "null pointer");
+    TD_REQUIRE(log_decay && (workspace || layout(cfg, false).total == NO_WORKSPACE) && (cfg->rows == 0 || (q && k && v && o)), "null pointer");
     TD_REQUIRE(!cfg->packed || offsets, "packed sequences need offsets");
     TD_REQUIRE(!state_out || state_out != state_in, "state_in and state_out must not be the same memory");
     hipStream_t st = (hipStream_t)stream;

@@ -3,12 +3,14 @@
 torch is used for device memory and stream handles only; every computation below runs in
 libtimediff_hip.so.  All tensors must live on the current ROCm device.
 """
+import contextlib
 import ctypes as C
+import struct
 
 import torch
 
 from . import _lib
-from ._lib import DecayConfig, DiffusionConfig, Rng, RnnConfig, check, lib, ptr, ptr_table
+from ._lib import DiffusionConfig, Rng, RnnConfig, check, lib, ptr, ptr_table
 
 
 def _stream():
@@ -334,37 +336,53 @@ class SamplerKernels:
 
 # -- decay attention (timediff_amd/decay_attention.py is the differentiable front) ------------------------------------------
 _ELEMENT = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
+_DECAY_FIELDS = struct.Struct("<10ifi12q")      # td_decay_config, packed in one call: these calls are as short as their launches
+_NO_WORKSPACE = 256                             # td_decay_workspace_bytes of a call that uses none
+
+
+def _on_device(index):
+    """A context for launches on device `index`: nothing where it is the current one."""
+    return _NOTHING if index == torch.cuda.current_device() else torch.cuda.device(index)
+
+
+_NOTHING = contextlib.nullcontext()
+
+
+def _raw_stream(index):
+    return torch.cuda.current_stream(index).cuda_stream
 
 
 def decay_check(q, k, v, log_decay, offsets=None, state=None, step=False):
     """Raises ValueError / TypeError where shapes, types or devices do not fit (td_decay_config's limits are the library's)."""
     lead = 1 if step or offsets is not None else 2
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        if t.dim() != lead + 2:
-            raise ValueError(f"{name} must have {lead + 2} dimensions, got shape {tuple(t.shape)}")
-        if t.dtype not in _ELEMENT or t.dtype != q.dtype:
+    qs, ks, vs, ls = q.shape, k.shape, v.shape, log_decay.shape
+    for name, t, shape in (("q", q, qs), ("k", k, ks), ("v", v, vs)):
+        if len(shape) != lead + 2:
+            raise ValueError(f"{name} must have {lead + 2} dimensions, got shape {tuple(shape)}")
+        if t.dtype not in _ELEMENT or t.dtype is not q.dtype:
             raise TypeError(f"q, k and v must all be float32 or all bfloat16, got {name} {t.dtype} and q {q.dtype}")
-        if t.shape[:lead] != q.shape[:lead]:
-            raise ValueError(f"q, k and v must agree in their leading dimensions, got {name} {tuple(t.shape)} and q {tuple(q.shape)}")
-    if k.shape[-1] != q.shape[-1]:
-        raise ValueError(f"q and k must agree in their last dimension, got {q.shape[-1]} and {k.shape[-1]}")
-    if log_decay.dim() != 1 or log_decay.dtype != torch.float32:
-        raise ValueError(f"log_decay must be a float32 vector, got {log_decay.dtype} of shape {tuple(log_decay.shape)}")
-    H = log_decay.shape[0]
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        if H < 1 or t.shape[-2] < 1 or H % t.shape[-2]:
-            raise ValueError(f"the heads of {name} ({t.shape[-2]}) must divide those of log_decay ({H})")
-        if not 1 <= t.shape[-1] <= _lib.DECAY_MAX_DIM:
-            raise ValueError(f"the last dimension of {name} must be 1 .. {_lib.DECAY_MAX_DIM}, got {t.shape[-1]}")
-    n = q.shape[0]
+        if shape[:lead] != qs[:lead]:
+            raise ValueError(f"q, k and v must agree in their leading dimensions, got {name} {tuple(shape)} and q {tuple(qs)}")
+    if ks[-1] != qs[-1]:
+        raise ValueError(f"q and k must agree in their last dimension, got {qs[-1]} and {ks[-1]}")
+    if len(ls) != 1 or log_decay.dtype is not torch.float32:
+        raise ValueError(f"log_decay must be a float32 vector, got {log_decay.dtype} of shape {tuple(ls)}")
+    H = ls[0]
+    for name, shape in (("q", qs), ("k", ks), ("v", vs)):
+        if H < 1 or shape[-2] < 1 or H % shape[-2]:
+            raise ValueError(f"the heads of {name} ({shape[-2]}) must divide those of log_decay ({H})")
+        if not 1 <= shape[-1] <= _lib.DECAY_MAX_DIM:
+            raise ValueError(f"the last dimension of {name} must be 1 .. {_lib.DECAY_MAX_DIM}, got {shape[-1]}")
+    n = qs[0]
     if offsets is not None:
-        if offsets.dim() != 1 or offsets.dtype != torch.int32 or offsets.shape[0] < 2:
+        if offsets.dim() != 1 or offsets.dtype is not torch.int32 or offsets.shape[0] < 2:
             raise ValueError(f"offsets must be an int32 vector of at least 2 entries, got {offsets.dtype} of shape {tuple(offsets.shape)}")
         n = offsets.shape[0] - 1
-    if state is not None and (state.dtype != torch.float32 or tuple(state.shape) != (n, H, q.shape[-1], v.shape[-1])):
-        raise ValueError(f"the state must be float32 of shape {(n, H, q.shape[-1], v.shape[-1])}, got {state.dtype} of {tuple(state.shape)}")
+    if state is not None and (state.dtype is not torch.float32 or state.shape != (n, H, qs[-1], vs[-1])):
+        raise ValueError(f"the state must be float32 of shape {(n, H, qs[-1], vs[-1])}, got {state.dtype} of {tuple(state.shape)}")
+    index = q.get_device()
     for t in (q, k, v, log_decay, offsets, state):
-        if t is not None and (not t.is_cuda or t.device != q.device):
+        if t is not None and (index < 0 or t.get_device() != index):
             raise ValueError(f"all tensors must be on one ROCm device, got {t.device} and {q.device}")
 
 
@@ -373,46 +391,62 @@ def _rows(t):
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
-def _decay_config(q, k, v, log_decay, scale, offsets, grad_o=None):
-    c = DecayConfig(n_seq=q.shape[0] if offsets is None else offsets.shape[0] - 1, rows=q.shape[1] if offsets is None else q.shape[0],
-                    packed=int(offsets is not None), heads=log_decay.shape[0], q_heads=q.shape[-2], k_heads=k.shape[-2],
-                    v_heads=v.shape[-2], dk=q.shape[-1], dv=v.shape[-1], dtype=_ELEMENT[q.dtype], scale=scale)
-    for field, t in ((c.q_stride, q), (c.k_stride, k), (c.v_stride, v), (c.grad_o_stride, grad_o)):
-        if t is not None:
-            field[0], field[1], field[2] = (0,) * (offsets is not None) + tuple(t.stride()[:-1])
-    return c
+def _decay_config(q, k, v, log_decay, scale, offsets, grad_o=None, step=False):
+    """td_decay_config as bytes: the library only reads it."""
+    qs, ks, vs = q.shape, k.shape, v.shape
+    packed = offsets is not None
+    n, rows = (offsets.shape[0] - 1, qs[0]) if packed else (qs[0], 1 if step else qs[1])
+    strides = []
+    for t in (q, k, v, grad_o):
+        if t is None:
+            strides += (0, 0, 0)
+        elif packed:
+            strides += (0, *t.stride()[:2])
+        elif step:
+            x = t.stride()
+            strides += (x[0], 0, x[1])
+        else:
+            strides += t.stride()[:3]
+    return _DECAY_FIELDS.pack(n, rows, packed, log_decay.shape[0], qs[-2], ks[-2], vs[-2], qs[-1], vs[-1], _ELEMENT[q.dtype], scale, 0, *strides)
 
 
 def _decay_workspace(cfg, backward, device):
-    need = lib().td_decay_workspace_bytes(C.byref(cfg), backward)
+    need = lib().td_decay_workspace_bytes(cfg, backward)
     if need == 0:
         raise _lib.TimediffError(lib().td_last_error().decode())
-    return torch.empty(need, dtype=torch.uint8, device=device)
+    return None if need == _NO_WORKSPACE else torch.empty(need, dtype=torch.uint8, device=device)
+
+
+def _address(t):
+    return None if t is None else t.data_ptr()
 
 
 def decay_forward(q, k, v, log_decay, scale, offsets=None, state=None, want_state=False):
     """-> (o, state after the last row or None); arguments as decay_check accepts them."""
     q, k, v, log_decay = _rows(q), _rows(k), _rows(v), log_decay.contiguous()
-    with torch.cuda.device(q.device):
-        o = torch.empty(*q.shape[:-2], log_decay.shape[0], v.shape[-1], dtype=q.dtype, device=q.device)
+    device, index = q.device, q.get_device()
+    H, Dv = log_decay.shape[0], v.shape[-1]
+    with _on_device(index):
+        o = torch.empty((*q.shape[:-2], H, Dv), dtype=q.dtype, device=device)
         n = q.shape[0] if offsets is None else offsets.shape[0] - 1
-        out = torch.empty(n, log_decay.shape[0], q.shape[-1], v.shape[-1], dtype=torch.float32, device=q.device) if want_state else None
+        out = torch.empty((n, H, q.shape[-1], Dv), dtype=torch.float32, device=device) if want_state else None
         if n:
             state = None if state is None else state.contiguous()
             offsets = None if offsets is None else offsets.contiguous()
             cfg = _decay_config(q, k, v, log_decay, scale, offsets)
-            ws = _decay_workspace(cfg, 0, q.device)
-            check(lib().td_decay_forward(C.byref(cfg), ptr(q), ptr(k), ptr(v), ptr(log_decay), ptr(offsets), ptr(state), ptr(o), ptr(out),
-                                         ptr(ws), _stream()))
+            ws = _decay_workspace(cfg, 0, device)
+            check(lib().td_decay_forward(cfg, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), _address(offsets), _address(state),
+                                         o.data_ptr(), _address(out), _address(ws), _raw_stream(index)))
     return o, out
 
 
 def decay_backward(q, k, v, log_decay, scale, grad_o, offsets=None, state=None, grad_state=None, want=(True,) * 5):
     """-> gradients of (q, k, v, log_decay, state), None where `want` says so."""
     q, k, v, log_decay, grad_o = _rows(q), _rows(k), _rows(v), log_decay.contiguous(), _rows(grad_o)
-    with torch.cuda.device(q.device):
-        new = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if w else None for t, w in zip((q, k, v, log_decay), want)]
-        d_state = torch.empty(state.shape, dtype=torch.float32, device=q.device) if state is not None and want[4] else None
+    device, index = q.device, q.get_device()
+    with _on_device(index):
+        new = [torch.empty(t.shape, dtype=t.dtype, device=device) if w else None for t, w in zip((q, k, v, log_decay), want)]
+        d_state = torch.empty(state.shape, dtype=torch.float32, device=device) if state is not None and want[4] else None
         if (q.shape[0] if offsets is None else offsets.shape[0] - 1) == 0:
             if new[3] is not None:
                 new[3].zero_()
@@ -421,9 +455,9 @@ def decay_backward(q, k, v, log_decay, scale, grad_o, offsets=None, state=None, 
         offsets = None if offsets is None else offsets.contiguous()
         grad_state = None if grad_state is None else grad_state.to(torch.float32).contiguous()
         cfg = _decay_config(q, k, v, log_decay, scale, offsets, grad_o)
-        ws = _decay_workspace(cfg, 1, q.device)
-        check(lib().td_decay_backward(C.byref(cfg), ptr(q), ptr(k), ptr(v), ptr(log_decay), ptr(offsets), ptr(state), ptr(grad_o),
-                                      ptr(grad_state), *[ptr(t) for t in new], ptr(d_state), ptr(ws), _stream()))
+        ws = _decay_workspace(cfg, 1, device)
+        check(lib().td_decay_backward(cfg, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), _address(offsets), _address(state),
+                                      grad_o.data_ptr(), _address(grad_state), *map(_address, new), _address(d_state), _address(ws), _raw_stream(index)))
     return (*new, d_state)
 
 
@@ -433,9 +467,10 @@ def decay_step(q, k, v, log_decay, state, scale):
     if not state.is_contiguous():
         raise ValueError("the state must be contiguous: it is updated in place")
     q, k, v, log_decay = _rows(q), _rows(k), _rows(v), log_decay.contiguous()
-    with torch.cuda.device(q.device):
-        o = torch.empty(q.shape[0], log_decay.shape[0], v.shape[-1], dtype=q.dtype, device=q.device)
+    index = q.get_device()
+    with _on_device(index):
+        o = torch.empty((q.shape[0], log_decay.shape[0], v.shape[-1]), dtype=q.dtype, device=q.device)
         if q.shape[0]:
-            cfg = _decay_config(q.unsqueeze(1), k.unsqueeze(1), v.unsqueeze(1), log_decay, scale, None)
-            check(lib().td_decay_step(C.byref(cfg), ptr(q), ptr(k), ptr(v), ptr(log_decay), ptr(state), ptr(o), _stream()))
+            check(lib().td_decay_step(_decay_config(q, k, v, log_decay, scale, None, step=True), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                                      log_decay.data_ptr(), state.data_ptr(), o.data_ptr(), _raw_stream(index)))
     return o

@@ -4,7 +4,10 @@
 costs 2 bytes of state instead of 8: exp_avg holds m and exp_avg_sq holds sqrt(v) as float8_e4m3fn, times one float32 scale
 for each 256 values (a moment's value is code.float() * scale), rounded stochastically.  No counterpart in the reference.
 """
+import array
 import ctypes as C
+import operator
+import struct
 
 import torch
 
@@ -12,14 +15,9 @@ from . import _lib, ops
 from ._lib import ADAMW_BLOCK, AdamwConfig, AdamwRecord, check, lib, ptr
 
 
-def _check_list(name, tensors, like, dtypes):
-    if len(tensors) != len(like):
-        raise ValueError(f"{len(tensors)} {name} for {len(like)} params")
-    kinds = {t.dtype for t in tensors}
-    if not kinds <= dtypes:
-        raise TypeError(f"{name} must be {' or '.join(sorted(str(d) for d in dtypes))}, got {', '.join(sorted(str(d) for d in kinds - dtypes))}")
-    if not all(map(torch.Tensor.is_contiguous, tensors)):
-        raise ValueError(f"{name} must be contiguous")
+_DTYPE, _NUMEL, _ADDRESS = operator.attrgetter("dtype"), torch.Tensor.numel, torch.Tensor.data_ptr
+_CONTIGUOUS, _DEVICE = torch.Tensor.is_contiguous, torch.Tensor.get_device
+_F32, _GRADS, _E4M3, _WORDS = {torch.float32}, {torch.float32, torch.bfloat16}, {torch.float8_e4m3fn}, {torch.int32}
 
 
 def adamw_(params, grads, exp_avgs, exp_avg_sqs, scales=None, *, lr, betas, eps, weight_decay, step, grad_scale=None, random=None,
@@ -35,42 +33,45 @@ def adamw_(params, grads, exp_avgs, exp_avg_sqs, scales=None, *, lr, betas, eps,
     if not params:
         return
     bits = 32 if scales is None else 8
-    state = {torch.float32} if bits == 32 else {torch.float8_e4m3fn}
-    lists = [("params", params, {torch.float32}), ("grads", grads, {torch.float32, torch.bfloat16}), ("exp_avgs", exp_avgs, state),
-             ("exp_avg_sqs", exp_avg_sqs, state)]
-    n = list(map(torch.Tensor.numel, params))
+    n = list(map(_NUMEL, params))
+    state = _F32 if bits == 32 else _E4M3
+    # (every pass over a list is one C loop: a step over hundreds of tensors is as long as these)
+    lists = [("params", params, _F32, n), ("grads", grads, _GRADS, n), ("exp_avgs", exp_avgs, state, n), ("exp_avg_sqs", exp_avg_sqs, state, n)]
     if bits == 8:
-        lists.append(("scales", scales, {torch.float32}))
-        if list(map(torch.Tensor.numel, scales)) != [2 * -(-k // ADAMW_BLOCK) for k in n]:
-            raise ValueError(f"scales must have 2 values for each {ADAMW_BLOCK} of their param")
+        lists.append(("scales", scales, _F32, [2 * -(-k // ADAMW_BLOCK) for k in n]))
         if random is not None:
-            lists.append(("random", random, {torch.int32}))
+            lists.append(("random", random, _WORDS, n))
     elif random is not None:
         raise ValueError("random is for 8-bit moments")
-    for name, tensors, dtypes in lists:
-        _check_list(name, tensors, params, dtypes)
-        if name not in ("params", "scales") and list(map(torch.Tensor.numel, tensors)) != n:
-            raise ValueError(f"{name} must have their params' sizes")
-    for name, tensors, _ in lists:
-        if set(map(torch.Tensor.get_device, tensors)) != {params[0].get_device()} or not params[0].is_cuda:
+    for name, tensors, dtypes, sizes in lists:
+        if len(tensors) != len(n):
+            raise ValueError(f"{len(tensors)} {name} for {len(n)} params")
+        kinds = set(map(_DTYPE, tensors))
+        if not kinds <= dtypes:
+            raise TypeError(f"{name} must be {' or '.join(sorted(map(str, dtypes)))}, got {', '.join(sorted(map(str, kinds - dtypes)))}")
+        if not all(map(_CONTIGUOUS, tensors)):
+            raise ValueError(f"{name} must be contiguous")
+        if name != "params" and list(map(_NUMEL, tensors)) != sizes:
+            raise ValueError(f"scales must have 2 values for each {ADAMW_BLOCK} of their param" if name == "scales" else f"{name} must have their params' sizes")
+    index = params[0].get_device()
+    for name, tensors, *_ in lists:
+        if index < 0 or set(map(_DEVICE, tensors)) != {index}:
             raise ValueError(f"{name} must be on one ROCm device, the params'")
-    if grad_scale is not None and (grad_scale.dtype != torch.float32 or grad_scale.numel() != 1 or grad_scale.device != params[0].device):
+    if grad_scale is not None and (grad_scale.dtype is not torch.float32 or grad_scale.numel() != 1 or grad_scale.get_device() != index):
         raise ValueError("grad_scale must be one float32 value on the params' device")
-    _launch(lists, n, AdamwConfig(lr=lr, beta1=betas[0], beta2=betas[1], eps=eps, weight_decay=weight_decay, step=step, seed=seed,
-                                  grad_scale=None if grad_scale is None else grad_scale.data_ptr(),
-                                  record=None if record is None else record.data_ptr(), state_bits=bits))
+    table = array.array("q", bytes(64 * len(n)))          # td_adamw_tensor is eight 64-bit words
+    for word, (_, tensors, *_) in enumerate(lists):
+        table[word::8] = array.array("q", map(_ADDRESS, tensors))
+    table[6::8] = array.array("q", n)
+    if set(map(_DTYPE, grads)) != _F32:
+        table[7::8] = array.array("q", [_lib.F32 if g.dtype is torch.float32 else _lib.BF16 for g in grads])
+    cfg = _CONFIG.pack(lr, betas[0], betas[1], eps, weight_decay, step, seed, 0 if grad_scale is None else grad_scale.data_ptr(),
+                       0 if record is None else record.data_ptr(), bits, 0)
+    with ops._on_device(index):
+        check(lib().td_adamw(cfg, table.buffer_info()[0], len(n), ops._raw_stream(index)))
 
 
-def _launch(lists, n, cfg):
-    """lists: params, grads, exp_avgs, exp_avg_sqs[, scales[, random]] as (name, tensors, ..)."""
-    count = len(n)
-    table = (C.c_uint64 * (8 * count))()         # td_adamw_tensor is eight 64-bit words
-    for word, (_, tensors, *_rest) in enumerate(lists):
-        table[word::8] = list(map(torch.Tensor.data_ptr, tensors))
-    table[6::8] = n
-    table[7::8] = [_lib.F32 if g.dtype is torch.float32 else _lib.BF16 for g in lists[1][1]]
-    with torch.cuda.device(lists[0][1][0].device):
-        check(lib().td_adamw(C.byref(cfg), C.cast(table, C.POINTER(_lib.AdamwTensor)), count, ops._stream()))
+_CONFIG = struct.Struct("<5dqQQQii")            # td_adamw_config
 
 
 class AdamW(torch.optim.Optimizer):
