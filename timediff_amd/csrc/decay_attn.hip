@@ -62,14 +62,15 @@ template <bool REV> __global__ __launch_bounds__(256) void td_decay_scan_kernel(
     }
 }
 
-// grad_log_decay[h] = the sum of head h's parts, in their order
-__global__ __launch_bounds__(256) void td_decay_slope_kernel(const double *parts, int n, int heads, float *grad) {
-    __shared__ double red[256];
+// grad_log_decay[h] = the sum of head h's parts, in an order of their own
+__global__ __launch_bounds__(1024) void td_decay_slope_kernel(const double *parts, int n, int heads, float *grad) {
+    __shared__ double red[1024];
     double s = 0.0;
-    for (int i = threadIdx.x; i < n; i += 256) s += parts[(int64_t)i * heads + blockIdx.x];
+#pragma unroll 4
+    for (int i = threadIdx.x; i < n; i += 1024) s += parts[(int64_t)i * heads + blockIdx.x];
     red[threadIdx.x] = s;
     __syncthreads();
-    for (int o = 128; o > 0; o >>= 1) {
+    for (int o = 512; o > 0; o >>= 1) {
         if ((int)threadIdx.x < o) red[threadIdx.x] += red[threadIdx.x + o];
         __syncthreads();
     }
@@ -134,7 +135,10 @@ size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 
 int esize(const td_decay_config *c) { return c->dtype == TD_BF16 ? 2 : 4; }
 
-View view(const td_decay_config *c, const void *p, const int64_t *s, int own, int d) { return View{p, s[0], s[1], s[2], c->heads / own, d}; }
+View view(const td_decay_config *c, const void *p, const int64_t *s, int own, int d) {
+    const bool even = (uintptr_t)p % 4 == 0 && d % 2 == 0 && s[0] % 2 == 0 && s[1] % 2 == 0 && s[2] % 2 == 0;
+    return View{p, s[0], s[1], s[2], c->heads / own, d, even};
+}
 
 // Whether a tensor can be read 16 bytes at a time, a chunk's rows at 32-bit offsets from its first (24 bits of row stride)
 bool wide(const td_decay_config *c, const View &v) {
@@ -316,7 +320,7 @@ extern "C" int td_decay_backward(const td_decay_config *cfg, const void *q, cons
     if (grad_k && k_shared)
         if (int rc = share_sum(cfg, parts_k, grad_k, cfg->k_heads, cfg->dk, st)) return rc;
     if (slope) {
-        hipLaunchKernelGGL(td_decay_slope_kernel, dim3(cfg->heads), dim3(256), 0, st, slopes, 2 * Q.slots, cfg->heads, grad_log_decay);
+        hipLaunchKernelGGL(td_decay_slope_kernel, dim3(cfg->heads), dim3(1024), 0, st, slopes, 2 * Q.slots, cfg->heads, grad_log_decay);
         TD_LAUNCH_CHECK();
     }
     return TD_OK;

@@ -25,6 +25,7 @@ struct View {                 // rows of one tensor; head h of the recurrence re
     const void *p;
     int64_t seq, row, head;
     int share, d;
+    int pairs;                // bfloat16: two neighbours can be read at once
 };
 
 struct Pass {
@@ -177,23 +178,37 @@ template <> struct Mat<float> {
 };
 
 // One chunk's rows of one tensor on their way from memory to LDS.  Memory is read in the order of its rows (n of them from `low` on), a
-// reversed pass turns them round in LDS.  VEC: 16 bytes a load, at 32-bit offsets from the chunk's first row, into registers that are filled
-// while the chunk before it is computed (unless there are too many).  These loads are never skipped, so that their registers have one writer:
-// a lane without a row or a column of its own reads its neighbours', and nothing of that is stored.  Else (odd sizes, strides or addresses)
-// element by element when the chunk begins.
-template <typename T, int D, int NT, bool VEC, bool REV> struct Stage {
-    static constexpr int PER = Mat<T>::VEC, PIECES = D / PER, N = VEC ? CHUNK * PIECES / NT : 1;
-    static constexpr bool AHEAD = VEC && N <= 4;
+// reversed pass turns them round in LDS.  The loads go into registers while the chunk before is computed (unless there are too many of them):
+// WIDE: 16 bytes each, at 32-bit offsets from the chunk's first row; else (odd sizes, strides or addresses) 4 bytes each.  They are never
+// skipped, so that their registers have one writer: a lane without a row or a column of its own reads its neighbours', and
+// nothing of that is stored.
+template <typename T, int D, int NT, bool WIDE, bool REV> struct Stage {
+    static constexpr int BYTES = WIDE ? 16 : 4, PER = BYTES / sizeof(T), PIECES = D / PER, N = CHUNK * PIECES / NT;
+    static constexpr bool AHEAD = N * BYTES <= 64;
     static_assert(NT % PIECES == 0, "a thread's pieces share their columns");
-    uint4 r[AHEAD ? N : 1];
+    struct Wide { uint4 x; };
+    struct Narrow { uint32_t x; };
+    template <bool W, typename A, typename B> struct Pick { typedef A Type; };
+    template <typename A, typename B> struct Pick<false, A, B> { typedef B Type; };
+    typedef decltype(Pick<WIDE, Wide, Narrow>::Type::x) Piece;
+    Piece r[AHEAD ? N : 1];
     // the columns behind the last are zeros from here on
     static __device__ __forceinline__ void init(T *lds, const View &v, int tid) {
-        if (VEC && v.d < D)
+        if (v.d < D)
             for (int i = tid; i < CHUNK * Mat<T>::pitch(D); i += NT) lds[i] = (T)0.0f;
     }
-    static __device__ __forceinline__ uint4 piece(const char *chunk, const View &v, int c, int n, int tid) {
-        const int row = min(tid / PIECES + c * (NT / PIECES), n - 1), col = min(tid % PIECES * PER, v.d - PER);
-        return *(const uint4 *)(chunk + (uint32_t)(__umul24(row, (uint32_t)v.row * sizeof(T)) + col * sizeof(T)));
+    static __device__ __forceinline__ Piece piece(const char *chunk, const View &v, int c, int n, int tid) {
+        const int row = min(tid / PIECES + c * (NT / PIECES), n - 1), own = tid % PIECES * PER;
+        if constexpr (WIDE) {
+            const int col = min(own, v.d - PER);
+            return *(const uint4 *)(chunk + (uint32_t)(__umul24(row, (uint32_t)v.row * sizeof(T)) + col * sizeof(T)));
+        } else if constexpr (sizeof(T) == 4) {
+            return *(const uint32_t *)(chunk + (row * v.row + min(own, v.d - 1)) * (int64_t)sizeof(T));
+        } else {
+            const uint16_t *p = (const uint16_t *)chunk + row * v.row;
+            if (v.pairs) return *(const uint32_t *)(p + min(own, v.d - 2));
+            return (uint32_t)p[min(own, v.d - 1)] | (own + 1 < v.d ? (uint32_t)p[min(own + 1, v.d - 1)] << 16 : 0u);
+        }
     }
     // n >= 1
     __device__ __forceinline__ void load(const T *base, const View &v, int low, int n, int tid) {
@@ -203,23 +218,16 @@ template <typename T, int D, int NT, bool VEC, bool REV> struct Stage {
         for (int c = 0; c < N; ++c) r[c] = piece(chunk, v, c, n, tid);
     }
     template <bool FULL> __device__ __forceinline__ void store(T *lds, const T *base, const View &v, int low, int n, int tid) const {
-        if (!VEC) {
-            const T *p = base + (int64_t)low * v.row;
-#pragma unroll 4
-            for (int i = tid; i < CHUNK * D; i += NT) {
-                const int row = i / D, col = i % D, to = REV && row < n ? n - 1 - row : row;
-                lds[Mat<T>::four_at(D, to, col >> 2) + (col & 3)] = row < n && col < v.d ? p[row * v.row + col] : (T)0.0f;
-            }
-            return;
-        }
         if (tid % PIECES * PER >= v.d) return;
         const char *chunk = (const char *)(base + (int64_t)low * v.row);
 #pragma unroll
         for (int c = 0; c < N; ++c) {
             const int row = tid / PIECES + c * (NT / PIECES), at = tid % PIECES, to = REV && (FULL || row < n) ? (FULL ? CHUNK : n) - 1 - row : row;
-            uint4 x = AHEAD ? r[AHEAD ? c : 0] : piece(chunk, v, c, FULL ? CHUNK : n, tid);
-            if (!FULL && row >= n) x = uint4{0, 0, 0, 0};
-            if constexpr (PER == 8) {
+            Piece x = AHEAD ? r[AHEAD ? c : 0] : piece(chunk, v, c, FULL ? CHUNK : n, tid);
+            if (!FULL && row >= n) x = Piece{};
+            if constexpr (!WIDE) {
+                *(uint32_t *)(lds + Mat<T>::four_at(D, to, at * PER >> 2) + (at * PER & 3)) = x;
+            } else if constexpr (PER == 8) {
                 *(uint2 *)(lds + Mat<T>::four_at(D, to, 2 * at)) = uint2{x.x, x.y};
                 *(uint2 *)(lds + Mat<T>::four_at(D, to, 2 * at + 1)) = uint2{x.z, x.w};
             } else {

@@ -14,21 +14,22 @@ typedef __bf16 T;
 typedef float T;
 #endif
 
-// waves a SIMD is to hold: what the registers of each size allow without spilling
+// A wave for each 16 columns of the output (backward: of the narrower of its two outputs).  Waves a SIMD is to hold: what the registers of each
+// size allow without spilling.
 template <bool VEC, int DA, int DC> int launch(const Work &w, hipStream_t st) {
-    constexpr int NW = DA == 32 ? 2 : 4, size = DA + DC;
+    constexpr int size = DA + DC, NW = TD_INST_KIND == 0 && size == 256 ? 4 : (TD_INST_KIND < 3 ? DC : DA < DC ? DA : DC) / 16;
     const Pass &P = w.p;
     const dim3 grid((unsigned)(P.slots * P.heads)), block(64 * NW);
 #if TD_INST_KIND == 0
-    hipLaunchKernelGGL((td_decay_out_kernel<T, DA, DC, NW, VEC, size <= 128 ? 3 : 2>), grid, block, 0, st, P);
+    hipLaunchKernelGGL((td_decay_out_kernel<T, DA, DC, NW, VEC, size <= 128 ? 3 : TD_INST_BF16 && size < 256 && DC == 128 ? 4 : 2>), grid, block, 0, st, P);
 #elif TD_INST_KIND == 1
-    hipLaunchKernelGGL((td_decay_sum_kernel<T, DA, DC, NW, VEC, false, size <= 128 ? 4 : 2>), grid, block, 0, st, P);
+    hipLaunchKernelGGL((td_decay_sum_kernel<T, DA, DC, NW, VEC, false, 4>), grid, block, 0, st, P);
 #elif TD_INST_KIND == 2
-    hipLaunchKernelGGL((td_decay_sum_kernel<T, DA, DC, NW, VEC, true, size <= 128 ? 4 : 2>), grid, block, 0, st, P);
+    hipLaunchKernelGGL((td_decay_sum_kernel<T, DA, DC, NW, VEC, true, 4>), grid, block, 0, st, P);
 #else
     const int64_t held = (int64_t)((P.seg_len + CHUNK - 1) / CHUNK) * DA * DC;
-    hipLaunchKernelGGL((td_decay_backward_kernel<T, DA, DC, NW, VEC, TD_INST_KIND == 4, size <= 64 || (size <= 128 && TD_INST_BF16) ? 2 : 1>), dim3((unsigned)w.groups), block, 0, st, w.p, w.r,
-                       w.chunk_states, held, w.ascending, w.descending);
+    hipLaunchKernelGGL((td_decay_backward_kernel<T, DA, DC, NW, VEC, TD_INST_KIND == 4, size <= 64 || (size <= 128 && TD_INST_BF16) || NW == 8 ? 2 : 1>),
+                       dim3((unsigned)w.groups), block, 0, st, w.p, w.r, w.chunk_states, held, w.ascending, w.descending);
 #endif
     TD_LAUNCH_CHECK();
     return TD_OK;
