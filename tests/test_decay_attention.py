@@ -77,6 +77,19 @@ def test_library_refuses_null_pointers_and_wrong_forms():
     assert L.td_decay_forward(C.byref(cfg), some, some, some, some, None, None, some, None, some, None) == 1 and b"offsets" in L.td_last_error()
 
 
+def test_workspace_stays_bounded():
+    """The states that the backward pass keeps do not grow with the rows: 512 places of 64 chunks of 128 x 128 (2 GiB); what does grow are
+    the states between segments, one for 4096 rows at least, twice."""
+    L = _lib.lib()
+    state = 128 * 128 * 4
+    for n_seq, rows, heads, packed in ((8, 32768, 64, 0), (1, 2 ** 24, 64, 0), (16, 2 ** 22, 32, 1), (1, 4097, 512, 0)):
+        cfg = _lib.DecayConfig(n_seq=n_seq, rows=rows, heads=heads, q_heads=heads, k_heads=heads, v_heads=heads, dk=128, dv=128, dtype=_lib.BF16,
+                               packed=packed, scale=1.0)
+        slots = (rows // 2048 + n_seq) if packed else n_seq * (rows // 2048 + 1)
+        need = L.td_decay_workspace_bytes(C.byref(cfg), 1)
+        assert 0 < need <= 512 * 64 * state + 2 * slots * heads * (state + 8) + 2048
+
+
 def test_reference_is_the_recurrence():
     g = torch.Generator().manual_seed(3)
     q, k, v, s0 = (torch.randn(*s, generator=g, dtype=torch.float64) for s in ((9, 5), (9, 5), (9, 4), (5, 4)))

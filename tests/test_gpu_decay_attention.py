@@ -311,3 +311,24 @@ def test_empty_batch(dev):
     assert d[0].shape == q.shape and (d[1] == 0).all()
     with torch.no_grad():
         assert decay_attention_step(q[:, 0], k[:, 0], v[:, 0], ld, s0).shape == (0, 2, 4)
+
+
+@pytest.mark.parametrize("packed", [False, True], ids=["dense", "packed"])
+def test_long_rows_of_many_heads(packed, dev):
+    """Enough heads for the chip and more than 4096 rows: the backward pass alone is cut into segments.  An entry is a sum over its
+    own head, so three heads are held against the reference."""
+    from timediff_amd.decay_attention import decay_attention
+    T, H, D, pick = 4400, 640, 4, [0, 3, 639]
+    cuts = [0, 4300, T] if packed else None
+    x = _inputs(41, (T,) if packed else (1, T), 2 if packed else 1, H, H, H, H, D, D, BF16, True)
+    off = torch.tensor(cuts, dtype=torch.int32) if packed else None
+    names = ("q", "k", "v", "log_decay", "state")
+    leaf = {n: x[n].to(dev).requires_grad_() for n in names}
+    o, s = decay_attention(*(leaf[n] for n in names[:4]), offsets=None if off is None else off.to(dev), initial_state=leaf["state"], return_state=True)
+    d = dict(zip(names, torch.autograd.grad([o, s], [leaf[n] for n in names], [x["grad_o"].to(dev), x["grad_state"].to(dev)])))
+    few = lambda n, t: t[pick] if n == "log_decay" else t[:, pick] if "state" in n else t[..., pick, :]  # noqa: E731
+    y = {n: few(n, t) for n, t in x.items()}
+    size = {n: t.abs() if n != "log_decay" else t for n, t in y.items()}
+    want, big = (ref.gradients(z["q"], z["k"], z["v"], z["log_decay"], z["grad_o"], z["grad_state"], state=z["state"], offsets=off) for z in (y, size))
+    for n in names:
+        _close("grad " + n, few(n, d[n]), want[n], big[n], 3 * T, D)

@@ -149,9 +149,15 @@ bool wide(const td_decay_config *c, const View &v) {
 
 // Segments: a sequence on its own is one after another, chunk by chunk, so few long ones are cut until there are workgroups for the chip (512: two
 // a compute unit), into segments of 256 rows at least; up to 512 rows a cut costs more (two launches and a second reading of k and v)
-// than it saves.
-void split(const td_decay_config *c, int &len, int &segs, int64_t &slots) {
-    const int64_t rows = total_rows(c), want = rows * c->heads / 512, longest = c->rows;
+// than it saves.  The backward pass keeps the states entering a segment's chunks (64 KB a chunk of 128 x 128), so its segments are 4096
+// rows at most: 2 GB in all 512 workgroups, where a sequence of 32768 rows in one piece would take 17 GB.
+void split(const td_decay_config *c, bool backward, int &len, int &segs, int64_t &slots) {
+    const int64_t rows = total_rows(c), longest = c->rows;
+    int64_t want = rows * c->heads / 512;
+    if (backward && longest > 4096) {
+        const int64_t pieces = (longest + 4095) / 4096, most = (longest + pieces - 1) / pieces;
+        if (want > most) want = most;
+    }
     int64_t l = (want > 256 ? want : 256) + CHUNK - 1;
     l -= l % CHUNK;
     if (l >= longest || longest <= 512) {
@@ -165,7 +171,7 @@ void split(const td_decay_config *c, int &len, int &segs, int64_t &slots) {
     }
 }
 
-Pass base_pass(const td_decay_config *c, const float *log_decay, const int32_t *offsets) {
+Pass base_pass(const td_decay_config *c, bool backward, const float *log_decay, const int32_t *offsets) {
     Pass P = {};
     P.log_decay = log_decay;
     P.offsets = c->packed ? offsets : nullptr;
@@ -174,7 +180,7 @@ Pass base_pass(const td_decay_config *c, const float *log_decay, const int32_t *
     P.heads = c->heads;
     P.out_scale = P.upd_scale = 1.0f;
     int64_t slots;
-    split(c, P.seg_len, P.segs, slots);
+    split(c, backward, P.seg_len, P.segs, slots);
     P.slots = (int)slots;
     return P;
 }
@@ -223,7 +229,7 @@ struct Layout { size_t seg, seg2, chunks, slope, parts, parts2, total; };
 Layout layout(const td_decay_config *c, bool backward) {
     int len, segs;
     int64_t slots;
-    split(c, len, segs, slots);
+    split(c, backward, len, segs, slots);
     const size_t state = (size_t)c->heads * c->dk * c->dv * sizeof(float), rows = (size_t)total_rows(c) * c->heads * sizeof(float);
     const int most = c->dk > c->dv ? c->dk : c->dv, side = most <= 32 ? 32 : most <= 64 ? 64 : 128;
     const size_t held = (size_t)side * side * sizeof(float) * ((len + CHUNK - 1) / CHUNK);
@@ -255,7 +261,7 @@ extern "C" int td_decay_forward(const td_decay_config *cfg, const void *q, const
     TD_REQUIRE(!cfg->packed || offsets, "packed sequences need offsets");
     TD_REQUIRE(!state_out || state_out != state_in, "state_in and state_out must not be the same memory");
     hipStream_t st = (hipStream_t)stream;
-    Pass P = base_pass(cfg, log_decay, offsets);
+    Pass P = base_pass(cfg, false, log_decay, offsets);
     P.a = view(cfg, q, cfg->q_stride, cfg->q_heads, cfg->dk);
     P.b = view(cfg, k, cfg->k_stride, cfg->k_heads, cfg->dk);
     P.c = view(cfg, v, cfg->v_stride, cfg->v_heads, cfg->dv);
@@ -289,7 +295,7 @@ extern "C" int td_decay_backward(const td_decay_config *cfg, const void *q, cons
     w.ascending = grad_q || slope;
     w.descending = grad_v || grad_k || grad_state_in || slope;
     Pass &Q = w.p, &R = w.r;
-    Q = R = base_pass(cfg, log_decay, offsets);
+    Q = R = base_pass(cfg, true, log_decay, offsets);
     w.groups = backward_groups(Q.slots, cfg->heads);
     double *slopes = (double *)(ws + l.slope);
     Q.a = vo; Q.b = vv; Q.c = vk; Q.e = vq;
@@ -331,7 +337,7 @@ extern "C" int td_decay_step(const td_decay_config *cfg, const void *q, const vo
     if (int rc = check_config(cfg)) return rc;
     TD_REQUIRE(cfg->rows == 1 && !cfg->packed, "td_decay_step takes one row of each sequence (rows = 1, packed = 0)");
     TD_REQUIRE(q && k && v && log_decay && state && o, "null pointer");
-    Pass P = base_pass(cfg, log_decay, nullptr);
+    Pass P = base_pass(cfg, false, log_decay, nullptr);
     P.a = view(cfg, q, cfg->q_stride, cfg->q_heads, cfg->dk);
     P.b = view(cfg, k, cfg->k_stride, cfg->k_heads, cfg->dk);
     P.c = view(cfg, v, cfg->v_stride, cfg->v_heads, cfg->dv);

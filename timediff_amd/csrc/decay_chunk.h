@@ -291,8 +291,8 @@ struct Place {
         int hi;
         slot_owner(P, slot, n_seq, segment);
         row_range(P.offsets, P.rows, n_seq, lo, hi);
+        if (segment < 0 || (segment > 0 && (int64_t)segment * P.seg_len >= hi - lo)) return false;
         t0 = segment * P.seg_len;
-        if (segment < 0 || (segment > 0 && t0 >= hi - lo)) return false;
         last = hi - lo - t0 <= P.seg_len;
         t1 = last ? hi - lo : t0 + P.seg_len;
         return true;
@@ -529,8 +529,8 @@ template <typename T, int DA, int DC, int NW, bool VEC, int TERMS> struct Stream
 // Rows of no sequence: zeros in head h's columns, shared out over the slots
 template <typename U> __device__ __forceinline__ void clear_rows(const Pass &P, U *out, int dc, int slot, int h, int tid, int nt) {
     const int lo = min(max(P.offsets[0], 0), P.rows), hi = min(max(P.offsets[P.n_seq], lo), P.rows);
-    for (int i = slot; i < lo + P.rows - hi; i += P.slots)
-        for (int c = tid; c < dc; c += nt) out[((int64_t)(i < lo ? i : hi + i - lo) * P.heads + h) * dc + c] = (U)0.0f;
+    for (int64_t i = slot; i < lo + (P.rows - hi); i += P.slots)
+        for (int c = tid; c < dc; c += nt) out[((i < lo ? i : hi + (i - lo)) * P.heads + h) * dc + c] = (U)0.0f;
 }
 template <typename T> __device__ __forceinline__ void clear_rows_of(const Pass &P, void *out, int f32, int dc, int slot, int h, int tid, int nt) {
     if (!out) return;
