@@ -78,7 +78,7 @@ def test_library_refuses_null_pointers_and_wrong_forms():
 
 
 def test_workspace_stays_bounded():
-    """The states that the backward pass keeps do not grow with the rows: 512 places of 64 chunks of 128 x 128 (2 GiB); what does grow are
+    """The states that the backward pass keeps do not grow with the rows: 512 places (packed 1024) of 64 chunks of 128 x 128 (2 or 4 GiB); what does grow are
     the states between segments, one for 4096 rows at least, twice."""
     L = _lib.lib()
     state = 128 * 128 * 4
@@ -87,7 +87,7 @@ def test_workspace_stays_bounded():
                                packed=packed, scale=1.0)
         slots = (rows // 2048 + n_seq) if packed else n_seq * (rows // 2048 + 1)
         need = L.td_decay_workspace_bytes(C.byref(cfg), 1)
-        assert 0 < need <= 512 * 64 * state + 2 * slots * heads * (state + 8) + 2048
+        assert 0 < need <= (1024 if packed else 512) * 64 * state + 2 * slots * heads * (state + 8) + 2048
 
 
 def test_reference_is_the_recurrence():

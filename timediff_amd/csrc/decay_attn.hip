@@ -147,18 +147,28 @@ bool wide(const td_decay_config *c, const View &v) {
            v.row * esize(c) < (1 << 24);
 }
 
-// Segments: a sequence on its own is one after another, chunk by chunk, so few long ones are cut until there are workgroups for the chip (512: two
-// a compute unit), into segments of 256 rows at least; up to 512 rows a cut costs more (two launches and a second reading of k and v)
-// than it saves.  The backward pass keeps the states entering a segment's chunks (64 KB a chunk of 128 x 128), so its segments are 4096
-// rows at most: 2 GB in all 512 workgroups, where a sequence of 32768 rows in one piece would take 17 GB.
+// Segments: a sequence on its own is one after another, chunk by chunk, so few long ones are cut until the chip is full, which costs two launches
+// and a second reading of k and v.  Measured (bfloat16, forward / backward):
+//   * rows of a segment: 256 at least, and nothing is cut up to 512 rows: the chip is full with 512 workgroups (two a compute unit), or with 256
+//     where one workgroup's registers fill a compute unit (backward of wide states); cut for 256 instead of 512 those backward passes
+//     take 309 instead of 343 us at 128 sequences and heads of 1024 rows, 128 x 128;
+//   * with a workgroup for three in four compute units nothing is cut: 256 of 1024 rows, 128 x 128, take 85 / 379 us whole and 146 / 590
+//     cut for 512.  States of 32 x 32 have less to do between their loads and gain up to 512: 256 of 2048 rows 77 / 207 us
+//     cut, about 95 / 276 whole.  Lengths of packed sequences are not known here: one of them may be nearly all rows;
+//   * the backward pass keeps the states entering a segment's chunks (64 KB a chunk of 128 x 128), so its segments are 4096 rows
+//     at most: 2 GB in all 512 workgroups, where a sequence of 32768 rows in one piece would take 17 GB.
 void split(const td_decay_config *c, bool backward, int &len, int &segs, int64_t &slots) {
     const int64_t rows = total_rows(c), longest = c->rows;
-    int64_t want = rows * c->heads / 512;
+    const int most = c->dk > c->dv ? c->dk : c->dv;
+    const bool one = backward && most > (c->dtype == TD_BF16 ? 64 : 32);
+    int64_t l = rows * c->heads / (one ? 256 : 512);
+    if (l < 256) l = 256;
+    if (!c->packed && most > 32 && (int64_t)c->n_seq * c->heads >= 192 && l < longest) l = longest;
     if (backward && longest > 4096) {
-        const int64_t pieces = (longest + 4095) / 4096, most = (longest + pieces - 1) / pieces;
-        if (want > most) want = most;
+        const int64_t pieces = (longest + 4095) / 4096, even = (longest + pieces - 1) / pieces;
+        if (l > even) l = even;
     }
-    int64_t l = (want > 256 ? want : 256) + CHUNK - 1;
+    l += CHUNK - 1;
     l -= l % CHUNK;
     if (l >= longest || longest <= 512) {
         len = (int)(longest > 1 ? longest : 1);
@@ -198,8 +208,13 @@ int launch(const td_decay_config *c, Kind kind, const Pass &P, bool vec, hipStre
     return launch(c, kind, w, vec, st);
 }
 
-// Workgroups of the backward pass: as many as the chip holds (two a compute unit), each with its own place for the states of a segment's chunks
-int backward_groups(int64_t slots, int heads) { return (int)(slots * heads < 512 ? slots * heads : 512); }
+// Workgroups of the backward pass, each with its own place for the states of a segment's chunks, one (slot, head) after another: as many as the
+// chip holds (two a compute unit).  Packed slots have different lengths, and workgroups that wait for a place on the chip even that out
+// (20011 rows of 40 sequences, 8 heads of 64 x 128: 296 us with 512, 270 with 1024).
+int backward_groups(const td_decay_config *c, int64_t slots) {
+    const int64_t most = c->packed ? 1024 : 512;
+    return (int)(slots * c->heads < most ? slots * c->heads : most);
+}
 
 // What the segments add, and the state that enters each of them (nothing to do where every sequence is one segment)
 template <bool REV> int enter_states(const td_decay_config *c, const Pass &P, bool vec, hipStream_t st) {
@@ -237,7 +252,7 @@ Layout layout(const td_decay_config *c, bool backward) {
     w.seg = 0;
     w.seg2 = segs == 1 ? 0 : up256(slots * state);
     w.chunks = w.seg2 + (backward && segs != 1 ? up256(slots * state) : 0);
-    w.slope = w.chunks + (backward ? held * backward_groups(slots, c->heads) : 0);
+    w.slope = w.chunks + (backward ? held * backward_groups(c, slots) : 0);
     w.parts = w.slope + (backward ? up256(2 * (size_t)slots * c->heads * sizeof(double)) : 0);
     const bool q = c->q_heads != c->heads, k = c->k_heads != c->heads, v = c->v_heads != c->heads;
     w.parts2 = w.parts + (backward && q ? up256(rows * c->dk) : 0);
@@ -296,7 +311,7 @@ extern "C" int td_decay_backward(const td_decay_config *cfg, const void *q, cons
     w.descending = grad_v || grad_k || grad_state_in || slope;
     Pass &Q = w.p, &R = w.r;
     Q = R = base_pass(cfg, true, log_decay, offsets);
-    w.groups = backward_groups(Q.slots, cfg->heads);
+    w.groups = backward_groups(cfg, Q.slots);
     double *slopes = (double *)(ws + l.slope);
     Q.a = vo; Q.b = vv; Q.c = vk; Q.e = vq;
     Q.da = cfg->dv; Q.dc = cfg->dk; Q.st_a = 1; Q.st_c = cfg->dv;
