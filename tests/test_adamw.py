@@ -36,6 +36,19 @@ def test_refusals(bits, bad, error, text):
         adamw_(**dict(_lists(bits=bits), **bad), **HYPER)
 
 
+@pytest.mark.parametrize("name", ["params", "exp_avgs", "exp_avg_sqs", "scales"])
+def test_same_tensor_twice(name):
+    lists = {k: [t.clone() for t in v for _ in range(2)] for k, v in _lists(bits=8).items()}
+    lists[name][1] = lists[name][0]
+    with pytest.raises(ValueError, match=f"the same tensor twice in {name}"):
+        adamw_(**lists, **HYPER)
+    # empty ones share an address, and a gradient is only read
+    lists = {k: [t.clone() for t in v for _ in range(2)] + [t[:0].clone() for t in v for _ in range(2)] for k, v in _lists(bits=8).items()}
+    lists["grads"][1] = lists["grads"][0]
+    with pytest.raises(ValueError, match="ROCm device"):
+        adamw_(**lists, **HYPER)
+
+
 def test_empty_list_is_no_step():
     adamw_([], [], [], [], **HYPER)
 

@@ -364,3 +364,19 @@ def test_mixer_trained_and_streamed(bits, dev):
             return o
         rows = [mix(x[:, :20], ps, prompt)] + [mix(x[:, t], ps, lambda *a: decay_attention_step(*a, keep["s"]))[:, None] for t in range(20, T)]
         assert ((torch.cat(rows, 1) - full).abs() <= 1e-4 * full.abs().max()).all()
+
+
+def test_written_params_are_noticed(dev):
+    """A param that a graph saved and a step then changed: the backward pass is refused, as for torch's own writes in place."""
+    from timediff_amd.optim import adamw_
+    w = torch.ones(300, device=dev, requires_grad=True)
+    loss = (w * w).sum()
+    zeros = [torch.zeros(300, device=dev) for _ in range(2)]
+    kw = dict(lr=0.1, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, step=1)
+    adamw_([w], [torch.ones(300, device=dev)], zeros[:1], zeros[1:], **kw)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.inference_mode():               # no such count there
+        p = torch.ones(300, device=dev)
+        adamw_([p, w], [torch.ones(300, device=dev) for _ in range(2)], *([torch.zeros(300, device=dev) for _ in range(2)] for _ in range(2)), **kw)
+    assert (p < 1).all()

@@ -332,3 +332,41 @@ def test_long_rows_of_many_heads(packed, dev):
     want, big = (ref.gradients(z["q"], z["k"], z["v"], z["log_decay"], z["grad_o"], z["grad_state"], state=z["state"], offsets=off) for z in (y, size))
     for n in names:
         _close("grad " + n, few(n, d[n]), want[n], big[n], 3 * T, D)
+
+
+def test_written_state_is_noticed(dev):
+    """A state that a graph saved and a step then changed: the backward pass is refused, as for torch's own writes in place."""
+    from timediff_amd.decay_attention import decay_attention, decay_attention_step
+    x = {n: None if t is None else t.to(dev) for n, t in _inputs(3, (2, 9), 2, 2, 2, 2, 2, 8, 8, F32, True).items()}
+    o = decay_attention(x["q"].requires_grad_(), x["k"], x["v"], x["log_decay"], initial_state=x["state"])
+    with torch.no_grad():
+        decay_attention_step(x["q"][:, 0], x["k"][:, 0], x["v"][:, 0], x["log_decay"], x["state"])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        o.sum().backward()
+    with torch.inference_mode():               # no such count there
+        state = x["state"].clone()
+        decay_attention_step(x["q"][:, 0], x["k"][:, 0], x["v"][:, 0], x["log_decay"], state)
+
+
+def test_captured_beside_an_eager_graph(dev):
+    """While an eager graph of the same leaves lives a capture is refused; once it is gone the same leaves are captured and replayed."""
+    from timediff_amd.decay_attention import decay_attention
+    x = _inputs(19, (2, 70), 2, 2, 2, 2, 2, 16, 16, F32, False)
+    leaf = [x[n].to(dev).requires_grad_() for n in ("q", "k", "v", "log_decay")]
+    go = x["grad_o"].to(dev)
+    eager = decay_attention(*leaf)
+    with pytest.raises(RuntimeError, match="still alive"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            decay_attention(*leaf)
+    want = torch.autograd.grad(eager, leaf, go)
+    del eager
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(decay_attention(*leaf), leaf, go)
+    for _ in range(3):
+        for g in got:
+            g.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)

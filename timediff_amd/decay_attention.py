@@ -33,6 +33,16 @@ class _DecayFn(torch.autograd.Function):
         return (*grads, None, None, None)
 
 
+def _claim(node):
+    """Marks the nodes that gather the leaves' gradients with the stream of their first graph.  Such a node lives as long as any graph of
+    its leaf, and a backward pass waits for its stream: under capture that stream would have to be the captured one."""
+    stream = torch.cuda.current_stream().cuda_stream
+    for leaf, _ in node.next_functions:
+        if hasattr(leaf, "variable") and leaf.metadata.setdefault("decay_attention stream", stream) != stream and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("decay_attention under graph capture: a graph of the same leaves, made on another stream, is still alive; drop it "
+                               "before the capture (or pass detached leaves)")
+
+
 def decay_attention(q, k, v, log_decay, *, scale=None, offsets=None, initial_state=None, return_state=False):
     """q (B, T, Hq, Dk), k (B, T, Hk, Dk), v (B, T, Hv, Dv), all float32 or all bfloat16; log_decay (H,) float32, meant to be
     <= 0; Hq, Hk and Hv divide H, and head h uses head h // (H // Hq) of q, and so on  ->  o (B, T, H, Dv) of q's type.
@@ -42,11 +52,15 @@ def decay_attention(q, k, v, log_decay, *, scale=None, offsets=None, initial_sta
     gradient.  Their values are read on the device when the kernels run.
     initial_state: (B or N, H, Dk, Dv) float32.  return_state: -> (o, state after the last row, the same shape).
     Differentiable once in q, k, v, log_decay and initial_state.  Any strides with a contiguous last dimension are read in place.
+    Rows are computed 64 at a time: a NaN or an infinity in a row's q, k or v may also reach the rows of its 64 before it, so rows that pad
+    a dense batch should hold finite values (packed rows of other sequences and of none are never read).
+    A captured backward pass needs leaves of which no graph made on another stream is alive: refused otherwise.
     """
     ops.decay_check(q, k, v, log_decay, offsets, initial_state)
     scale = float(q.shape[-1] ** -0.5 if scale is None else scale)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, log_decay, initial_state)):
         o, state = _DecayFn.apply(q, k, v, log_decay, initial_state, offsets, scale, return_state)
+        _claim(o.grad_fn)
     else:
         o, state = ops.decay_forward(q, k, v, log_decay, scale, offsets, initial_state, return_state)
     return (o, state) if return_state else o

@@ -461,6 +461,16 @@ def decay_backward(q, k, v, log_decay, scale, grad_o, offsets=None, state=None, 
     return (*new, d_state)
 
 
+def _written(tensors):
+    """Counts a write to each tensor, as torch does for its own: a graph that saved one of them is then refused its backward pass."""
+    try:
+        torch.autograd.graph.increment_version(tensors)
+    except RuntimeError:                      # an inference tensor has no such count
+        for t in tensors:
+            if not t.is_inference():
+                torch.autograd.graph.increment_version(t)
+
+
 def decay_step(q, k, v, log_decay, state, scale):
     """One row of each sequence; `state` is updated in place -> o (B, H, Dv)."""
     decay_check(q, k, v, log_decay, None, state, step=True)
@@ -471,6 +481,8 @@ def decay_step(q, k, v, log_decay, state, scale):
     with _on_device(index):
         o = torch.empty((q.shape[0], log_decay.shape[0], v.shape[-1]), dtype=q.dtype, device=q.device)
         if q.shape[0]:
+            if not state.is_inference():
+                _written(state)
             check(lib().td_decay_step(_decay_config(q, k, v, log_decay, scale, None, step=True), q.data_ptr(), k.data_ptr(), v.data_ptr(),
                                       log_decay.data_ptr(), state.data_ptr(), o.data_ptr(), _raw_stream(index)))
     return o

@@ -17,13 +17,14 @@ from ._lib import ADAMW_BLOCK, AdamwConfig, AdamwRecord, check, lib, ptr
 
 _DTYPE, _NUMEL, _ADDRESS = operator.attrgetter("dtype"), torch.Tensor.numel, torch.Tensor.data_ptr
 _CONTIGUOUS, _DEVICE = torch.Tensor.is_contiguous, torch.Tensor.get_device
+_READ = {"grads", "random"}
 _F32, _GRADS, _E4M3, _WORDS = {torch.float32}, {torch.float32, torch.bfloat16}, {torch.float8_e4m3fn}, {torch.int32}
 
 
 def adamw_(params, grads, exp_avgs, exp_avg_sqs, scales=None, *, lr, betas, eps, weight_decay, step, grad_scale=None, random=None,
            seed=0, record=None):
     """One AdamW step in place over lists of tensors (one launch for every 48): params float32, grads float32 or bfloat16, all
-    contiguous and on one device.
+    contiguous and on one device, none that is written twice in its list and none overlapping another.
     Moments in 32 bits: exp_avgs (m) and exp_avg_sqs (v) float32.  In 8 bits, where `scales` is given: exp_avgs (m) and exp_avg_sqs
     (sqrt(v)) float8_e4m3fn, scales float32 (ceil(n / 256), 2); all zeros is the state before the first step.
     random: for 8-bit moments, int32 tensors of the params' sizes whose low and high 16 bits round m and sqrt(v); by default the
@@ -53,20 +54,25 @@ def adamw_(params, grads, exp_avgs, exp_avg_sqs, scales=None, *, lr, betas, eps,
             raise ValueError(f"{name} must be contiguous")
         if name != "params" and list(map(_NUMEL, tensors)) != sizes:
             raise ValueError(f"scales must have 2 values for each {ADAMW_BLOCK} of their param" if name == "scales" else f"{name} must have their params' sizes")
+    table = array.array("q", bytes(64 * len(n)))          # td_adamw_tensor is eight 64-bit words
+    for word, (name, tensors, *_) in enumerate(lists):
+        table[word::8] = at = array.array("q", map(_ADDRESS, tensors))
+        if name not in _READ and len(set(at)) != len(n):
+            at = [a for a, k in zip(at, n) if k]
+            if len(set(at)) != len(at):
+                raise ValueError(f"the same tensor twice in {name}")
     index = params[0].get_device()
     for name, tensors, *_ in lists:
         if index < 0 or set(map(_DEVICE, tensors)) != {index}:
             raise ValueError(f"{name} must be on one ROCm device, the params'")
     if grad_scale is not None and (grad_scale.dtype is not torch.float32 or grad_scale.numel() != 1 or grad_scale.get_device() != index):
         raise ValueError("grad_scale must be one float32 value on the params' device")
-    table = array.array("q", bytes(64 * len(n)))          # td_adamw_tensor is eight 64-bit words
-    for word, (_, tensors, *_) in enumerate(lists):
-        table[word::8] = array.array("q", map(_ADDRESS, tensors))
     table[6::8] = array.array("q", n)
     if set(map(_DTYPE, grads)) != _F32:
         table[7::8] = array.array("q", [_lib.F32 if g.dtype is torch.float32 else _lib.BF16 for g in grads])
-    cfg = _CONFIG.pack(lr, betas[0], betas[1], eps, weight_decay, step, seed, 0 if grad_scale is None else grad_scale.data_ptr(),
+    cfg = _CONFIG.pack(lr, betas[0], betas[1], eps, weight_decay, step, seed & (2 ** 64 - 1), 0 if grad_scale is None else grad_scale.data_ptr(),
                        0 if record is None else record.data_ptr(), bits, 0)
+    ops._written(params)
     with ops._on_device(index):
         check(lib().td_adamw(cfg, table.buffer_info()[0], len(n), ops._raw_stream(index)))
 
