@@ -758,11 +758,6 @@ __device__ __forceinline__ void pair_sweep(const Pass &P, int item, PairLds<T, D
         typedef decltype(rows) R;
         constexpr bool FULL = R::FULL;
         const int tid = here(tid_), lane = tid & 63, g = lane >> 4, li = lane & 15;
-        sk.template store<FULL>(lk, pk, P.a, t, n, tid);
-        sq.template store<FULL>(lq, pq, P.b, t, n, tid);
-        so.template store<FULL>(lo, po, P.c, t, n, tid);
-        sv.template store<FULL>(lv, pv, P.e, t, n, tid);
-        __syncthreads();
         f32x4 F[SLOPE ? K::TA : 1][K::CT];         // the state that entered this chunk ascending
         if (SLOPE) {
             const f32x4 *from = (const f32x4 *)chunk_states + (((t - at.t0) / CHUNK * NW + wave) * K::TA * K::CT) * 64 + lane;
@@ -771,6 +766,11 @@ __device__ __forceinline__ void pair_sweep(const Pass &P, int item, PairLds<T, D
 #pragma unroll
                 for (int ct = 0; ct < K::CT; ++ct) F[mt][ct] = from[(mt * K::CT + ct) * 64];
         }
+        sk.template store<FULL>(lk, pk, P.a, t, n, tid);
+        sq.template store<FULL>(lq, pq, P.b, t, n, tid);
+        so.template store<FULL>(lo, po, P.c, t, n, tid);
+        sv.template store<FULL>(lv, pv, P.e, t, n, tid);
+        __syncthreads();
         fetch(next, tid);
         float sum = 0.0f;
 #pragma unroll
@@ -787,6 +787,14 @@ __device__ __forceinline__ void pair_sweep(const Pass &P, int item, PairLds<T, D
             V::keep(sv, scores_v, it, jt, lane);
             K::keep(sk, scores_k, it, jt, lane);
         }
+        const int64_t row0 = (packed ? 0 : (int64_t)at.n_seq * P.rows) + at.lo + t;
+        phase();
+        xk.template from_state<R>(lv, n, w, g, li);
+        if (SLOPE) sum += xk.template dot<R>(lk, n, 0, wave, g, li);
+        __syncthreads();
+        phase();
+        xk.columns(lq, wave, g, li);
+        xk.template from_rows<R, true>(scores_k, n, 1.0f, P.out2, P.out2_f32, row0, P.heads, h, P.da, wave, lane);
         if (SLOPE) {
             float cross = 0.0f;
 #pragma unroll
@@ -795,16 +803,8 @@ __device__ __forceinline__ void pair_sweep(const Pass &P, int item, PairLds<T, D
                 for (int ct = 0; ct < K::CT; ++ct)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) cross += F[mt][ct][r] * xk.S[mt][ct][r];
-            sum += (float)n * power(w.lg2, n) * cross;
+            slope += (double)(sum + (float)n * power(w.lg2, n) * cross);
         }
-        const int64_t row0 = (packed ? 0 : (int64_t)at.n_seq * P.rows) + at.lo + t;
-        phase();
-        xk.template from_state<R>(lv, n, w, g, li);
-        if (SLOPE) slope += (double)(sum + xk.template dot<R>(lk, n, 0, wave, g, li));
-        __syncthreads();
-        phase();
-        xk.columns(lq, wave, g, li);
-        xk.template from_rows<R, true>(scores_k, n, 1.0f, P.out2, P.out2_f32, row0, P.heads, h, P.da, wave, lane);
         phase();
         xk.template advance<R>(lo, n, w, P.upd_scale, 1, g, li);
         phase();
