@@ -538,16 +538,17 @@ template <typename T> __device__ __forceinline__ void clear_rows_of(const Pass &
     else clear_rows(P, (T *)out, dc, slot, h, tid, nt);
 }
 
-// The sum of a workgroup's values, in a fixed order
+// The sum of a workgroup's values, in a fixed order: inside the waves, then wave by wave
 template <int NT> __device__ __forceinline__ void workgroup_sum(double x, double *red, double *to, int tid) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o);
     __syncthreads();
-    red[tid] = x;
+    if ((tid & 63) == 0) red[tid >> 6] = x;
     __syncthreads();
-    for (int o = NT / 2; o > 0; o >>= 1) {
-        if (tid < o) red[tid] += red[tid + o];
-        __syncthreads();
+    if (tid == 0) {
+        for (int w = 1; w < NT / 64; ++w) x += red[w];
+        *to = x;
     }
-    if (tid == 0) *to = red[0];
 }
 
 // What a segment adds to the state
