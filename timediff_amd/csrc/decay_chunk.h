@@ -177,6 +177,16 @@ template <> struct Mat<float> {
     static __device__ __forceinline__ float elem(Op o, int, int r) { return o[r]; }
 };
 
+// A chunk's rows: a whole chunk, or the last rows of a sequence, of which tiles of 16 there are at most LIVE.  (How many tiles a product covers is
+// a constant in each form: a branch on it would stand between a matrix instruction and the readers of its result.)
+template <int LIVE_, bool FULL_> struct Rows {
+    static constexpr int LIVE = LIVE_;
+    static constexpr bool FULL = FULL_;
+};
+typedef Rows<CHUNK / 16, true> Whole;
+typedef Rows<CHUNK / 16, false> Most;
+typedef Rows<CHUNK / 32, false> Half;
+
 // One chunk's rows of one tensor on their way from memory to LDS.  Memory is read in the order of its rows (n of them from `low` on), a
 // reversed pass turns them round in LDS.  The loads go into registers while the chunk before is computed (unless there are too many of them):
 // WIDE: 16 bytes each, at 32-bit offsets from the chunk's first row; else (odd sizes, strides or addresses) 4 bytes each.  They are never
@@ -217,11 +227,14 @@ template <typename T, int D, int NT, bool WIDE, bool REV> struct Stage {
 #pragma unroll
         for (int c = 0; c < N; ++c) r[c] = piece(chunk, v, c, n, tid);
     }
-    template <bool FULL> __device__ __forceinline__ void store(T *lds, const T *base, const View &v, int low, int n, int tid) const {
+    // the tiles of rows that R has
+    template <typename R> __device__ __forceinline__ void store(T *lds, const T *base, const View &v, int low, int n, int tid) const {
+        constexpr bool FULL = R::FULL;
+        constexpr int AT_ONCE = NT / PIECES, LAST = (R::LIVE * 16 + AT_ONCE - 1) / AT_ONCE;
         if (tid % PIECES * PER >= v.d) return;
         const char *chunk = (const char *)(base + (int64_t)low * v.row);
 #pragma unroll
-        for (int c = 0; c < N; ++c) {
+        for (int c = 0; c < LAST; ++c) {
             const int row = tid / PIECES + c * (NT / PIECES), at = tid % PIECES, to = REV && (FULL || row < n) ? (FULL ? CHUNK : n) - 1 - row : row;
             Piece x = AHEAD ? r[AHEAD ? c : 0] : piece(chunk, v, c, FULL ? CHUNK : n, tid);
             if (!FULL && row >= n) x = Piece{};
@@ -272,16 +285,6 @@ __device__ __forceinline__ void settle() {
     asm volatile("s_nop 15");
     __builtin_amdgcn_sched_barrier(0);
 }
-
-// A chunk's rows: a whole chunk, or the last rows of a sequence, of which tiles of 16 there are at most LIVE.  (How many tiles a product covers is
-// a constant in each form: a branch on it would stand between a matrix instruction and the readers of its result.)
-template <int LIVE_, bool FULL_> struct Rows {
-    static constexpr int LIVE = LIVE_;
-    static constexpr bool FULL = FULL_;
-};
-typedef Rows<CHUNK / 16, true> Whole;
-typedef Rows<CHUNK / 16, false> Most;
-typedef Rows<CHUNK / 32, false> Half;
 
 // Which segment of which sequence a workgroup has
 struct Place {
@@ -432,11 +435,11 @@ template <typename T, int DA, int DC, int NW, bool VEC, int TERMS> struct Stream
         }
         return sum;
     }
-    __device__ __forceinline__ void columns(const T *lc, int wave, int g, int li) {
+    template <typename R> __device__ __forceinline__ void columns(const T *lc, int wave, int g, int li) {
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
-            for (int kr = 0; kr < KR; ++kr) vt[ct][kr] = M::col_op(lc, LC, wave * CT + ct, kr, g, li);
+            for (int kr = 0; kr < (R::LIVE + M::KT - 1) / M::KT; ++kr) vt[ct][kr] = M::col_op(lc, LC, wave * CT + ct, kr, g, li);
     }
     // o += the rows of this chunk; rows of o to memory
     template <typename R, bool REV> __device__ __forceinline__ void from_rows(const Op *scores, int n, float scale, void *out, int out_f32, int64_t row0, int heads, int h, int dc,
@@ -581,11 +584,11 @@ template <typename T, int DA, int DC, int NW, bool VEC, bool REV, int WAVES> __g
         typedef decltype(rows) R;
         constexpr bool FULL = R::FULL;
         const int tid = here(tid_), lane = tid & 63, g = lane >> 4, li = lane & 15;
-        sb.template store<FULL>(lb, pb, P.b, t, n, tid);
-        sc.template store<FULL>(lc, pc, P.c, t, n, tid);
+        sb.template store<R>(lb, pb, P.b, t, n, tid);
+        sc.template store<R>(lc, pc, P.c, t, n, tid);
         __syncthreads();
         fetch(next, tid);
-        x.columns(lc, wave, g, li);
+        x.template columns<R>(lc, wave, g, li);
         x.template advance<R>(lb, n, w, P.upd_scale, REV, g, li);
         __syncthreads();
     };
@@ -651,10 +654,10 @@ __device__ __forceinline__ void out_sweep(const Pass &P, int item, OutLds<T, DA,
         typedef decltype(rows) R;
         constexpr bool FULL = R::FULL;
         const int tid = here(tid_), lane = tid & 63, g = lane >> 4, li = lane & 15;
-        sb.template store<FULL>(lb, pb, P.b, t, n, tid);
-        sa.template store<FULL>(la, pa, P.a, t, n, tid);
-        sc.template store<FULL>(lc, pc, P.c, t, n, tid);
-        if (SLOPE) se.template store<FULL>(le, pe, P.e, t, n, tid);
+        sb.template store<R>(lb, pb, P.b, t, n, tid);
+        sa.template store<R>(la, pa, P.a, t, n, tid);
+        sc.template store<R>(lc, pc, P.c, t, n, tid);
+        if (SLOPE) se.template store<R>(le, pe, P.e, t, n, tid);
         __syncthreads();
         if (FULL) fetch(t + CHUNK, tid);
 #pragma unroll
@@ -678,7 +681,7 @@ __device__ __forceinline__ void out_sweep(const Pass &P, int item, OutLds<T, DA,
         if (SLOPE) slope += (double)(x.template dot<R>(le, n, 1, wave, g, li) * P.out_scale);
         __syncthreads();
         phase();
-        x.columns(lc, wave, g, li);
+        x.template columns<R>(lc, wave, g, li);
         x.template from_rows<R, false>(scores, n, P.out_scale, P.out, P.out_f32, (packed ? 0 : (int64_t)at.n_seq * P.rows) + at.lo + t, P.heads, h, P.dc, wave, lane);
         phase();
         x.template advance<R>(lb, n, w, P.upd_scale, 0, g, li);
@@ -767,10 +770,10 @@ __device__ __forceinline__ void pair_sweep(const Pass &P, int item, PairLds<T, D
 #pragma unroll
                 for (int ct = 0; ct < K::CT; ++ct) F[mt][ct] = from[(mt * K::CT + ct) * 64];
         }
-        sk.template store<FULL>(lk, pk, P.a, t, n, tid);
-        sq.template store<FULL>(lq, pq, P.b, t, n, tid);
-        so.template store<FULL>(lo, po, P.c, t, n, tid);
-        sv.template store<FULL>(lv, pv, P.e, t, n, tid);
+        sk.template store<R>(lk, pk, P.a, t, n, tid);
+        sq.template store<R>(lq, pq, P.b, t, n, tid);
+        so.template store<R>(lo, po, P.c, t, n, tid);
+        sv.template store<R>(lv, pv, P.e, t, n, tid);
         __syncthreads();
         fetch(next, tid);
         float sum = 0.0f;
@@ -794,7 +797,7 @@ __device__ __forceinline__ void pair_sweep(const Pass &P, int item, PairLds<T, D
         if (SLOPE) sum += xk.template dot<R>(lk, n, 0, wave, g, li);
         __syncthreads();
         phase();
-        xk.columns(lq, wave, g, li);
+        xk.template columns<R>(lq, wave, g, li);
         xk.template from_rows<R, true>(scores_k, n, 1.0f, P.out2, P.out2_f32, row0, P.heads, h, P.da, wave, lane);
         if (SLOPE) {
             float cross = 0.0f;
@@ -811,7 +814,7 @@ __device__ __forceinline__ void pair_sweep(const Pass &P, int item, PairLds<T, D
         phase();
         xv.template from_state<R>(lk, n, w, g, li);
         phase();
-        xv.columns(lo, wave, g, li);
+        xv.template columns<R>(lo, wave, g, li);
         xv.template from_rows<R, true>(scores_v, n, 1.0f, P.out, P.out_f32, row0, P.heads, h, P.dc, wave, lane);
         phase();
         xv.template advance<R>(lq, n, w, P.upd_scale, 1, g, li);
