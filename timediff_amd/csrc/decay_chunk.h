@@ -188,13 +188,15 @@ typedef Rows<CHUNK / 16, false> Most;
 typedef Rows<CHUNK / 32, false> Half;
 
 // One chunk's rows of one tensor on their way from memory to LDS.  Memory is read in the order of its rows (n of them from `low` on), a
-// reversed pass turns them round in LDS.  The loads go into registers while the chunk before is computed (unless there are too many of them):
+// reversed pass turns them round in LDS.  The loads go into registers while the chunk before is computed (unless there are too many of them:
+// 64 bytes of each tensor a thread; 4 bytes at a time in workgroups of 512 threads, whose registers four tensors would fill, 32: 101 x 41 float32,
+// 16 sequences of 1024 rows, 8 heads: 546 us backward, 834 with 64).
 // WIDE: 16 bytes each, at 32-bit offsets from the chunk's first row; else (odd sizes, strides or addresses) 4 bytes each.  They are never
 // skipped, so that their registers have one writer: a lane without a row or a column of its own reads its neighbours', and
 // nothing of that is stored.
 template <typename T, int D, int NT, bool WIDE, bool REV> struct Stage {
     static constexpr int BYTES = WIDE ? 16 : 4, PER = BYTES / sizeof(T), PIECES = D / PER, N = CHUNK * PIECES / NT;
-    static constexpr bool AHEAD = N * BYTES <= 64;
+    static constexpr bool AHEAD = N * BYTES <= (WIDE || NT < 512 ? 64 : 32);
     static_assert(NT % PIECES == 0, "a thread's pieces share their columns");
     struct Wide { uint4 x; };
     struct Narrow { uint32_t x; };

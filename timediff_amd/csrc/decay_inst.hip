@@ -14,8 +14,12 @@ typedef __bf16 T;
 typedef float T;
 #endif
 
-// A wave for each 16 columns of the output (backward: of the narrower of its two outputs).  Waves a SIMD is to hold: what the registers of each
-// size allow without spilling.
+// A wave for each 16 columns of the output (backward: of the narrower of its two outputs); the forward pass of 128 x 128 takes 32 columns a wave, so
+// that two workgroups share a compute unit.  Waves a SIMD is to hold: what the registers of each size allow with few or no spills.  Measured
+// in bfloat16, 16 sequences of 1024 rows, 8 heads, unless said otherwise:
+//   forward 128 x 128: 4 waves of 32 columns 171 us, 8 waves of 16 199 (both before whole sequences stayed uncut); 64 x 128: 8 waves, 4 a SIMD 56, 4 waves 60;
+//   backward 128 x 128: 8 waves 350, 4 waves 402; 64 x 128: one wave a SIMD 205, two (spilling) 268; 64 x 64, 2048 sequences of 272 rows: two
+//   a SIMD 1.02 ms, three (spilling) 1.92 ms.
 template <bool VEC, int DA, int DC> int launch(const Work &w, hipStream_t st) {
     constexpr int size = DA + DC, NW = TD_INST_KIND == 0 && size == 256 ? 4 : (TD_INST_KIND < 3 ? DC : DA < DC ? DA : DC) / 16;
     const Pass &P = w.p;
@@ -37,8 +41,9 @@ template <bool VEC, int DA, int DC> int launch(const Work &w, hipStream_t st) {
 
 }  // namespace
 
-// (sizes that are not a multiple of 16 bytes take the nearest square: what they gain from fewer kernels they do not lose to padding, their
-// loads are the bound)
+// Sizes, strides or addresses that are not multiples of 16 bytes have kernels of their own; their backward pass takes the square that holds them (41 x 101
+// and 101 x 41, 16 sequences of 1024 rows, 8 heads: 559 and 576 us bfloat16, 531 and 546 float32; rectangles 591, 605, 513, 677; forward,
+// bfloat16: 117 and 154 us in rectangles, 179 and 167 in squares).
 int TD_CAT(td_decay_launch_, TD_INST_BF16, TD_INST_KIND)(const Work &w, int vec, hipStream_t st) {
     const Pass &P = TD_INST_KIND < 3 ? w.p : w.r;          // backward: (da, dc) = (dk, dv)
     const int most = P.da > P.dc ? P.da : P.dc;
@@ -51,5 +56,9 @@ int TD_CAT(td_decay_launch_, TD_INST_BF16, TD_INST_KIND)(const Work &w, int vec,
     }
     if (most <= 32) return launch<false, 32, 32>(w, st);
     if (most <= 64) return launch<false, 64, 64>(w, st);
+#if TD_INST_KIND < 3
+    if (P.da <= 64) return launch<false, 64, 128>(w, st);
+    if (P.dc <= 64) return launch<false, 128, 64>(w, st);
+#endif
     return launch<false, 128, 128>(w, st);
 }

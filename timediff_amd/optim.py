@@ -6,7 +6,6 @@ for each 256 values (a moment's value is code.float() * scale), rounded stochast
 """
 import array
 import ctypes as C
-import operator
 import struct
 
 import torch
@@ -15,7 +14,7 @@ from . import _lib, ops
 from ._lib import ADAMW_BLOCK, AdamwConfig, AdamwRecord, check, lib, ptr
 
 
-_DTYPE, _NUMEL, _ADDRESS = operator.attrgetter("dtype"), torch.Tensor.numel, torch.Tensor.data_ptr
+_DTYPE, _NUMEL, _ADDRESS = torch.Tensor.dtype.__get__, torch.Tensor.numel, torch.Tensor.data_ptr
 _CONTIGUOUS, _DEVICE = torch.Tensor.is_contiguous, torch.Tensor.get_device
 _READ = {"grads", "random"}
 _F32, _GRADS, _E4M3, _WORDS = {torch.float32}, {torch.float32, torch.bfloat16}, {torch.float8_e4m3fn}, {torch.int32}
