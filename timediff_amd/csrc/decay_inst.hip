@@ -14,14 +14,14 @@ typedef __bf16 T;
 typedef float T;
 #endif
 
-// A wave for each 16 columns of the output (backward: of the narrower of its two outputs); the forward pass of 128 x 128 takes 32 columns a wave, so
-// that two workgroups share a compute unit.  Waves a SIMD is to hold: what the registers of each size allow with few or no spills.  Measured
+// A wave for each 16 columns of the output (backward: of the narrower of its two outputs); the bfloat16 forward pass of 128 x 128 takes 32 columns a
+// wave, so that two workgroups share a compute unit (float32, of whose rows LDS holds one workgroup's: 64 sequences 423 us with 8 waves, 805 with 4).  Waves a SIMD is to hold: what the registers of each size allow with few or no spills.  Measured
 // in bfloat16, 16 sequences of 1024 rows, 8 heads, unless said otherwise:
 //   forward 128 x 128: 4 waves of 32 columns 171 us, 8 waves of 16 199 (both before whole sequences stayed uncut); 64 x 128: 8 waves, 4 a SIMD 56, 4 waves 60;
 //   backward 128 x 128: 8 waves 350, 4 waves 402; 64 x 128: one wave a SIMD 205, two (spilling) 268; 64 x 64, 2048 sequences of 272 rows: two
 //   a SIMD 1.02 ms, three (spilling) 1.92 ms.
 template <bool VEC, int DA, int DC> int launch(const Work &w, hipStream_t st) {
-    constexpr int size = DA + DC, NW = TD_INST_KIND == 0 && size == 256 ? 4 : (TD_INST_KIND < 3 ? DC : DA < DC ? DA : DC) / 16;
+    constexpr int size = DA + DC, NW = TD_INST_KIND == 0 && TD_INST_BF16 && size == 256 ? 4 : (TD_INST_KIND < 3 ? DC : DA < DC ? DA : DC) / 16;
     const Pass &P = w.p;
     const dim3 grid((unsigned)(P.slots * P.heads)), block(64 * NW);
 #if TD_INST_KIND == 0
