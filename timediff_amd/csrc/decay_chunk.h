@@ -288,6 +288,8 @@ __device__ __forceinline__ void settle() {
     __builtin_amdgcn_sched_barrier(0);
 }
 
+template <bool V> struct Flag { static constexpr bool value = V; };
+
 // Which segment of which sequence a workgroup has
 struct Place {
     int n_seq, segment, lo, t0, t1;      // rows lo + t0 .. lo + t1 - 1
@@ -331,18 +333,35 @@ template <int NW> struct Weights {
     __device__ __forceinline__ int apart(int m, int r, int g, int li) const { return (it[m] - jt[m]) * 16 + li - (g * 4 + r); }
 };
 
+// Which of a chunk's four row tiles a wave's outputs have.  NI = 4: all of them.  NI = 2: two teams of waves hold the same state, team 0 has the
+// outputs of tiles 0 and 3, team 1 those of 1 and 2: as many products with scores (and in `most` of two tiles, as many tiles) for each.
+template <int NI> struct Tiles {
+    int team;
+    float factor[NI];            // g^(16 tile)
+    __device__ __forceinline__ void init(float lg2, int team_) {
+        team = team_;
+#pragma unroll
+        for (int j = 0; j < NI; ++j) factor[j] = power(lg2, 16 * at(j));
+    }
+    __device__ __forceinline__ int at(int j) const { return NI == 4 ? j : j == 0 ? team : 3 - team; }
+    static constexpr bool live(int j, int most) { return NI == 4 ? j < most : j == 0 || most > 2; }
+};
+
 // One product stream: the state M (DA x DC) and what a chunk does with it.  TA x CT tiles of the state a wave.
-template <typename T, int DA, int DC, int NW, bool VEC, int TERMS> struct Stream {
+template <typename T, int DA, int DC, int NW, bool VEC, int TERMS, int NI = 4> struct Stream {
     typedef Mat<T> M;
     typedef typename M::Op Op;
     static constexpr int LA = DA, LC = DC, PA = M::pitch(DA), PC = M::pitch(DC), TA = DA / 16, CT = DC / 16 / NW, KS = TA / M::KT, RT = CHUNK / 16, KR = RT / M::KT;
     static constexpr int S2 = M::SPLIT ? 2 : 1, S3 = M::SPLIT ? 3 : 1, SF = M::SPLIT ? TERMS : 1;      // terms of scores, of decayed rows, of the state
     static constexpr int PAIRS = M::KT == 2 ? RT / 2 * (RT / 2 + 1) : RT * (RT + 1) / 2;               // score operands: (it, kr), kr <= it / KT
     static_assert(CT * NW * 16 == DC && CT > 0, "every column tile has a wave");
-    f32x4 S[TA][CT], o[RT][CT];
+    f32x4 S[TA][CT], o[NI][CT];
     Op vt[CT][KR];
+    Tiles<NI> tiles;
 
     static __device__ __forceinline__ int pair(int it, int kr) { return M::KT == 2 ? (it >> 1) * ((it >> 1) + 1) + (it & 1) * ((it >> 1) + 1) + kr : it * (it + 1) / 2 + kr; }
+    // score operands of row tile j; with two teams as many for both, a tile of zeros where a team's own tile has one less
+    static constexpr int operands(int j) { return NI == 4 ? j / M::KT + 1 : M::KT == 2 ? j + 1 : 2 * j + 2; }
 
     // the halves of score operands above the diagonal
     static __device__ __forceinline__ void clear_scores(Op *scores, int lane) {
@@ -392,11 +411,11 @@ template <typename T, int DA, int DC, int NW, bool VEC, int TERMS> struct Stream
                 }
     }
     // o = g^(i+1) F^T a
-    template <typename R, typename W> __device__ __forceinline__ void from_state(const T *la, int n, const W &w, int g, int li) {
+    template <typename R, typename W> __device__ __forceinline__ void from_state(const T *la, const W &w, int g, int li) {
 #pragma unroll
-        for (int it = 0; it < R::LIVE; ++it)
+        for (int j = 0; j < NI; ++j)
 #pragma unroll
-            for (int ct = 0; ct < CT; ++ct) o[it][ct] = f32x4{0, 0, 0, 0};
+            for (int ct = 0; ct < CT; ++ct) o[j][ct] = f32x4{0, 0, 0, 0};
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             Op f[CT][SF];
@@ -408,32 +427,35 @@ template <typename T, int DA, int DC, int NW, bool VEC, int TERMS> struct Stream
                 M::template split<SF>(part, f[ct]);
             }
 #pragma unroll
-            for (int it = 0; it < R::LIVE; ++it) {
-                const Op q = M::row_op(la, LA, it * 16 + li, s, g);
+            for (int j = 0; j < NI; ++j) {
+                if (!tiles.live(j, R::LIVE)) continue;
+                const Op q = M::row_op(la, LA, tiles.at(j) * 16 + li, s, g);
 #pragma unroll
                 for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
-                    for (int k = 0; k < SF; ++k) o[it][ct] = M::mma(f[ct][k], q, o[it][ct]);
+                    for (int k = 0; k < SF; ++k) o[j][ct] = M::mma(f[ct][k], q, o[j][ct]);
             }
         }
 #pragma unroll
-        for (int it = 0; it < R::LIVE; ++it)
+        for (int j = 0; j < NI; ++j)
 #pragma unroll
-            for (int ct = 0; ct < CT; ++ct) o[it][ct] = o[it][ct] * (w.wo * w.tiles[it]);
+            for (int ct = 0; ct < CT; ++ct) o[j][ct] = o[j][ct] * (w.wo * tiles.factor[j]);
     }
     // sum of (first + i) o_i . e_i over this lane's entries
-    template <typename R> __device__ __forceinline__ float dot(const T *le, int n, int first, int wave, int g, int li) const {
+    template <typename R> __device__ __forceinline__ float dot(const T *le, int first, int wave, int g, int li) const {
         float sum = 0.0f;
 #pragma unroll
-        for (int it = 0; it < R::LIVE; ++it) {
+        for (int j = 0; j < NI; ++j) {
+            if (!tiles.live(j, R::LIVE)) continue;
+            const int i = tiles.at(j) * 16 + li;
             float part = 0.0f;
 #pragma unroll
             for (int ct = 0; ct < CT; ++ct) {
-                const T *e = le + M::four_at(LC, it * 16 + li, (wave * CT + ct) * 4 + g);
+                const T *e = le + M::four_at(LC, i, (wave * CT + ct) * 4 + g);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) part += o[it][ct][r] * (float)e[r];
+                for (int r = 0; r < 4; ++r) part += o[j][ct][r] * (float)e[r];
             }
-            sum += (float)(first + it * 16 + li) * part;
+            sum += (float)(first + i) * part;
         }
         return sum;
     }
@@ -451,29 +473,32 @@ template <typename T, int DA, int DC, int NW, bool VEC, int TERMS> struct Stream
         const uint32_t by = (uint32_t)heads * dc;
         const int64_t first = row0 * by + (int64_t)h * dc;
 #pragma unroll
-        for (int it = 0; it < R::LIVE; ++it)
+        for (int j = 0; j < NI; ++j) {
+            if (!tiles.live(j, R::LIVE)) continue;
 #pragma unroll
-            for (int kr = 0; kr <= it / M::KT; ++kr)
+            for (int kr = 0; kr < operands(j); ++kr)
 #pragma unroll
                 for (int k = 0; k < S2; ++k) {
-                    const Op f = scores[(pair(it, kr) * S2 + k) * 64 + lane];
+                    Op f = scores[(pair(tiles.at(j), kr) * S2 + k) * 64 + lane];
+                    if (NI == 2 && M::KT == 1) f = kr <= tiles.at(j) ? f : Op{};
 #pragma unroll
-                    for (int ct = 0; ct < CT; ++ct) o[it][ct] = M::mma(vt[ct][kr], f, o[it][ct]);
+                    for (int ct = 0; ct < CT; ++ct) o[j][ct] = M::mma(vt[ct][kr], f, o[j][ct]);
                 }
+        }
 #pragma unroll
-        for (int it = 0; it < R::LIVE; ++it)
+        for (int j = 0; j < NI; ++j)
 #pragma unroll
-            for (int ct = 0; ct < CT; ++ct) o[it][ct] = o[it][ct] * scale;
+            for (int ct = 0; ct < CT; ++ct) o[j][ct] = o[j][ct] * scale;
 #pragma unroll
-        for (int it = 0; it < R::LIVE; ++it) {
-            const int i = it * 16 + li;
-            if (!R::FULL && i >= n) continue;
+        for (int j = 0; j < NI; ++j) {
+            const int i = tiles.at(j) * 16 + li;
+            if (!tiles.live(j, R::LIVE) || (!R::FULL && i >= n)) continue;
 #pragma unroll
             for (int ct = 0; ct < CT; ++ct) {
                 const int col = (wave * CT + ct) * 16 + g * 4;
                 const uint32_t at = (uint32_t)(REV ? n - 1 - i : i) * by + col;
-                if (out_f32) put((float *)out + first, at, o[it][ct], dc - col);
-                else put((T *)out + first, at, o[it][ct], dc - col);
+                if (out_f32) put((float *)out + first, at, o[j][ct], dc - col);
+                else put((T *)out + first, at, o[j][ct], dc - col);
             }
         }
     }
@@ -611,14 +636,14 @@ template <typename T, int DA, int DC, int NW, bool SLOPE> struct OutLds {
     T a[CHUNK * X::PA], b[CHUNK * X::PA], c[CHUNK * X::PC], e[SLOPE ? CHUNK * X::PC : 8];
     typename X::Op scores[X::PAIRS * X::S2 * 64];
 };
-template <typename T, int DA, int DC, int NW, bool VEC, bool SLOPE>
+template <typename T, int DA, int DC, int NW, int TEAMS, bool VEC, bool SLOPE>
 __device__ __forceinline__ void out_sweep(const Pass &P, int item, OutLds<T, DA, DC, NW, SLOPE> &lds, float *chunk_states) {
-    typedef Stream<T, DA, DC, NW, VEC, SLOPE ? 3 : 2> X;
+    typedef Stream<T, DA, DC, NW, VEC, SLOPE ? 3 : 2, 4 / TEAMS> X;
     typedef typename X::Op Op;
-    constexpr int NT = 64 * NW;
+    constexpr int NT = 64 * NW * TEAMS;
     T *const la = lds.a, *const lb = lds.b, *const lc = lds.c, *const le = lds.e;
     Op *const scores = lds.scores;
-    const int tid_ = here(threadIdx.x), tid = tid_, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, li = lane & 15;
+    const int tid_ = here(threadIdx.x), tid = tid_, all = __builtin_amdgcn_readfirstlane(tid >> 6), wave = all % NW, team = all / NW, lane = tid & 63, g = lane >> 4, li = lane & 15;
     const int h = item % P.heads, slot = item / P.heads;
     const bool packed = P.offsets != nullptr;
     if (packed) clear_rows_of<T>(P, P.out, P.out_f32, P.dc, slot, h, tid, NT);
@@ -645,11 +670,12 @@ __device__ __forceinline__ void out_sweep(const Pass &P, int item, OutLds<T, DA,
     };
     if (at.t0 < at.t1) fetch(at.t0, tid);
     __syncthreads();
-    Weights<NW> w;
-    w.init(P.log_decay[h], P.upd_scale, 0, wave, g, li);
-    if (wave == 0) X::clear_scores(scores, lane);
+    Weights<NW * TEAMS> w;
+    w.init(P.log_decay[h], P.upd_scale, 0, all, g, li);
+    if (all == 0) X::clear_scores(scores, lane);
     const int64_t state_at = ((int64_t)at.n_seq * P.heads + h) * P.da * P.dc;
     X x;
+    x.tiles.init(w.lg2, team);
     x.enter(at.segment > 0 ? P.seg + (int64_t)item * P.da * P.dc : P.state_in ? P.state_in + state_at : nullptr, P.st_a, P.st_c, P.da, P.dc, wave, g, li);
     double slope = 0.0;
     const auto chunk = [&](auto rows, int t, int n) __attribute__((always_inline)) {
@@ -671,7 +697,7 @@ __device__ __forceinline__ void out_sweep(const Pass &P, int item, OutLds<T, DA,
             for (int r = 0; r < 4; ++r) s[r] *= w.wa[m][r];
             X::keep(s, scores, it, jt, lane);
         }
-        if (SLOPE) {
+        if (SLOPE && team == 0) {
             f32x4 *to = (f32x4 *)chunk_states + (((t - at.t0) / CHUNK * NW + wave) * X::TA * X::CT) * 64 + lane;
 #pragma unroll
             for (int mt = 0; mt < X::TA; ++mt)
@@ -679,8 +705,8 @@ __device__ __forceinline__ void out_sweep(const Pass &P, int item, OutLds<T, DA,
                 for (int ct = 0; ct < X::CT; ++ct) to[(mt * X::CT + ct) * 64] = x.S[mt][ct];
         }
         phase();
-        x.template from_state<R>(la, n, w, g, li);
-        if (SLOPE) slope += (double)(x.template dot<R>(le, n, 1, wave, g, li) * P.out_scale);
+        x.template from_state<R>(la, w, g, li);
+        if (SLOPE) slope += (double)(x.template dot<R>(le, 1, wave, g, li) * P.out_scale);
         __syncthreads();
         phase();
         x.template columns<R>(lc, wave, g, li);
@@ -693,32 +719,33 @@ __device__ __forceinline__ void out_sweep(const Pass &P, int item, OutLds<T, DA,
     for (; at.t1 - t >= CHUNK; t += CHUNK) chunk(Whole(), t, CHUNK);
     if (at.t1 - t > CHUNK / 2) chunk(Most(), t, at.t1 - t);
     else if (t < at.t1) chunk(Half(), t, at.t1 - t);
-    x.leave(at.last && P.state_out ? P.state_out + state_at : nullptr, P.st_a, P.st_c, P.da, P.dc, wave, g, li);
+    x.leave(at.last && P.state_out && team == 0 ? P.state_out + state_at : nullptr, P.st_a, P.st_c, P.da, P.dc, wave, g, li);
     if (SLOPE) workgroup_sum<NT>(slope, (double *)&lds, P.slope + item, tid);
 }
 
 template <typename T, int DA, int DC, int NW, bool VEC, int WAVES> __global__ __launch_bounds__(64 * NW, WAVES) void td_decay_out_kernel(Pass P) {
     __shared__ __align__(16) OutLds<T, DA, DC, NW, false> lds;
-    out_sweep<T, DA, DC, NW, VEC, false>(P, blockIdx.x, lds, nullptr);
+    out_sweep<T, DA, DC, NW, 1, VEC, false>(P, blockIdx.x, lds, nullptr);
 }
 
 // out from (a, b, c) and out2 from (e, c, b), rows descending: the gradients of v and k from (k, q, grad_o) and (v, grad_o, q).  SLOPE: the rest of
 // the derivative by log g: pairs of rows of one chunk; what a chunk's rows owe to the chunks behind it; and the chunk's own n rows, for every pair with one
-// row before and one behind it, which is n g^n <state entering the chunk, its gradient when it leaves>.
+// row before and one behind it, which is n g^n <state entering the chunk, its gradient when it leaves>.  TEAMS = 2: NW waves for each of the two
+// gradients, at the same time, where one workgroup's LDS or registers fill a compute unit and NW = 4 waves would leave half of each SIMD's places empty.
 template <typename T, int DK, int DV, int NW> struct PairLds {
     typedef Stream<T, DK, DV, NW, true, 2> V;
     T k[CHUNK * V::PA], q[CHUNK * V::PA], o[CHUNK * V::PC], v[CHUNK * V::PC];
     typename V::Op scores[2][V::PAIRS * V::S2 * 64];
 };
-template <typename T, int DK, int DV, int NW, bool VEC, bool SLOPE>
+template <typename T, int DK, int DV, int NW, int TEAMS, bool VEC, bool SLOPE>
 __device__ __forceinline__ void pair_sweep(const Pass &P, int item, PairLds<T, DK, DV, NW> &lds, const float *chunk_states) {
     typedef Stream<T, DK, DV, NW, VEC, 2> V;
     typedef Stream<T, DV, DK, NW, VEC, SLOPE ? 3 : 2> K;
     typedef typename V::Op Op;
-    constexpr int NT = 64 * NW;
+    constexpr int NT = 64 * NW * TEAMS;
     T *const lk = lds.k, *const lq = lds.q, *const lo = lds.o, *const lv = lds.v;
     Op *const scores_k = lds.scores[0], *const scores_v = lds.scores[1];
-    const int tid_ = here(threadIdx.x), tid = tid_, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, li = lane & 15;
+    const int tid_ = here(threadIdx.x), tid = tid_, all = __builtin_amdgcn_readfirstlane(tid >> 6), wave = all % NW, team = all / NW, lane = tid & 63, g = lane >> 4, li = lane & 15;
     const int h = item % P.heads, slot = item / P.heads;
     const bool packed = P.offsets != nullptr;
     if (packed) {
@@ -749,101 +776,177 @@ __device__ __forceinline__ void pair_sweep(const Pass &P, int item, PairLds<T, D
     __syncthreads();
     Weights<NW> w;
     w.init(P.log_decay[h], P.upd_scale, 1, wave, g, li);
-    if (wave == 0) {
+    if (all == 0) {
         V::clear_scores(scores_k, lane);
         V::clear_scores(scores_v, lane);
     }
     const int64_t state_at = ((int64_t)at.n_seq * P.heads + h) * P.da * P.dc;
     const float *from = !at.last ? P.seg + (int64_t)item * P.da * P.dc : P.state_in ? P.state_in + state_at : nullptr;
-    V xv;
-    K xk;
-    xv.enter(from, P.st_a, P.st_c, P.da, P.dc, wave, g, li);
-    xk.enter(from, P.st_c, P.st_a, P.dc, P.da, wave, g, li);
     double slope = 0.0;
-    const auto chunk = [&](auto rows, int t, int n, Next next) __attribute__((always_inline)) {
-        typedef decltype(rows) R;
-        constexpr bool FULL = R::FULL;
-        const int tid = here(tid_), lane = tid & 63, g = lane >> 4, li = lane & 15;
-        f32x4 F[SLOPE ? K::TA : 1][K::CT];         // the state that entered this chunk ascending
-        if (SLOPE) {
-            const f32x4 *from = (const f32x4 *)chunk_states + (((t - at.t0) / CHUNK * NW + wave) * K::TA * K::CT) * 64 + lane;
+    if constexpr (TEAMS == 2) {
+        // One gradient a team: X its stream with rows x, y, z as (a, b, c), SL whether it has the slope's sums too
+        const auto one = [&](auto stream, T *lx, T *ly, T *lz, typename V::Op *scores, void *out, int out_f32, int64_t st_x, int64_t st_z, int dx, int dz, auto sums)
+                             __attribute__((always_inline)) {
+            typedef decltype(stream) X;
+            constexpr bool SL = decltype(sums)::value;
+            X x;
+            x.tiles.init(w.lg2, 0);
+            x.enter(from, st_x, st_z, dx, dz, wave, g, li);
+            const auto chunk = [&](auto rows, int t, int n, Next next) __attribute__((always_inline)) {
+                typedef decltype(rows) R;
+                const int tid = here(tid_), lane = tid & 63, g = lane >> 4, li = lane & 15;
+                f32x4 F[SL ? X::TA : 1][X::CT];
+                if (SL) {
+                    const f32x4 *from = (const f32x4 *)chunk_states + (((t - at.t0) / CHUNK * NW + wave) * X::TA * X::CT) * 64 + lane;
 #pragma unroll
-            for (int mt = 0; mt < K::TA; ++mt)
+                    for (int mt = 0; mt < X::TA; ++mt)
 #pragma unroll
-                for (int ct = 0; ct < K::CT; ++ct) F[mt][ct] = from[(mt * K::CT + ct) * 64];
-        }
-        sk.template store<R>(lk, pk, P.a, t, n, tid);
-        sq.template store<R>(lq, pq, P.b, t, n, tid);
-        so.template store<R>(lo, po, P.c, t, n, tid);
-        sv.template store<R>(lv, pv, P.e, t, n, tid);
-        __syncthreads();
-        fetch(next, tid);
-        float sum = 0.0f;
+                        for (int ct = 0; ct < X::CT; ++ct) F[mt][ct] = from[(mt * X::CT + ct) * 64];
+                }
+                sk.template store<R>(lk, pk, P.a, t, n, tid);
+                sq.template store<R>(lq, pq, P.b, t, n, tid);
+                so.template store<R>(lo, po, P.c, t, n, tid);
+                sv.template store<R>(lv, pv, P.e, t, n, tid);
+                __syncthreads();
+                fetch(next, tid);
+                float sum = 0.0f;
 #pragma unroll
-        for (int m = 0; m < w.MINE; ++m) {
-            const int it = w.it[m], jt = w.jt[m];
-            if (it >= R::LIVE) continue;
-            f32x4 sv = V::score(lk, lq, it, jt, g, li), sk = K::score(lv, lo, it, jt, g, li);
+                for (int m = 0; m < w.MINE; ++m) {
+                    const int it = w.it[m], jt = w.jt[m];
+                    if (it >= R::LIVE) continue;
+                    f32x4 s = X::score(lx, ly, it, jt, g, li);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                sv[r] *= w.wa[m][r];
-                if (SLOPE) sum += (float)w.apart(m, r, g, li) * sv[r] * sk[r];
-                sk[r] *= w.wa[m][r];
+                    for (int r = 0; r < 4; ++r) s[r] *= w.wa[m][r];
+                    X::keep(s, scores, it, jt, lane);
+                    if (SL) {
+                        const f32x4 other = V::score(lk, lq, it, jt, g, li);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) sum += (float)w.apart(m, r, g, li) * s[r] * other[r];
+                    }
+                }
+                const int64_t row0 = (packed ? 0 : (int64_t)at.n_seq * P.rows) + at.lo + t;
+                phase();
+                x.template from_state<R>(lx, w, g, li);
+                if (SL) sum += x.template dot<R>(lk, 0, wave, g, li);
+                __syncthreads();
+                phase();
+                x.template columns<R>(lz, wave, g, li);
+                x.template from_rows<R, true>(scores, n, 1.0f, out, out_f32, row0, P.heads, h, dz, wave, lane);
+                if (SL) {
+                    float cross = 0.0f;
+#pragma unroll
+                    for (int mt = 0; mt < X::TA; ++mt)
+#pragma unroll
+                        for (int ct = 0; ct < X::CT; ++ct)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) cross += F[mt][ct][r] * x.S[mt][ct][r];
+                    slope += (double)(sum + (float)n * power(w.lg2, n) * cross);
+                }
+                phase();
+                x.template advance<R>(ly, n, w, P.upd_scale, 1, g, li);
+                __syncthreads();
+            };
+            const Next before = whole ? Next{at.t1 - tail - CHUNK, CHUNK} : Next{at.t0, 1};
+            if (tail > CHUNK / 2) chunk(Most(), at.t1 - tail, tail, before);
+            else if (tail) chunk(Half(), at.t1 - tail, tail, before);
+            for (int c = whole - 1; c >= 0; --c) chunk(Whole(), at.t0 + c * CHUNK, CHUNK, c > 0 ? Next{at.t0 + (c - 1) * CHUNK, CHUNK} : Next{at.t0, 1});
+            x.leave(at.segment == 0 && P.state_out && team == 1 ? P.state_out + state_at : nullptr, st_x, st_z, dx, dz, wave, g, li);
+        };
+        // (both ways have the same barriers)
+        if (team) one(V(), lk, lq, lo, scores_v, P.out, P.out_f32, P.st_a, P.st_c, P.da, P.dc, Flag<false>());
+        else one(K(), lv, lo, lq, scores_k, P.out2, P.out2_f32, P.st_c, P.st_a, P.dc, P.da, Flag<SLOPE>());
+    } else {
+        V xv;
+        K xk;
+        xv.tiles.init(w.lg2, 0);
+        xk.tiles.init(w.lg2, 0);
+        xv.enter(from, P.st_a, P.st_c, P.da, P.dc, wave, g, li);
+        xk.enter(from, P.st_c, P.st_a, P.dc, P.da, wave, g, li);
+        const auto chunk = [&](auto rows, int t, int n, Next next) __attribute__((always_inline)) {
+            typedef decltype(rows) R;
+            constexpr bool FULL = R::FULL;
+            const int tid = here(tid_), lane = tid & 63, g = lane >> 4, li = lane & 15;
+            f32x4 F[SLOPE ? K::TA : 1][K::CT];         // the state that entered this chunk ascending
+            if (SLOPE) {
+                const f32x4 *from = (const f32x4 *)chunk_states + (((t - at.t0) / CHUNK * NW + wave) * K::TA * K::CT) * 64 + lane;
+#pragma unroll
+                for (int mt = 0; mt < K::TA; ++mt)
+#pragma unroll
+                    for (int ct = 0; ct < K::CT; ++ct) F[mt][ct] = from[(mt * K::CT + ct) * 64];
             }
-            V::keep(sv, scores_v, it, jt, lane);
-            K::keep(sk, scores_k, it, jt, lane);
-        }
-        const int64_t row0 = (packed ? 0 : (int64_t)at.n_seq * P.rows) + at.lo + t;
-        phase();
-        xk.template from_state<R>(lv, n, w, g, li);
-        if (SLOPE) sum += xk.template dot<R>(lk, n, 0, wave, g, li);
-        __syncthreads();
-        phase();
-        xk.template columns<R>(lq, wave, g, li);
-        xk.template from_rows<R, true>(scores_k, n, 1.0f, P.out2, P.out2_f32, row0, P.heads, h, P.da, wave, lane);
-        if (SLOPE) {
-            float cross = 0.0f;
+            sk.template store<R>(lk, pk, P.a, t, n, tid);
+            sq.template store<R>(lq, pq, P.b, t, n, tid);
+            so.template store<R>(lo, po, P.c, t, n, tid);
+            sv.template store<R>(lv, pv, P.e, t, n, tid);
+            __syncthreads();
+            fetch(next, tid);
+            float sum = 0.0f;
 #pragma unroll
-            for (int mt = 0; mt < K::TA; ++mt)
+            for (int m = 0; m < w.MINE; ++m) {
+                const int it = w.it[m], jt = w.jt[m];
+                if (it >= R::LIVE) continue;
+                f32x4 sv = V::score(lk, lq, it, jt, g, li), sk = K::score(lv, lo, it, jt, g, li);
 #pragma unroll
-                for (int ct = 0; ct < K::CT; ++ct)
+                for (int r = 0; r < 4; ++r) {
+                    sv[r] *= w.wa[m][r];
+                    if (SLOPE) sum += (float)w.apart(m, r, g, li) * sv[r] * sk[r];
+                    sk[r] *= w.wa[m][r];
+                }
+                V::keep(sv, scores_v, it, jt, lane);
+                K::keep(sk, scores_k, it, jt, lane);
+            }
+            const int64_t row0 = (packed ? 0 : (int64_t)at.n_seq * P.rows) + at.lo + t;
+            phase();
+            xk.template from_state<R>(lv, w, g, li);
+            if (SLOPE) sum += xk.template dot<R>(lk, 0, wave, g, li);
+            __syncthreads();
+            phase();
+            xk.template columns<R>(lq, wave, g, li);
+            xk.template from_rows<R, true>(scores_k, n, 1.0f, P.out2, P.out2_f32, row0, P.heads, h, P.da, wave, lane);
+            if (SLOPE) {
+                float cross = 0.0f;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) cross += F[mt][ct][r] * xk.S[mt][ct][r];
-            slope += (double)(sum + (float)n * power(w.lg2, n) * cross);
-        }
-        phase();
-        xk.template advance<R>(lo, n, w, P.upd_scale, 1, g, li);
-        phase();
-        xv.template from_state<R>(lk, n, w, g, li);
-        phase();
-        xv.template columns<R>(lo, wave, g, li);
-        xv.template from_rows<R, true>(scores_v, n, 1.0f, P.out, P.out_f32, row0, P.heads, h, P.dc, wave, lane);
-        phase();
-        xv.template advance<R>(lq, n, w, P.upd_scale, 1, g, li);
-        __syncthreads();
-    };
-    const Next before = whole ? Next{at.t1 - tail - CHUNK, CHUNK} : Next{at.t0, 1};
-    if (tail > CHUNK / 2) chunk(Most(), at.t1 - tail, tail, before);
-    else if (tail) chunk(Half(), at.t1 - tail, tail, before);
-    for (int c = whole - 1; c >= 0; --c) chunk(Whole(), at.t0 + c * CHUNK, CHUNK, c > 0 ? Next{at.t0 + (c - 1) * CHUNK, CHUNK} : Next{at.t0, 1});
-    xv.leave(at.segment == 0 && P.state_out ? P.state_out + state_at : nullptr, P.st_a, P.st_c, P.da, P.dc, wave, g, li);
+                for (int mt = 0; mt < K::TA; ++mt)
+#pragma unroll
+                    for (int ct = 0; ct < K::CT; ++ct)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) cross += F[mt][ct][r] * xk.S[mt][ct][r];
+                slope += (double)(sum + (float)n * power(w.lg2, n) * cross);
+            }
+            phase();
+            xk.template advance<R>(lo, n, w, P.upd_scale, 1, g, li);
+            phase();
+            xv.template from_state<R>(lk, w, g, li);
+            phase();
+            xv.template columns<R>(lo, wave, g, li);
+            xv.template from_rows<R, true>(scores_v, n, 1.0f, P.out, P.out_f32, row0, P.heads, h, P.dc, wave, lane);
+            phase();
+            xv.template advance<R>(lq, n, w, P.upd_scale, 1, g, li);
+            __syncthreads();
+        };
+        const Next before = whole ? Next{at.t1 - tail - CHUNK, CHUNK} : Next{at.t0, 1};
+        if (tail > CHUNK / 2) chunk(Most(), at.t1 - tail, tail, before);
+        else if (tail) chunk(Half(), at.t1 - tail, tail, before);
+        for (int c = whole - 1; c >= 0; --c) chunk(Whole(), at.t0 + c * CHUNK, CHUNK, c > 0 ? Next{at.t0 + (c - 1) * CHUNK, CHUNK} : Next{at.t0, 1});
+        xv.leave(at.segment == 0 && P.state_out ? P.state_out + state_at : nullptr, P.st_a, P.st_c, P.da, P.dc, wave, g, li);
+    }
     if (SLOPE) workgroup_sum<NT>(slope, (double *)&lds, P.slope + item, tid);
 }
 
 // The gradients of one (slot, head) after another: that of q with Q's rows ascending, those of k and v with R's descending, right behind each other
 // so that the second reading of q, k, v and grad_o (and, for the slope, of the states entering the chunks, in a place of the
 // workgroup's own: `held` floats) comes from the caches.
-template <typename T, int DK, int DV, int NW, bool VEC, bool SLOPE, int WAVES>
-__global__ __launch_bounds__(64 * NW, WAVES) void td_decay_backward_kernel(Pass Q, Pass R, float *chunk_states, int64_t held, int ascending, int descending) {
+template <typename T, int DK, int DV, int NW, int TEAMS, bool VEC, bool SLOPE, int WAVES>
+__global__ __launch_bounds__(64 * NW * TEAMS, WAVES) void td_decay_backward_kernel(Pass Q, Pass R, float *chunk_states, int64_t held, int ascending, int descending) {
     __shared__ __align__(16) union {
         OutLds<T, DV, DK, NW, SLOPE> out;
         PairLds<T, DK, DV, NW> pair;
     } lds;
     float *mine = chunk_states + blockIdx.x * held;
     for (int item = blockIdx.x; item < Q.slots * Q.heads; item += gridDim.x) {
-        if (ascending) out_sweep<T, DV, DK, NW, VEC, SLOPE>(argument<Pass>(0), item, lds.out, mine);
+        if (ascending) out_sweep<T, DV, DK, NW, TEAMS, VEC, SLOPE>(argument<Pass>(0), item, lds.out, mine);
         __syncthreads();
-        if (descending) pair_sweep<T, DK, DV, NW, VEC, SLOPE>(argument<Pass>(sizeof(Pass)), item, lds.pair, mine);
+        if (descending) pair_sweep<T, DK, DV, NW, TEAMS, VEC, SLOPE>(argument<Pass>(sizeof(Pass)), item, lds.pair, mine);
         __syncthreads();
     }
 }

@@ -14,12 +14,15 @@ typedef __bf16 T;
 typedef float T;
 #endif
 
-// A wave for each 16 columns of the output (backward: of the narrower of its two outputs); the bfloat16 forward pass of 128 x 128 takes 32 columns a
-// wave, so that two workgroups share a compute unit (float32, of whose rows LDS holds one workgroup's: 64 sequences 423 us with 8 waves, 805 with 4).  Waves a SIMD is to hold: what the registers of each size allow with few or no spills.  Measured
-// in bfloat16, 16 sequences of 1024 rows, 8 heads, unless said otherwise:
-//   forward 128 x 128: 4 waves of 32 columns 171 us, 8 waves of 16 199 (both before whole sequences stayed uncut); 64 x 128: 8 waves, 4 a SIMD 56, 4 waves 60;
-//   backward 128 x 128: 8 waves 350, 4 waves 402; 64 x 128: one wave a SIMD 205, two (spilling) 268; 64 x 64, 2048 sequences of 272 rows: two
-//   a SIMD 1.02 ms, three (spilling) 1.92 ms.
+// A wave for each 16 columns of the output (backward: of the narrower of its two outputs); the bfloat16 forward pass of 128 x 128 takes 32 columns
+// a wave, so that two workgroups share a compute unit.  Backward passes of four waves of which a compute unit holds one workgroup take a second team of
+// four.  Waves a SIMD is to hold: what the registers of each size allow with few or no spills.  Measured with 16 sequences of 1024
+// rows, 8 heads, unless said otherwise:
+//   forward, bfloat16: 128 x 128 4 waves of 32 columns 171 us, 8 of 16 199 (cut into segments); 64 x 128 8 waves, 4 a SIMD 56, 4 waves 60;
+//   forward, float32 (LDS holds one workgroup): 128 x 128, 64 sequences, 8 waves 423 us, 4 waves 805;
+//   backward, bfloat16: 128 x 128 8 waves 350, 4 waves 402; 64 x 128 one team 180, two 162 (one team at two workgroups a compute unit,
+//   spilling, 268); 64 x 64, 2048 sequences of 272 rows: two workgroups of one team 1.02 ms, of two teams (spilling) 1.26, three of one (spilling) 1.92;
+//   backward, float32: 64 x 64 one team 203, two 193; 64 x 128 414 and 326.
 template <bool VEC, int DA, int DC> int launch(const Work &w, hipStream_t st) {
     constexpr int size = DA + DC, NW = TD_INST_KIND == 0 && TD_INST_BF16 && size == 256 ? 4 : (TD_INST_KIND < 3 ? DC : DA < DC ? DA : DC) / 16;
     const Pass &P = w.p;
@@ -32,8 +35,9 @@ template <bool VEC, int DA, int DC> int launch(const Work &w, hipStream_t st) {
     hipLaunchKernelGGL((td_decay_sum_kernel<T, DA, DC, NW, VEC, true, 4>), grid, block, 0, st, P);
 #else
     const int64_t held = (int64_t)((P.seg_len + CHUNK - 1) / CHUNK) * DA * DC;
-    hipLaunchKernelGGL((td_decay_backward_kernel<T, DA, DC, NW, VEC, TD_INST_KIND == 4, size <= 64 || (size <= 128 && TD_INST_BF16) || NW == 8 ? 2 : 1>),
-                       dim3((unsigned)w.groups), block, 0, st, w.p, w.r, w.chunk_states, held, w.ascending, w.descending);
+    constexpr int TEAMS = NW == 4 && (!TD_INST_BF16 || size > 128) ? 2 : 1;
+    hipLaunchKernelGGL((td_decay_backward_kernel<T, DA, DC, NW, TEAMS, VEC, TD_INST_KIND == 4, 2>), dim3((unsigned)w.groups), dim3(64 * NW * TEAMS), 0, st, w.p, w.r,
+                       w.chunk_states, held, w.ascending, w.descending);
 #endif
     TD_LAUNCH_CHECK();
     return TD_OK;
