@@ -370,3 +370,33 @@ def test_captured_beside_an_eager_graph(dev):
         torch.cuda.synchronize()
         for a, b in zip(got, want):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("T", [1, 17, 40, 64, 100, 129])
+@pytest.mark.parametrize("Dk, Dv", [(64, 128), (128, 48), (41, 101), (101, 41)])
+def test_rectangles(Dk, Dv, T, dtype, dev):
+    """States wider than high and the other way round, at every number of row tiles that the last rows of a sequence can have."""
+    _check(_inputs(T + Dk, (2, T), 2, 2, 1, 2, 2, Dk, Dv, dtype, True), dev)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("B, T, H, D", [(100, 530, 2, 40), (3, 1100, 2, 72), (2, 700, 2, 16)], ids=["whole", "wide cut", "narrow cut"])
+def test_cut_or_whole(B, T, H, D, dtype, dev):
+    """Sequences long enough to be cut into segments, enough of them to be left whole, and states that are cut differently backward."""
+    x = _inputs(T, (B, T), B, H, H, H, H, D, D, dtype, True)
+    from timediff_amd.decay_attention import decay_attention
+    names = ["q", "k", "v", "log_decay", "state"]
+    leaf = {n: x[n].to(dev).requires_grad_() for n in names}
+    o, s = decay_attention(*(leaf[n] for n in names[:4]), initial_state=leaf["state"], return_state=True)
+    d = dict(zip(names, torch.autograd.grad([o, s], list(leaf.values()), [x["grad_o"].to(dev), x["grad_state"].to(dev)])))
+    few = slice(0, 2)             # a sequence's results are its own; log_decay's gradient sums over all of them
+    y = {n: t if n == "log_decay" else t[few] for n, t in x.items()}
+    size = {n: t.abs() if n != "log_decay" else t for n, t in y.items()}
+    want, big = (ref.decay_attention(z["q"], z["k"], z["v"], z["log_decay"], state=z["state"]) for z in (y, size))
+    _close("o", o[few], want[0], big[0], T, D)
+    _close("state", s[few], want[1], big[1], T, D)
+    dwant, dbig = (ref.gradients(z["q"], z["k"], z["v"], z["log_decay"], z["grad_o"], z["grad_state"], state=z["state"]) for z in (y, size))
+    for n in names:
+        if n != "log_decay" or B == 2:
+            _close("grad " + n, d[n] if n == "log_decay" else d[n][few], dwant[n], dbig[n], 3 * T * (B if n == "log_decay" else 1), D)
