@@ -436,11 +436,15 @@ __global__ __launch_bounds__(256, 1) void td_rnn_layer_kernel(TdLayerParams p) {
                 // rows r-1, r are neighbours in the bf16 fragment: convert them as a pair
                 if constexpr ((r & 1) == 0) hprev = hval;
                 else {
-                    const __bf16 b0 = (__bf16)hprev, b1 = (__bf16)hval;
-                    hn[2 * ub + (r >> 3)][(r & 7) - 1] = b0;
-                    hn[2 * ub + (r >> 3)][r & 7] = b1;
+                    typedef __attribute__((ext_vector_type(2))) float f32x2;
+                    typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+                    const bf16x2 b = __builtin_convertvector(f32x2{hprev, hval}, bf16x2);
+                    hn[2 * ub + (r >> 3)][(r & 7) - 1] = b[0];
+                    hn[2 * ub + (r >> 3)][r & 7] = b[1];
                     if constexpr (HEAD) {
-                        const float f0 = (float)b0, f1 = (float)b1;
+                        // the values from the pair's bits: converted one by one they cost two conversions more
+                        const uint32_t bits = __builtin_bit_cast(uint32_t, b);
+                        const float f0 = __uint_as_float(bits << 16), f1 = __uint_as_float(bits & 0xFFFF0000u);
                         hs1 += f0 + f1;
                         hs2 = __builtin_fmaf(f0, f0, __builtin_fmaf(f1, f1, hs2));
                     }
