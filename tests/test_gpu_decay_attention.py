@@ -400,3 +400,15 @@ def test_cut_or_whole(B, T, H, D, dtype, dev):
     for n in names:
         if n != "log_decay" or B == 2:
             _close("grad " + n, d[n] if n == "log_decay" else d[n][few], dwant[n], dbig[n], 3 * T * (B if n == "log_decay" else 1), D)
+
+
+@pytest.mark.parametrize("B, H, Dk, Dv", [(200, 3, 40, 72), (300, 2, 7, 16), (171, 3, 128, 30), (3, 1, 128, 32), (4, 2, 120, 50), (2, 3, 50, 120)])
+def test_step_forms(B, H, Dk, Dv, dev):
+    """Few and many states, narrow and wide: every number of threads and of columns of the single row."""
+    from timediff_amd.decay_attention import decay_attention_step
+    x = _inputs(B + Dk, (B, 1), B, H, H, H, H, Dk, Dv, F32, True)
+    want, big = (ref.decay_attention(*(f(x[n]) for n in "qkv"), x["log_decay"], state=f(x["state"])) for f in (lambda t: t, torch.abs))
+    state = x["state"].to(dev)
+    o = decay_attention_step(*(x[n][:, 0].to(dev) for n in "qkv"), x["log_decay"].to(dev), state)
+    _close("o", o, want[0][:, 0], big[0][:, 0], 1, Dk)
+    _close("state", state, want[1], big[1], 1, Dk)

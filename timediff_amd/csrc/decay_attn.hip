@@ -89,18 +89,22 @@ __global__ __launch_bounds__(256) void td_decay_share_sum_kernel(const float *__
     }
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void td_decay_step_kernel(Pass P) {
-    constexpr int D = TD_DECAY_MAX_DIM;
-    __shared__ float part[256];
-    const int h = blockIdx.x % P.heads, n = blockIdx.x / P.heads, tid = threadIdx.x, col = tid & (D - 1), half = tid / D;
+// One row: a workgroup of NT threads for each state, W threads across its columns, the NT / W groups of them sharing out the rows.  Bound by memory:
+// the state is read and written once (1024 x 8 states of 128 x 128: 4.4 TB/s).  W: the least of 16, 32, 64 and 128 that has every column (with
+// 128 for all of them 2048 x 8 states of 64 x 64 take 172 us, with 64 125; 4096 x 8 of 32 x 32 float32 147 and 55).
+template <typename T, int W, int NT>
+__global__ __launch_bounds__(NT) void td_decay_step_kernel(Pass P) {
+    constexpr int GROUPS = NT / W;
+    __shared__ float part[NT];
+    const int h = blockIdx.x % P.heads, n = blockIdx.x / P.heads, tid = threadIdx.x, col = tid % W, group = tid / W;
     const float g = expf(P.log_decay[h]);
     float sum = 0.0f;
     if (col < P.dc) {
         const T *a = base_of<T>(P.a, false, n, h), *b = base_of<T>(P.b, false, n, h);
         const float c = as_float<T>(base_of<T>(P.c, false, n, h)[col]);
         float *S = P.state_out + (int64_t)blockIdx.x * P.da * P.dc + col;
-        for (int i = half; i < P.da; i += 2) {
+#pragma unroll 4
+        for (int i = group; i < P.da; i += GROUPS) {
             const float s = g * S[(int64_t)i * P.dc] + as_float<T>(b[i]) * c;
             S[(int64_t)i * P.dc] = s;
             sum += as_float<T>(a[i]) * s;
@@ -108,7 +112,24 @@ __global__ __launch_bounds__(256) void td_decay_step_kernel(Pass P) {
     }
     part[tid] = sum;
     __syncthreads();
-    if (half == 0 && col < P.dc) ((T *)P.out)[(int64_t)blockIdx.x * P.dc + col] = (T)((part[tid] + part[tid + D]) * P.out_scale);
+    if (group == 0 && col < P.dc) {
+#pragma unroll
+        for (int k = 1; k < GROUPS; ++k) sum += part[tid + k * W];
+        ((T *)P.out)[(int64_t)blockIdx.x * P.dc + col] = (T)(sum * P.out_scale);
+    }
+}
+template <typename T, int NT> void launch_step(const Pass &P, hipStream_t st) {
+    const dim3 grid(P.n_seq * P.heads), block(NT);
+    if (NT == 256 && P.dc <= 16) hipLaunchKernelGGL((td_decay_step_kernel<T, 16, 256>), grid, block, 0, st, P);
+    else if (P.dc <= 32) hipLaunchKernelGGL((td_decay_step_kernel<T, 32, NT>), grid, block, 0, st, P);
+    else if (P.dc <= 64) hipLaunchKernelGGL((td_decay_step_kernel<T, 64, NT>), grid, block, 0, st, P);
+    else hipLaunchKernelGGL((td_decay_step_kernel<T, 128, NT>), grid, block, 0, st, P);
+}
+// Few states that are not small: 1024 threads for each, of which the chip holds 512 (64 x 8 states of 128 x 128: 14 us a call, 22 with 256 threads; 65 x 8
+// take 23 either way)
+template <typename T> void launch_step(const Pass &P, hipStream_t st) {
+    if (P.n_seq * P.heads <= 512 && P.da * P.dc >= 4096) launch_step<T, 1024>(P, st);
+    else launch_step<T, 256>(P, st);
 }
 
 // ---- host side -----------------------------------------------------------------------------------------------------------
@@ -359,9 +380,8 @@ extern "C" int td_decay_step(const td_decay_config *cfg, const void *q, const vo
     P.c = view(cfg, v, cfg->v_stride, cfg->v_heads, cfg->dv);
     P.da = cfg->dk; P.dc = cfg->dv;
     P.state_out = state; P.out = o; P.out_scale = cfg->scale;
-    const dim3 grid(cfg->n_seq * cfg->heads);
-    if (cfg->dtype == TD_BF16) hipLaunchKernelGGL(td_decay_step_kernel<__bf16>, grid, dim3(256), 0, (hipStream_t)stream, P);
-    else hipLaunchKernelGGL(td_decay_step_kernel<float>, grid, dim3(256), 0, (hipStream_t)stream, P);
+    if (cfg->dtype == TD_BF16) launch_step<__bf16>(P, (hipStream_t)stream);
+    else launch_step<float>(P, (hipStream_t)stream);
     TD_LAUNCH_CHECK();
     return TD_OK;
 }
