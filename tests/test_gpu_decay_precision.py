@@ -1,0 +1,84 @@
+"""How exact decay attention is: bfloat16 results are the float32 results rounded once.
+
+One row of each sequence (many sequences) has a closed form, with x . y the sum over D entries and S, dS the entering state and the
+gradient of the state left behind:
+    o = c (q . k) v + c g S^T q         dq = c (v . do) k + c g S do         state = g S + k v^T
+    dk = c (v . do) q + dS v            dv = c (q . k) do + dS^T k           dstate = g (dS + c q do^T)
+Float32 computes each with sums of D products (of bfloat16 values: exact), D roundings of 2^-24 each, and at most 12 more: the
+weight g by exp2 (2) of a rounded exponent (|log2 g| <= 1: 2), the scale, a product carried as three bfloat16 terms (2^-24 once, and its
+three products added: 3), the products with weight and scale (3), the sum of the two parts (1).  Then one rounding to bfloat16: half
+a step at the result."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+@pytest.fixture(scope="module")
+def dev():
+    assert torch.cuda.is_available(), "these tests need the MI355X"
+    return torch.device("cuda:0")
+
+
+def _half_step(x):
+    """Half the distance between bfloat16 neighbours at x (float64 holding bfloat16 values)."""
+    return torch.ldexp(torch.ones_like(x), torch.frexp(x).exponent - 9)
+
+
+@pytest.mark.parametrize("D", [4, 40, 72, 128])
+@pytest.mark.parametrize("state", [False, True], ids=["alone", "with a state"])
+@pytest.mark.parametrize("slope", [False, True], ids=["fixed decay", "learned decay"])
+def test_one_row(D, state, slope, dev):
+    from timediff_amd.decay_attention import decay_attention
+    B, H, c = 4096 if D == 4 else 512, 2, 0.37
+    g = torch.Generator(device=dev).manual_seed(D)
+    r = lambda *s: torch.randn(*s, generator=g, device=dev)  # noqa: E731
+    q, k, v, do = (r(B, 1, H, D).to(BF16) for _ in range(4))
+    S, dS = (r(B, H, D, D), r(B, H, D, D)) if state else (None, None)
+    ld = torch.tensor([-0.01, -0.6], device=dev)
+    leaf = [t.clone().requires_grad_() for t in (q, k, v)] + ([S.clone().requires_grad_()] if state else [])
+    o, s = decay_attention(*leaf[:3], ld.clone().requires_grad_(slope), scale=c, initial_state=leaf[3] if state else None, return_state=True)
+    d = torch.autograd.grad([o, s] if state else [o], leaf, [do, dS] if state else [do])
+    got = dict(zip(("o", "dq", "dk", "dv", "dS"), [o.detach(), *d]))
+    c32 = float(torch.tensor(c, dtype=F32))
+
+    def formula(mag):
+        f = (lambda t: t.double().abs()) if mag else (lambda t: t.double())  # noqa: E731
+        Q, K, V, DO = (f(t)[:, 0] for t in (q, k, v, do))
+        w = ld.double().exp()[:, None]
+        qk, vo = (Q * K).sum(-1, keepdim=True), (V * DO).sum(-1, keepdim=True)
+        res = dict(o=c32 * qk * V, dq=c32 * vo * K, dk=c32 * vo * Q, dv=c32 * qk * DO)
+        if state:
+            left, right = (lambda M, x: (M * x[..., None, :]).sum(-1)), (lambda M, x: (M * x[..., :, None]).sum(-2))
+            E, dE = f(S), f(dS)
+            res["o"] = res["o"] + c32 * w * right(E, Q)
+            res["dq"] = res["dq"] + c32 * w * left(E, DO)
+            res["dk"] = res["dk"] + left(dE, V)
+            res["dv"] = res["dv"] + right(dE, K)
+            res["dS"] = w[..., None] * (dE + c32 * Q[..., :, None] * DO[..., None, :])
+        return res
+    want, size = formula(False), formula(True)
+    for n, w in want.items():
+        x = got[n].double()
+        x = x if n == "dS" else x[:, 0]
+        room = (D + 12) * 2.0 ** -24 * size[n] + (2.0 ** -24 * w.abs() if n == "dS" else _half_step(x))
+        off = (x - w).abs() - room
+        assert (off <= 0).all(), f"{n}: {(off > 0).sum().item()} of {off.numel()} further off than float32 and one rounding allow, by {off.max().item():.3g}"
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("Dk, Dv", [(16, 16), (64, 64), (64, 128), (128, 64), (128, 128), (41, 101)])
+def test_gradients_do_not_depend_on_what_else_is_wanted(Dk, Dv, dtype, dev):
+    """q's, k's and v's gradients are the same bits with learned and with fixed decays."""
+    from timediff_amd.decay_attention import decay_attention
+    g = torch.Generator().manual_seed(5)
+    q, k, v, do = (torch.randn(2, 150, 2, d, generator=g).to(dtype).to(dev) for d in (Dk, Dk, Dv, Dv))
+    res = []
+    for slope in (True, False):
+        leaf = [t.clone().requires_grad_() for t in (q, k, v)]
+        o = decay_attention(*leaf, torch.tensor([-0.02, -0.4], device=dev, requires_grad=slope))
+        res.append(torch.autograd.grad(o, leaf, do))
+    for a, b in zip(*res):
+        assert torch.equal(a, b)

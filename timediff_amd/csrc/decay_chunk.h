@@ -9,9 +9,9 @@
 //     the operand of F^T a, and the scores' accumulators (rows j in registers, lane = row i) the operand of the sum over j: the waves
 //     share out the ten score tiles on and below the diagonal and pass them on through LDS as operands, lane by lane;
 //   * b and c are read from LDS with rows as the inner index by transposing loads (ds_read_b64_tr_b16).
-// bfloat16: v_mfma_f32_16x16x32_bf16, and an operand that is not an input is split into bf16 terms: scores and states
-// into two (2^-17 of each, below what the output's own rounding leaves), decayed rows that enter the state, and everything behind a float32
-// result, into three (2^-24).  float32: v_mfma_f32_16x16x4_f32.
+// bfloat16: v_mfma_f32_16x16x32_bf16, and an operand that is not an input (scores, states, decayed rows that enter the state) is split into three
+// bf16 terms, 2^-24 of it: a result is float32's, rounded once.  (Two terms for scores and states, 2^-17 of each, change one bfloat16 result in
+// a few hundred.)  float32: v_mfma_f32_16x16x4_f32.
 #pragma once
 #include "common.h"
 
@@ -348,11 +348,11 @@ template <int NI> struct Tiles {
 };
 
 // One product stream: the state M (DA x DC) and what a chunk does with it.  TA x CT tiles of the state a wave.
-template <typename T, int DA, int DC, int NW, bool VEC, int TERMS, int NI = 4> struct Stream {
+template <typename T, int DA, int DC, int NW, bool VEC, int NI = 4> struct Stream {
     typedef Mat<T> M;
     typedef typename M::Op Op;
     static constexpr int LA = DA, LC = DC, PA = M::pitch(DA), PC = M::pitch(DC), TA = DA / 16, CT = DC / 16 / NW, KS = TA / M::KT, RT = CHUNK / 16, KR = RT / M::KT;
-    static constexpr int S2 = M::SPLIT ? 2 : 1, S3 = M::SPLIT ? 3 : 1, SF = M::SPLIT ? TERMS : 1;      // terms of scores, of decayed rows, of the state
+    static constexpr int TERMS = M::SPLIT ? 3 : 1;      // of scores, of decayed rows and of the state
     static constexpr int PAIRS = M::KT == 2 ? RT / 2 * (RT / 2 + 1) : RT * (RT + 1) / 2;               // score operands: (it, kr), kr <= it / KT
     static_assert(CT * NW * 16 == DC && CT > 0, "every column tile has a wave");
     f32x4 S[TA][CT], o[NI][CT];
@@ -370,7 +370,7 @@ template <typename T, int DA, int DC, int NW, bool VEC, int TERMS, int NI = 4> s
 #pragma unroll
             for (int it = 0; it < RT; it += 2)
 #pragma unroll
-                for (int k = 0; k < S2; ++k) scores[(pair(it, it / 2) * S2 + k) * 64 + lane] = zero;
+                for (int k = 0; k < TERMS; ++k) scores[(pair(it, it / 2) * TERMS + k) * 64 + lane] = zero;
     }
     // (b_j . a_i) of tile (it, jt)
     static __device__ __forceinline__ f32x4 score(const T *la, const T *lb, int it, int jt, int g, int li) {
@@ -380,7 +380,7 @@ template <typename T, int DA, int DC, int NW, bool VEC, int TERMS, int NI = 4> s
         return w;
     }
     static __device__ __forceinline__ void keep(f32x4 w, Op *scores, int it, int jt, int lane) {
-        M::template keep<S2>(w, scores + pair(it, jt / M::KT) * S2 * 64 + lane, jt % M::KT);
+        M::template keep<TERMS>(w, scores + pair(it, jt / M::KT) * TERMS * 64 + lane, jt % M::KT);
     }
     __device__ __forceinline__ void enter(const float *from, int64_t st_a, int64_t st_c, int da, int dc, int wave, int g, int li) {
 #pragma unroll
@@ -418,13 +418,13 @@ template <typename T, int DA, int DC, int NW, bool VEC, int TERMS, int NI = 4> s
             for (int ct = 0; ct < CT; ++ct) o[j][ct] = f32x4{0, 0, 0, 0};
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
-            Op f[CT][SF];
+            Op f[CT][TERMS];
 #pragma unroll
             for (int ct = 0; ct < CT; ++ct) {
                 f32x4 part[M::KT];
 #pragma unroll
                 for (int k = 0; k < M::KT; ++k) part[k] = S[s * M::KT + k][ct];
-                M::template split<SF>(part, f[ct]);
+                M::template split<TERMS>(part, f[ct]);
             }
 #pragma unroll
             for (int j = 0; j < NI; ++j) {
@@ -433,7 +433,7 @@ template <typename T, int DA, int DC, int NW, bool VEC, int TERMS, int NI = 4> s
 #pragma unroll
                 for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
-                    for (int k = 0; k < SF; ++k) o[j][ct] = M::mma(f[ct][k], q, o[j][ct]);
+                    for (int k = 0; k < TERMS; ++k) o[j][ct] = M::mma(f[ct][k], q, o[j][ct]);
             }
         }
 #pragma unroll
@@ -478,8 +478,8 @@ template <typename T, int DA, int DC, int NW, bool VEC, int TERMS, int NI = 4> s
 #pragma unroll
             for (int kr = 0; kr < operands(j); ++kr)
 #pragma unroll
-                for (int k = 0; k < S2; ++k) {
-                    Op f = scores[(pair(tiles.at(j), kr) * S2 + k) * 64 + lane];
+                for (int k = 0; k < TERMS; ++k) {
+                    Op f = scores[(pair(tiles.at(j), kr) * TERMS + k) * 64 + lane];
                     if (NI == 2 && M::KT == 1) f = kr <= tiles.at(j) ? f : Op{};
 #pragma unroll
                     for (int ct = 0; ct < CT; ++ct) o[j][ct] = M::mma(vt[ct][kr], f, o[j][ct]);
@@ -533,7 +533,7 @@ template <typename T, int DA, int DC, int NW, bool VEC, int TERMS, int NI = 4> s
                     const int tile = kr * M::KT + k, j = tile * 16 + g * 4 + r;
                     wr[k][r] = R::FULL ? w.wu[r] * w.tiles[RT - 1 - tile] : j < n ? power(w.lg2, n - 1 - j + late) * scale : 0.0f;
                 }
-            Op u[CT][S3];
+            Op u[CT][TERMS];
 #pragma unroll
             for (int ct = 0; ct < CT; ++ct) {
                 f32x4 y[M::KT];
@@ -541,7 +541,7 @@ template <typename T, int DA, int DC, int NW, bool VEC, int TERMS, int NI = 4> s
                 for (int k = 0; k < M::KT; ++k)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) y[k][r] = M::elem(vt[ct][kr], k, r) * wr[k][r];
-                M::template split<S3>(y, u[ct]);
+                M::template split<TERMS>(y, u[ct]);
             }
 #pragma unroll
             for (int mt = 0; mt < TA; ++mt) {
@@ -549,7 +549,7 @@ template <typename T, int DA, int DC, int NW, bool VEC, int TERMS, int NI = 4> s
 #pragma unroll
                 for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
-                    for (int k = 0; k < S3; ++k) S[mt][ct] = M::mma(b, u[ct][k], S[mt][ct]);
+                    for (int k = 0; k < TERMS; ++k) S[mt][ct] = M::mma(b, u[ct][k], S[mt][ct]);
             }
         }
         settle();
@@ -583,7 +583,7 @@ template <int NT> __device__ __forceinline__ void workgroup_sum(double x, double
 
 // What a segment adds to the state
 template <typename T, int DA, int DC, int NW, bool VEC, bool REV, int WAVES> __global__ __launch_bounds__(64 * NW, WAVES) void td_decay_sum_kernel(Pass P) {
-    typedef Stream<T, DA, DC, NW, VEC, 2> X;
+    typedef Stream<T, DA, DC, NW, VEC> X;
     constexpr int NT = 64 * NW;
     __shared__ __align__(16) T lb[CHUNK * X::PA];
     __shared__ __align__(16) T lc[CHUNK * X::PC];
@@ -632,13 +632,13 @@ template <typename T, int DA, int DC, int NW, bool VEC, bool REV, int WAVES> __g
 // out from (a, b, c), rows ascending.  SLOPE: the part of the derivative by log g that rows owe to the states entering their chunks, dotted with
 // e, and those states for the pass over the other gradients.
 template <typename T, int DA, int DC, int NW, bool SLOPE> struct OutLds {
-    typedef Stream<T, DA, DC, NW, true, 2> X;
+    typedef Stream<T, DA, DC, NW, true> X;
     T a[CHUNK * X::PA], b[CHUNK * X::PA], c[CHUNK * X::PC], e[SLOPE ? CHUNK * X::PC : 8];
-    typename X::Op scores[X::PAIRS * X::S2 * 64];
+    typename X::Op scores[X::PAIRS * X::TERMS * 64];
 };
 template <typename T, int DA, int DC, int NW, int TEAMS, bool VEC, bool SLOPE>
 __device__ __forceinline__ void out_sweep(const Pass &P, int item, OutLds<T, DA, DC, NW, SLOPE> &lds, float *chunk_states) {
-    typedef Stream<T, DA, DC, NW, VEC, SLOPE ? 3 : 2, 4 / TEAMS> X;
+    typedef Stream<T, DA, DC, NW, VEC, 4 / TEAMS> X;
     typedef typename X::Op Op;
     constexpr int NT = 64 * NW * TEAMS;
     T *const la = lds.a, *const lb = lds.b, *const lc = lds.c, *const le = lds.e;
@@ -733,14 +733,14 @@ template <typename T, int DA, int DC, int NW, bool VEC, int WAVES> __global__ __
 // row before and one behind it, which is n g^n <state entering the chunk, its gradient when it leaves>.  TEAMS = 2: NW waves for each of the two
 // gradients, at the same time, where one workgroup's LDS or registers fill a compute unit and NW = 4 waves would leave half of each SIMD's places empty.
 template <typename T, int DK, int DV, int NW> struct PairLds {
-    typedef Stream<T, DK, DV, NW, true, 2> V;
+    typedef Stream<T, DK, DV, NW, true> V;
     T k[CHUNK * V::PA], q[CHUNK * V::PA], o[CHUNK * V::PC], v[CHUNK * V::PC];
-    typename V::Op scores[2][V::PAIRS * V::S2 * 64];
+    typename V::Op scores[2][V::PAIRS * V::TERMS * 64];
 };
 template <typename T, int DK, int DV, int NW, int TEAMS, bool VEC, bool SLOPE>
 __device__ __forceinline__ void pair_sweep(const Pass &P, int item, PairLds<T, DK, DV, NW> &lds, const float *chunk_states) {
-    typedef Stream<T, DK, DV, NW, VEC, 2> V;
-    typedef Stream<T, DV, DK, NW, VEC, SLOPE ? 3 : 2> K;
+    typedef Stream<T, DK, DV, NW, VEC> V;
+    typedef Stream<T, DV, DK, NW, VEC> K;
     typedef typename V::Op Op;
     constexpr int NT = 64 * NW * TEAMS;
     T *const lk = lds.k, *const lq = lds.q, *const lo = lds.o, *const lv = lds.v;
