@@ -485,6 +485,7 @@ template <typename T, int DA, int DC, int NW, bool VEC, int NI = 4> struct Strea
                     for (int ct = 0; ct < CT; ++ct) o[j][ct] = M::mma(vt[ct][kr], f, o[j][ct]);
                 }
         }
+        settle();                 // the lanes without a row branch past the readers
 #pragma unroll
         for (int j = 0; j < NI; ++j)
 #pragma unroll
