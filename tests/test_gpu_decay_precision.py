@@ -82,3 +82,25 @@ def test_gradients_do_not_depend_on_what_else_is_wanted(Dk, Dv, dtype, dev):
         res.append(torch.autograd.grad(o, leaf, do))
     for a, b in zip(*res):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("log_decay", [-0.01, -0.3, -0.6])
+def test_weights(log_decay, dev):
+    """One row's reach: with k_0 alone nonzero o_t = g^t, with grad_o's last row alone nonzero grad_v_j = g^(T-1-j), a single weight each, down
+    to 2^-111.  A weight is 2^x (one unit in the last place: 2 roundings), a first-order correction (2), and itself rounded (1), 3 more for the
+    products around it: 8 within a chunk of 64.  Across a border three weights (8 each), their products (6), and 2 for every chunk's decay."""
+    from timediff_amd.decay_attention import decay_attention
+    T = 128
+    one = torch.ones(1, T, 1, 1, device=dev)
+    k, do = torch.zeros_like(one), torch.zeros_like(one)
+    k[:, 0], do[:, -1] = 1, 1
+    ld = torch.tensor([log_decay], device=dev)
+    t = torch.arange(T, device=dev)
+    exact = torch.exp(ld.double() * t)
+    room = torch.where(t < 64, 8, 30 + 4) * 2.0 ** -24 * exact
+    o = decay_attention(one, k, one, ld, scale=1.0)[0, :, 0, 0].double()
+    v = one.clone().requires_grad_()
+    dv = torch.autograd.grad(decay_attention(one, one, v, ld, scale=1.0), v, do)[0][0, :, 0, 0].double().flip(0)
+    for name, x in (("o", o), ("dv", dv)):
+        off = (x - exact).abs() - room
+        assert (off <= 0).all(), f"{name}: {((x - exact).abs() / exact).max().item() * 2 ** 24:.1f} roundings at most, {(off > 0).nonzero().flatten().tolist()[:5]} ..."

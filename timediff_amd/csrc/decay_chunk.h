@@ -82,8 +82,24 @@ __device__ __forceinline__ void slot_owner(const Pass &P, int slot, int &n, int 
     segment = slot - first_place(P, lo, P.seg_len);
 }
 
-// g^e for a whole number e: 1 for e = 0, also where log g is -inf
-__device__ __forceinline__ float power(float lg2, int e) { return e == 0 ? 1.0f : __builtin_amdgcn_exp2f(lg2 * (float)e); }
+// log2 g as two floats.  One float alone, multiplied by e, leaves 2^-24 |log2 g^e| twice in the exponent: a weight of 2^-50 would be off by 40
+// roundings.  Finite (g = 0 is 2^-1e30), so that e = 0 gives 1.
+struct Log2 {
+    float hi, lo;
+    static __device__ __forceinline__ Log2 of(float log_g) {
+        log_g = log_g < -1e30f ? -1e30f : log_g > 1e30f ? 1e30f : log_g;
+        const float x = log_g * 1.44269502f;                       // log2(e) = 1.44269502162933 + 1.92596299e-8
+        return Log2{x, __builtin_fmaf(log_g, 1.92596299e-8f, __builtin_fmaf(log_g, 1.44269502f, -x))};
+    }
+};
+
+// g^e for a whole number e: 2^x by the hardware (one unit in the last place), times 1 and what x leaves out, to first order (half a unit at
+// most while 2^x is neither 0 nor infinite; the bound keeps those two what they are).  No selection: the compiler makes branches of them, and between
+// matrix instructions a branch is a place where it has left out waits.
+__device__ __forceinline__ float power(Log2 lg2, int e) {
+    const float n = (float)e, x = lg2.hi * n, rest = __builtin_fmaf(lg2.lo, n, __builtin_fmaf(lg2.hi, n, -x));
+    return __builtin_amdgcn_exp2f(x) * fmaxf(__builtin_fmaf(rest, 0.693147181f, 1.0f), 0.5f);
+}
 
 // g^e as two floats: it multiplies a state again and again, and its own rounding would add up over a long memory
 struct Factor { float hi, lo; };
@@ -92,7 +108,7 @@ __device__ __forceinline__ Factor factor(float log_g, int e) {
     const float hi = (float)x;
     return Factor{hi, isinf(hi) || hi == 0.0f ? 0.0f : (float)(x - (double)hi)};
 }
-__device__ __forceinline__ float times(Factor f, float x) { return f.hi * x + f.lo * x; }
+__device__ __forceinline__ float times(Factor f, float x) { return __builtin_fmaf(f.hi, x, f.lo * x); }
 
 template <typename T> struct Mat;
 template <> struct Mat<__bf16> {
@@ -309,12 +325,13 @@ struct Place {
 // The weights of a head that every chunk uses
 template <int NW> struct Weights {
     static constexpr int RT = CHUNK / 16, SCORES = RT * (RT + 1) / 2, MINE = (SCORES + NW - 1) / NW;   // score tiles; at most so many a wave
-    float lg2, wo, wu[4], wa[MINE][4], tiles[RT];
+    Log2 lg2;
+    float wo, wu[4], wa[MINE][4], tiles[RT];
     int it[MINE], jt[MINE];
     Factor whole;
     // late: 1 in reversed passes
     __device__ __forceinline__ void init(float log_g, float scale, int late, int wave, int g, int li) {
-        lg2 = log_g * 1.44269504f;
+        lg2 = Log2::of(log_g);
         whole = factor(log_g, CHUNK);
         wo = power(lg2, li + 1 - late);                                             // of row i: g^(its place in its tile + 1), times
 #pragma unroll
@@ -338,7 +355,7 @@ template <int NW> struct Weights {
 template <int NI> struct Tiles {
     int team;
     float factor[NI];            // g^(16 tile)
-    __device__ __forceinline__ void init(float lg2, int team_) {
+    __device__ __forceinline__ void init(Log2 lg2, int team_) {
         team = team_;
 #pragma unroll
         for (int j = 0; j < NI; ++j) factor[j] = power(lg2, 16 * at(j));
@@ -841,7 +858,7 @@ __device__ __forceinline__ void pair_sweep(const Pass &P, int item, PairLds<T, D
                         for (int ct = 0; ct < X::CT; ++ct)
 #pragma unroll
                             for (int r = 0; r < 4; ++r) cross += F[mt][ct][r] * x.S[mt][ct][r];
-                    slope += (double)(sum + (float)n * power(w.lg2, n) * cross);
+                    slope += (double)(sum + (float)n * (R::FULL ? w.whole.hi : power(w.lg2, n)) * cross);
                 }
                 phase();
                 x.template advance<R>(ly, n, w, P.upd_scale, 1, g, li);
@@ -912,7 +929,7 @@ __device__ __forceinline__ void pair_sweep(const Pass &P, int item, PairLds<T, D
                     for (int ct = 0; ct < K::CT; ++ct)
 #pragma unroll
                         for (int r = 0; r < 4; ++r) cross += F[mt][ct][r] * xk.S[mt][ct][r];
-                slope += (double)(sum + (float)n * power(w.lg2, n) * cross);
+                slope += (double)(sum + (float)n * (R::FULL ? w.whole.hi : power(w.lg2, n)) * cross);
             }
             phase();
             xk.template advance<R>(lo, n, w, P.upd_scale, 1, g, li);
