@@ -104,3 +104,27 @@ def test_weights(log_decay, dev):
     for name, x in (("o", o), ("dv", dv)):
         off = (x - exact).abs() - room
         assert (off <= 0).all(), f"{name}: {((x - exact).abs() / exact).max().item() * 2 ** 24:.1f} roundings at most, {(off > 0).nonzero().flatten().tolist()[:5]} ..."
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("D", [16, 48, 100])
+@pytest.mark.parametrize("T, log_decay", [(1, 6.0), (5, 3.0), (20, 2.9), (40, 1.5), (50, 1.45)])
+def test_growing_states_of_short_sequences(T, log_decay, D, dtype, dev):
+    """Decays above zero whose g^T is far from overflowing, while g^32 or g^64 would: every result is finite, log_decay's gradient too, and as
+    near the 64-bit one as float32's sums of T and D terms, 32 roundings beside, and a rounding to the result's type allow."""
+    import decay_reference as ref
+    from timediff_amd.decay_attention import decay_attention
+    g = torch.Generator().manual_seed(T)
+    x = {n: torch.randn(2, T, 2, D, generator=g).to(dtype) for n in ("q", "k", "v", "do")}
+    x["S"], x["dS"] = torch.randn(2, 2, D, D, generator=g), torch.randn(2, 2, D, D, generator=g)
+    x["ld"] = torch.tensor([log_decay, 0.5])
+    names = ["q", "k", "v", "ld", "S"]
+    leaf = {n: x[n].to(dev).requires_grad_() for n in names}
+    o, s = decay_attention(*(leaf[n] for n in names[:4]), initial_state=leaf["S"], return_state=True)
+    got = torch.autograd.grad([o, s], [leaf[n] for n in names], [x["do"].to(dev), x["dS"].to(dev)])
+    want, size = (ref.gradients(f(x["q"]), f(x["k"]), f(x["v"]), x["ld"], f(x["do"]), f(x["dS"]), state=f(x["S"])) for f in (lambda t: t, torch.abs))
+    for n, d in zip(("q", "k", "v", "log_decay", "state"), got):
+        d = d.cpu().double()
+        assert torch.isfinite(d).all(), n
+        room = ((4 if n == "log_decay" else 1) * T + 2 * D + 32) * 2.0 ** -24 * size[n] + (2.0 ** -8 if dtype is BF16 and n in "qkv" else 2.0 ** -24) * want[n].abs()
+        assert ((d - want[n]).abs() <= room).all(), n

@@ -348,6 +348,8 @@ template <int NW> struct Weights {
         }
     }
     __device__ __forceinline__ int apart(int m, int r, int g, int li) const { return (it[m] - jt[m]) * 16 + li - (g * 4 + r); }
+    // wa of the n rows there are
+    template <typename R> __device__ __forceinline__ float score(int m, int r, int n, int li) const { return R::FULL || it[m] * 16 + li < n ? wa[m][r] : 0.0f; }
 };
 
 // Which of a chunk's four row tiles a wave's outputs have.  NI = 4: all of them.  NI = 2: two teams of waves hold the same state, team 0 has the
@@ -427,8 +429,8 @@ template <typename T, int DA, int DC, int NW, bool VEC, int NI = 4> struct Strea
                     if (i < da && j < dc) to[i * st_a + j * st_c] = S[mt][ct][r];
                 }
     }
-    // o = g^(i+1) F^T a
-    template <typename R, typename W> __device__ __forceinline__ void from_state(const T *la, const W &w, int g, int li) {
+    // o = g^(i+1) F^T a (rows behind the n-th have no weight: g^(i+1) of a growing state may be infinite there)
+    template <typename R, typename W> __device__ __forceinline__ void from_state(const T *la, int n, const W &w, int g, int li) {
 #pragma unroll
         for (int j = 0; j < NI; ++j)
 #pragma unroll
@@ -454,9 +456,11 @@ template <typename T, int DA, int DC, int NW, bool VEC, int NI = 4> struct Strea
             }
         }
 #pragma unroll
-        for (int j = 0; j < NI; ++j)
+        for (int j = 0; j < NI; ++j) {
+            const float weight = R::FULL || tiles.at(j) * 16 + li < n ? w.wo * tiles.factor[j] : 0.0f;
 #pragma unroll
-            for (int ct = 0; ct < CT; ++ct) o[j][ct] = o[j][ct] * (w.wo * tiles.factor[j]);
+            for (int ct = 0; ct < CT; ++ct) o[j][ct] = o[j][ct] * weight;
+        }
     }
     // sum of (first + i) o_i . e_i over this lane's entries
     template <typename R> __device__ __forceinline__ float dot(const T *le, int first, int wave, int g, int li) const {
@@ -712,7 +716,7 @@ __device__ __forceinline__ void out_sweep(const Pass &P, int item, OutLds<T, DA,
             if (it >= R::LIVE) continue;
             f32x4 s = X::score(la, lb, it, jt, g, li);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) s[r] *= w.wa[m][r];
+            for (int r = 0; r < 4; ++r) s[r] *= w.template score<R>(m, r, n, li);
             X::keep(s, scores, it, jt, lane);
         }
         if (SLOPE && team == 0) {
@@ -723,7 +727,7 @@ __device__ __forceinline__ void out_sweep(const Pass &P, int item, OutLds<T, DA,
                 for (int ct = 0; ct < X::CT; ++ct) to[(mt * X::CT + ct) * 64] = x.S[mt][ct];
         }
         phase();
-        x.template from_state<R>(la, w, g, li);
+        x.template from_state<R>(la, n, w, g, li);
         if (SLOPE) slope += (double)(x.template dot<R>(le, 1, wave, g, li) * P.out_scale);
         __syncthreads();
         phase();
@@ -834,7 +838,7 @@ __device__ __forceinline__ void pair_sweep(const Pass &P, int item, PairLds<T, D
                     if (it >= R::LIVE) continue;
                     f32x4 s = X::score(lx, ly, it, jt, g, li);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) s[r] *= w.wa[m][r];
+                    for (int r = 0; r < 4; ++r) s[r] *= w.template score<R>(m, r, n, li);
                     X::keep(s, scores, it, jt, lane);
                     if (SL) {
                         const f32x4 other = V::score(lk, lq, it, jt, g, li);
@@ -844,7 +848,7 @@ __device__ __forceinline__ void pair_sweep(const Pass &P, int item, PairLds<T, D
                 }
                 const int64_t row0 = (packed ? 0 : (int64_t)at.n_seq * P.rows) + at.lo + t;
                 phase();
-                x.template from_state<R>(lx, w, g, li);
+                x.template from_state<R>(lx, n, w, g, li);
                 if (SL) sum += x.template dot<R>(lk, 0, wave, g, li);
                 __syncthreads();
                 phase();
@@ -906,16 +910,17 @@ __device__ __forceinline__ void pair_sweep(const Pass &P, int item, PairLds<T, D
                 f32x4 sv = V::score(lk, lq, it, jt, g, li), sk = K::score(lv, lo, it, jt, g, li);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    sv[r] *= w.wa[m][r];
+                    const float weight = w.template score<R>(m, r, n, li);
+                    sv[r] *= weight;
                     if (SLOPE) sum += (float)w.apart(m, r, g, li) * sv[r] * sk[r];
-                    sk[r] *= w.wa[m][r];
+                    sk[r] *= weight;
                 }
                 V::keep(sv, scores_v, it, jt, lane);
                 K::keep(sk, scores_k, it, jt, lane);
             }
             const int64_t row0 = (packed ? 0 : (int64_t)at.n_seq * P.rows) + at.lo + t;
             phase();
-            xk.template from_state<R>(lv, w, g, li);
+            xk.template from_state<R>(lv, n, w, g, li);
             if (SLOPE) sum += xk.template dot<R>(lk, 0, wave, g, li);
             __syncthreads();
             phase();
@@ -934,7 +939,7 @@ __device__ __forceinline__ void pair_sweep(const Pass &P, int item, PairLds<T, D
             phase();
             xk.template advance<R>(lo, n, w, P.upd_scale, 1, g, li);
             phase();
-            xv.template from_state<R>(lk, w, g, li);
+            xv.template from_state<R>(lk, n, w, g, li);
             phase();
             xv.template columns<R>(lo, wave, g, li);
             xv.template from_rows<R, true>(scores_v, n, 1.0f, P.out, P.out_f32, row0, P.heads, h, P.dc, wave, lane);
