@@ -100,3 +100,13 @@ def test_reference_is_the_recurrence():
         S = torch.exp(ld) * S + k[t][:, None] * v[t][None, :]
         assert torch.allclose(o[t], 0.7 * q[t] @ S, rtol=1e-12, atol=1e-12)
     assert torch.allclose(s, S, rtol=1e-12, atol=1e-12)
+
+
+def test_rows_are_counted_in_32_bits():
+    L = _lib.lib()
+    cfg = _lib.DecayConfig(n_seq=1, rows=2 ** 31 - 129, heads=1, q_heads=1, k_heads=1, v_heads=1, dk=1, dv=1, dtype=_lib.BF16, scale=1.0)
+    for packed in (0, 1):
+        cfg.packed = packed
+        assert L.td_decay_workspace_bytes(C.byref(cfg), 0) > 0 and L.td_decay_workspace_bytes(C.byref(cfg), 1) > 0
+    cfg.rows += 1
+    assert L.td_decay_workspace_bytes(C.byref(cfg), 0) == 0 and b"rows must be" in L.td_last_error()

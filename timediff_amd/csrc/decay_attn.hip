@@ -33,7 +33,7 @@ template <bool REV> __global__ __launch_bounds__(256) void td_decay_scan_kernel(
     const int h = blockIdx.x / blocks % P.heads, n = blockIdx.x / blocks / P.heads;
     int lo, hi;
     row_range(P.offsets, P.rows, n, lo, hi);
-    const int segments = (hi - lo + P.seg_len - 1) / P.seg_len;
+    const int segments = hi > lo ? (hi - lo - 1) / P.seg_len + 1 : 0;
     if (segments < 2 || el >= size) return;
     const float ld = P.log_decay[h];
     const Factor whole = factor(ld, P.seg_len);
@@ -63,11 +63,11 @@ template <bool REV> __global__ __launch_bounds__(256) void td_decay_scan_kernel(
 }
 
 // grad_log_decay[h] = the sum of head h's parts, in an order of their own
-__global__ __launch_bounds__(1024) void td_decay_slope_kernel(const double *parts, int n, int heads, float *grad) {
+__global__ __launch_bounds__(1024) void td_decay_slope_kernel(const double *parts, int64_t n, int heads, float *grad) {
     __shared__ double red[1024];
     double s = 0.0;
 #pragma unroll 4
-    for (int i = threadIdx.x; i < n; i += 1024) s += parts[(int64_t)i * heads + blockIdx.x];
+    for (int64_t i = threadIdx.x; i < n; i += 1024) s += parts[i * heads + blockIdx.x];
     red[threadIdx.x] = s;
     __syncthreads();
     for (int o = 512; o > 0; o >>= 1) {
@@ -136,7 +136,8 @@ template <typename T> void launch_step(const Pass &P, hipStream_t st) {
 int check_config(const td_decay_config *c) {
     TD_REQUIRE(c, "configuration required");
     TD_REQUIRE(c->n_seq >= 1, "n_seq must be at least 1, got %d", c->n_seq);
-    TD_REQUIRE(c->rows >= 0, "rows must not be negative, got %d", c->rows);
+    // (a chunk's first row and the one behind it are counted in 32 bits)
+    TD_REQUIRE(c->rows >= 0 && c->rows <= INT32_MAX - 2 * CHUNK, "rows must be 0 .. %d, got %d", INT32_MAX - 2 * CHUNK, c->rows);
     TD_REQUIRE(c->packed == 0 || c->packed == 1, "packed must be 0 or 1, got %d", c->packed);
     TD_REQUIRE(c->dtype == TD_F32 || c->dtype == TD_BF16, "dtype must be TD_F32 or TD_BF16, got %d", c->dtype);
     TD_REQUIRE(c->dk >= 1 && c->dk <= TD_DECAY_MAX_DIM && c->dv >= 1 && c->dv <= TD_DECAY_MAX_DIM,
@@ -363,7 +364,7 @@ extern "C" int td_decay_backward(const td_decay_config *cfg, const void *q, cons
     if (grad_k && k_shared)
         if (int rc = share_sum(cfg, parts_k, grad_k, cfg->k_heads, cfg->dk, st)) return rc;
     if (slope) {
-        hipLaunchKernelGGL(td_decay_slope_kernel, dim3(cfg->heads), dim3(1024), 0, st, slopes, 2 * Q.slots, cfg->heads, grad_log_decay);
+        hipLaunchKernelGGL(td_decay_slope_kernel, dim3(cfg->heads), dim3(1024), 0, st, slopes, 2 * (int64_t)Q.slots, cfg->heads, grad_log_decay);
         TD_LAUNCH_CHECK();
     }
     return TD_OK;
