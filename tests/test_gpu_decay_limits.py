@@ -26,3 +26,23 @@ def test_rows_near_two_to_the_31(dev):
     want = torch.expm1(ld * (t + 1).double()) / torch.expm1(ld)
     room = (3 * 2.0 ** -24 / -torch.expm1(64 * ld) + 2.0 ** -8) * want
     assert ((o[t].double() - want).abs() <= room).all()
+
+
+def test_more_workgroups_than_one_launch_takes(dev):
+    """A launch holds fewer than 2^32 threads: 2^24 and a few states step with 256 each, 2^25 and a few sequences run with 128 each.  One
+    row and 1 x 1 states: o = c (g S + k v) q in float32 (10 roundings), rounded to bfloat16 (half a step)."""
+    from timediff_amd.decay_attention import decay_attention, decay_attention_step
+    g = torch.Generator(device=dev).manual_seed(1)
+    for n, step in ((2 ** 24 + 3, True), (2 ** 25 + 3, False)):
+        q, k, v = (torch.randn(n, 1, 1, generator=g, device=dev).to(BF16) for _ in range(3))
+        S, ld = torch.randn(n, 1, 1, 1, generator=g, device=dev), torch.tensor([-0.3], device=dev)
+        new = ld.double().exp() * S.double().view(-1) + k.double().view(-1) * v.double().view(-1)
+        size = S.double().view(-1).abs() + (k.double() * v.double()).view(-1).abs()
+        want = 0.5 * new * q.double().view(-1)
+        if step:
+            state = S.clone()
+            o = decay_attention_step(q, k, v, ld, state, scale=0.5)
+        else:
+            o, state = decay_attention(*(t[:, None] for t in (q, k, v)), ld, scale=0.5, initial_state=S, return_state=True)
+        assert ((state.view(-1).double() - new).abs() <= 10 * 2.0 ** -24 * size).all()
+        assert ((o.view(-1).double() - want).abs() <= 2.0 ** -8 * want.abs() + 20 * 2.0 ** -24 * size * q.double().view(-1).abs()).all()

@@ -29,8 +29,8 @@ template <typename T> __device__ __forceinline__ float as_float(T x) { return (f
 
 // The state entering each segment (REV: its gradient behind each segment) from what each segment adds: in place, one thread an element
 template <bool REV> __global__ __launch_bounds__(256) void td_decay_scan_kernel(Pass P) {
-    const int size = P.da * P.dc, blocks = (size + 255) / 256, el = blockIdx.x % blocks * 256 + threadIdx.x;
-    const int h = blockIdx.x / blocks % P.heads, n = blockIdx.x / blocks / P.heads;
+    const int size = P.da * P.dc, blocks = (size + 255) / 256, place = P.first + blockIdx.x, el = place % blocks * 256 + threadIdx.x;
+    const int h = place / blocks % P.heads, n = place / blocks / P.heads;
     int lo, hi;
     row_range(P.offsets, P.rows, n, lo, hi);
     const int segments = hi > lo ? (hi - lo - 1) / P.seg_len + 1 : 0;
@@ -96,13 +96,13 @@ template <typename T, int W, int NT>
 __global__ __launch_bounds__(NT) void td_decay_step_kernel(Pass P) {
     constexpr int GROUPS = NT / W;
     __shared__ float part[NT];
-    const int h = blockIdx.x % P.heads, n = blockIdx.x / P.heads, tid = threadIdx.x, col = tid % W, group = tid / W;
+    const int item = P.first + blockIdx.x, h = item % P.heads, n = item / P.heads, tid = threadIdx.x, col = tid % W, group = tid / W;
     const float g = expf(P.log_decay[h]);
     float sum = 0.0f;
     if (col < P.dc) {
         const T *a = base_of<T>(P.a, false, n, h), *b = base_of<T>(P.b, false, n, h);
         const float c = as_float<T>(base_of<T>(P.c, false, n, h)[col]);
-        float *S = P.state_out + (int64_t)blockIdx.x * P.da * P.dc + col;
+        float *S = P.state_out + (int64_t)item * P.da * P.dc + col;
 #pragma unroll 4
         for (int i = group; i < P.da; i += GROUPS) {
             const float s = g * S[(int64_t)i * P.dc] + as_float<T>(b[i]) * c;
@@ -115,15 +115,17 @@ __global__ __launch_bounds__(NT) void td_decay_step_kernel(Pass P) {
     if (group == 0 && col < P.dc) {
 #pragma unroll
         for (int k = 1; k < GROUPS; ++k) sum += part[tid + k * W];
-        ((T *)P.out)[(int64_t)blockIdx.x * P.dc + col] = (T)(sum * P.out_scale);
+        ((T *)P.out)[(int64_t)item * P.dc + col] = (T)(sum * P.out_scale);
     }
 }
 template <typename T, int NT> void launch_step(const Pass &P, hipStream_t st) {
-    const dim3 grid(P.n_seq * P.heads), block(NT);
-    if (NT == 256 && P.dc <= 16) hipLaunchKernelGGL((td_decay_step_kernel<T, 16, 256>), grid, block, 0, st, P);
-    else if (P.dc <= 32) hipLaunchKernelGGL((td_decay_step_kernel<T, 32, NT>), grid, block, 0, st, P);
-    else if (P.dc <= 64) hipLaunchKernelGGL((td_decay_step_kernel<T, 64, NT>), grid, block, 0, st, P);
-    else hipLaunchKernelGGL((td_decay_step_kernel<T, 128, NT>), grid, block, 0, st, P);
+    launch_parts(P, (int64_t)P.n_seq * P.heads, NT, [&](const Pass &P, dim3 grid) {
+        const dim3 block(NT);
+        if (NT == 256 && P.dc <= 16) hipLaunchKernelGGL((td_decay_step_kernel<T, 16, 256>), grid, block, 0, st, P);
+        else if (P.dc <= 32) hipLaunchKernelGGL((td_decay_step_kernel<T, 32, NT>), grid, block, 0, st, P);
+        else if (P.dc <= 64) hipLaunchKernelGGL((td_decay_step_kernel<T, 64, NT>), grid, block, 0, st, P);
+        else hipLaunchKernelGGL((td_decay_step_kernel<T, 128, NT>), grid, block, 0, st, P);
+    });
 }
 // Few states that are not small: 1024 threads for each, of which the chip holds 512 (64 x 8 states of 128 x 128: 14 us a call, 22 with 256 threads; 65 x 8
 // take 23 either way)
@@ -147,7 +149,7 @@ int check_config(const td_decay_config *c) {
                "q_heads, k_heads and v_heads must divide heads, got %d, %d, %d and %d", c->q_heads, c->k_heads, c->v_heads, c->heads);
     TD_REQUIRE(((int64_t)c->n_seq + c->rows / CHUNK) * c->heads * ((c->dk * c->dv + 255) / 256) < (1LL << 31) &&
                    (int64_t)c->n_seq * (c->rows / 256 + 1) * c->heads < (1LL << 31),
-               "too many sequences, rows and heads for one launch: n_seq %d, rows %d, heads %d", c->n_seq, c->rows, c->heads);
+               "too many sequences, rows and heads for one call: n_seq %d, rows %d, heads %d", c->n_seq, c->rows, c->heads);
     TD_REQUIRE((int64_t)c->heads * TD_DECAY_MAX_DIM * CHUNK * 4 < (1LL << 31), "heads must be below 65536, got %d", c->heads);
     return TD_OK;
 }
@@ -244,7 +246,7 @@ template <bool REV> int enter_states(const td_decay_config *c, const Pass &P, bo
     if (P.segs == 1) return TD_OK;
     if (int rc = launch(c, REV ? SUM_REVERSED : SUM, P, vec, st)) return rc;
     const int64_t blocks = (int64_t)P.n_seq * P.heads * ((P.da * P.dc + 255) / 256);
-    hipLaunchKernelGGL(td_decay_scan_kernel<REV>, dim3((unsigned)blocks), dim3(256), 0, st, P);
+    launch_parts(P, blocks, 256, [&](const Pass &P, dim3 grid) { hipLaunchKernelGGL(td_decay_scan_kernel<REV>, grid, dim3(256), 0, st, P); });
     TD_LAUNCH_CHECK();
     return TD_OK;
 }

@@ -41,8 +41,18 @@ struct Pass {
     int out_f32, out2_f32;
     int n_seq, rows, heads, da, dc;
     int seg_len, segs, slots; // rows of a segment (a multiple of CHUNK), segments of a dense sequence (1: seg_len covers all), slots in all
+    int first;                // workgroup 0's place among all of them (launch_parts)
     float out_scale, upd_scale;
 };
+
+// HIP launches fewer than 2^32 threads at once: `groups` workgroups in as many launches as that takes
+template <typename L> void launch_parts(Pass P, int64_t groups, int threads, L launch) {
+    const int64_t most = 0xFFFFFFFFll / threads;
+    for (int64_t at = 0; at < groups; at += most) {
+        P.first = (int)at;
+        launch(P, dim3((unsigned)(groups - at < most ? groups - at : most)));
+    }
+}
 
 // What a launcher takes.  Backward: p ascending, r descending, `groups` workgroups that share out the slots and heads
 struct Work {
@@ -610,7 +620,7 @@ template <typename T, int DA, int DC, int NW, bool VEC, bool REV, int WAVES> __g
     __shared__ __align__(16) T lb[CHUNK * X::PA];
     __shared__ __align__(16) T lc[CHUNK * X::PC];
     const int tid_ = here(threadIdx.x), tid = tid_, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = (tid & 63) >> 4, li = tid & 15;
-    const int h = blockIdx.x % P.heads, slot = blockIdx.x / P.heads;
+    const int item = P.first + blockIdx.x, h = item % P.heads, slot = item / P.heads;
     Place at;
     if (!at.find(P, slot) || (REV ? at.segment == 0 : at.last)) return;      // nothing enters a segment from these
     const T *pb = base_of<T>(P.b, P.offsets, at.n_seq, h) + (int64_t)at.lo * P.b.row, *pc = base_of<T>(P.c, P.offsets, at.n_seq, h) + (int64_t)at.lo * P.c.row;
@@ -648,7 +658,7 @@ template <typename T, int DA, int DC, int NW, bool VEC, bool REV, int WAVES> __g
         const int t = REV ? at.t0 + (whole - 1 - c) * CHUNK : at.t0 + c * CHUNK;
         chunk(Whole(), t, CHUNK, c + 1 < whole ? Next{REV ? t - CHUNK : t + CHUNK, CHUNK} : Next{t, 1});
     }
-    x.leave(P.seg + (int64_t)blockIdx.x * P.da * P.dc, P.st_a, P.st_c, P.da, P.dc, wave, g, li);
+    x.leave(P.seg + (int64_t)item * P.da * P.dc, P.st_a, P.st_c, P.da, P.dc, wave, g, li);
 }
 
 // out from (a, b, c), rows ascending.  SLOPE: the part of the derivative by log g that rows owe to the states entering their chunks, dotted with
@@ -747,7 +757,7 @@ __device__ __forceinline__ void out_sweep(const Pass &P, int item, OutLds<T, DA,
 
 template <typename T, int DA, int DC, int NW, bool VEC, int WAVES> __global__ __launch_bounds__(64 * NW, WAVES) void td_decay_out_kernel(Pass P) {
     __shared__ __align__(16) OutLds<T, DA, DC, NW, false> lds;
-    out_sweep<T, DA, DC, NW, 1, VEC, false>(P, blockIdx.x, lds, nullptr);
+    out_sweep<T, DA, DC, NW, 1, VEC, false>(P, P.first + blockIdx.x, lds, nullptr);
 }
 
 // out from (a, b, c) and out2 from (e, c, b), rows descending: the gradients of v and k from (k, q, grad_o) and (v, grad_o, q).  SLOPE: the rest of
@@ -966,7 +976,7 @@ __global__ __launch_bounds__(64 * NW * TEAMS, WAVES) void td_decay_backward_kern
         PairLds<T, DK, DV, NW> pair;
     } lds;
     float *mine = chunk_states + blockIdx.x * held;
-    for (int item = blockIdx.x; item < Q.slots * Q.heads; item += gridDim.x) {
+    for (unsigned item = blockIdx.x; item < (unsigned)(Q.slots * Q.heads); item += gridDim.x) {
         if (ascending) out_sweep<T, DV, DK, NW, TEAMS, VEC, SLOPE>(argument<Pass>(0), item, lds.out, mine);
         __syncthreads();
         if (descending) pair_sweep<T, DK, DV, NW, TEAMS, VEC, SLOPE>(argument<Pass>(sizeof(Pass)), item, lds.pair, mine);

@@ -26,13 +26,14 @@ typedef float T;
 template <bool VEC, int DA, int DC> int launch(const Work &w, hipStream_t st) {
     constexpr int size = DA + DC, NW = TD_INST_KIND == 0 && TD_INST_BF16 && size == 256 ? 4 : (TD_INST_KIND < 3 ? DC : DA < DC ? DA : DC) / 16;
     const Pass &P = w.p;
-    const dim3 grid((unsigned)(P.slots * P.heads)), block(64 * NW);
+#if TD_INST_KIND < 3
+    launch_parts(P, (int64_t)P.slots * P.heads, 64 * NW, [&](const Pass &P, dim3 grid) {
 #if TD_INST_KIND == 0
-    hipLaunchKernelGGL((td_decay_out_kernel<T, DA, DC, NW, VEC, size <= 128 ? 3 : TD_INST_BF16 && size < 256 && DC == 128 ? 4 : 2>), grid, block, 0, st, P);
-#elif TD_INST_KIND == 1
-    hipLaunchKernelGGL((td_decay_sum_kernel<T, DA, DC, NW, VEC, false, 4>), grid, block, 0, st, P);
-#elif TD_INST_KIND == 2
-    hipLaunchKernelGGL((td_decay_sum_kernel<T, DA, DC, NW, VEC, true, 4>), grid, block, 0, st, P);
+        hipLaunchKernelGGL((td_decay_out_kernel<T, DA, DC, NW, VEC, size <= 128 ? 3 : TD_INST_BF16 && size < 256 && DC == 128 ? 4 : 2>), grid, dim3(64 * NW), 0, st, P);
+#else
+        hipLaunchKernelGGL((td_decay_sum_kernel<T, DA, DC, NW, VEC, TD_INST_KIND == 2, 4>), grid, dim3(64 * NW), 0, st, P);
+#endif
+    });
 #else
     const int64_t held = (int64_t)((P.seg_len + CHUNK - 1) / CHUNK) * DA * DC;
     constexpr int TEAMS = NW == 4 && (!TD_INST_BF16 || size > 128) ? 2 : 1;
