@@ -423,7 +423,7 @@ typedef struct td_adamw_config {
     int32_t reserved;
 } td_adamw_config;
 
-/* `tensors_host`: `count` records in host memory, read during the call.  One launch for every 48 tensors. */
+/* `tensors_host`: `count` records in host memory, read during the call.  One launch for every 48 tensors, or 2^34 values. */
 TD_API int td_adamw(const td_adamw_config *cfg, const td_adamw_tensor *tensors_host, int32_t count, void *stream);
 /* The record of (lr, betas, weight_decay, step, seed) of cfg, computed as td_adamw computes its own values and written by a
  * one-thread kernel (stream-ordered). */

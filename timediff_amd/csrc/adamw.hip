@@ -11,11 +11,13 @@ namespace {
 
 constexpr int MAX_TENSORS = 48;      // records of one launch: 48 x 64 bytes of the 4 KiB of kernel arguments
 constexpr int WAVES = 4;             // blocks of 256 values that a workgroup takes
+constexpr int64_t MAX_GROUPS = 0xFFFFFFFFll / (64 * WAVES);      // HIP launches fewer than 2^32 threads at once
 
 struct Batch {
     td_adamw_tensor t[MAX_TENSORS];  // .reserved: 1 where every pointer is aligned for four values at once
     int first[MAX_TENSORS + 1];      // workgroups before each tensor's own
     int count, position;             // records here; place of the first one in the caller's list
+    int done;                        // workgroups of the first record that an earlier launch had
     float beta1, beta2, omb1, omb2, eps, step_size, inv_sqrt_bc2, decay;
     uint64_t seed;
     uint32_t step;
@@ -222,7 +224,7 @@ template <int BITS> __global__ __launch_bounds__(64 * WAVES) void td_adamw_kerne
     Scalars s{B.step_size, B.inv_sqrt_bc2, B.decay, B.seed, B.step};
     if (B.rec) s = Scalars{B.rec->step_size, B.rec->inv_sqrt_bc2, B.rec->decay, B.rec->seed, (uint32_t)B.rec->step};
     const float gs = B.grad_scale ? B.grad_scale[0] : 1.0f;
-    const int64_t block = (int64_t)(blockIdx.x - B.first[lo]) * WAVES + threadIdx.x / 64;
+    const int64_t block = (int64_t)(blockIdx.x - B.first[lo] + (lo == 0 ? B.done : 0)) * WAVES + threadIdx.x / 64;
     if (block * TD_ADAMW_BLOCK < t.n) step_block<BITS>(B, s, t, B.position + lo, block, threadIdx.x % 64, gs);
 }
 
@@ -257,6 +259,7 @@ extern "C" int td_adamw(const td_adamw_config *cfg, const td_adamw_tensor *tenso
     for (int i = 0; i < count; ++i) {
         const td_adamw_tensor &t = tensors_host[i];
         TD_REQUIRE(t.n >= 0, "tensor %d: bad size", i);
+        TD_REQUIRE(t.n < (1LL << 40), "tensor %d: too large", i);
         TD_REQUIRE(t.n == 0 || (t.param && t.grad && t.exp_avg && t.exp_avg_sq), "tensor %d: null pointer", i);
         TD_REQUIRE(t.grad_dtype == TD_F32 || t.grad_dtype == TD_BF16, "tensor %d: gradients must be TD_F32 or TD_BF16, got %d", i, t.grad_dtype);
         TD_REQUIRE(t.n == 0 || cfg->state_bits == 32 || t.scales, "tensor %d: 8-bit moments need scales", i);
@@ -266,18 +269,23 @@ extern "C" int td_adamw(const td_adamw_config *cfg, const td_adamw_tensor *tenso
     B.eps = (float)cfg->eps;
     step_values(cfg, B.step_size, B.inv_sqrt_bc2, B.decay);
     B.seed = cfg->seed; B.step = (uint32_t)cfg->step; B.grad_scale = cfg->grad_scale; B.rec = cfg->record;
+    B.done = 0;
     for (int i = 0; i < count;) {
         int64_t groups = 0;
+        int left_off = 0;
         B.position = i;
         B.count = 0;
-        while (i < count && B.count < MAX_TENSORS) {
+        while (i < count && B.count < MAX_TENSORS && groups < MAX_GROUPS) {
             const td_adamw_tensor &t = tensors_host[i];
-            const int64_t mine = (t.n + TD_ADAMW_BLOCK * WAVES - 1) / (TD_ADAMW_BLOCK * WAVES);
-            TD_REQUIRE(mine < (1 << 30), "tensor %d: too large", i);
-            if (groups + mine >= (1LL << 31) - 1) break;
+            const int64_t done = B.count == 0 ? B.done : 0, mine = (t.n + TD_ADAMW_BLOCK * WAVES - 1) / (TD_ADAMW_BLOCK * WAVES) - done;
             B.t[B.count] = t;
             B.t[B.count].reserved = aligned(t, cfg->state_bits);
             B.first[B.count++] = (int)groups;
+            if (groups + mine > MAX_GROUPS) {          // the next launch goes on inside this tensor
+                left_off = (int)(done + MAX_GROUPS - groups);
+                groups = MAX_GROUPS;
+                break;
+            }
             groups += mine;
             ++i;
         }
@@ -285,6 +293,7 @@ extern "C" int td_adamw(const td_adamw_config *cfg, const td_adamw_tensor *tenso
         if (cfg->state_bits == 32) hipLaunchKernelGGL(td_adamw_kernel<32>, dim3((unsigned)groups), dim3(64 * WAVES), 0, (hipStream_t)stream, B);
         else hipLaunchKernelGGL(td_adamw_kernel<8>, dim3((unsigned)groups), dim3(64 * WAVES), 0, (hipStream_t)stream, B);
         TD_LAUNCH_CHECK();
+        B.done = left_off;
     }
     return TD_OK;
 }
