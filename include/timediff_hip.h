@@ -360,8 +360,11 @@ typedef struct td_decay_config {
                                                                         dimension of every tensor is contiguous */
 } td_decay_config;
 
-/* Scratch of one forward (backward = 0) or backward (1) call; 0 with td_last_error() set for a bad configuration.  A forward call
- * that asks for 256 uses none and takes NULL. */
+/* Which gradients a backward call takes: all of them, or TD_DECAY_GRAD_SOME with those of q, k, v and log_decay that are not NULL (that of the
+ * entering state needs no memory). */
+enum { TD_DECAY_GRAD_ALL = 1, TD_DECAY_GRAD_SOME = 2, TD_DECAY_GRAD_Q = 4, TD_DECAY_GRAD_K = 8, TD_DECAY_GRAD_V = 16, TD_DECAY_GRAD_LOG_DECAY = 32 };
+/* Scratch of one forward (backward = 0) or backward (as above) call; 0 with td_last_error() set for a bad configuration.  A call that
+ * asks for 256 uses none and takes NULL. */
 TD_API size_t td_decay_workspace_bytes(const td_decay_config *cfg, int32_t backward);
 /* o: (.., rows, heads, dv) contiguous; state_in, state_out: (n_seq, heads, dk, dv) float32 or NULL (not the same memory). */
 TD_API int td_decay_forward(const td_decay_config *cfg, const void *q, const void *k, const void *v, const float *log_decay,

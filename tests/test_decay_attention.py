@@ -110,3 +110,21 @@ def test_rows_are_counted_in_32_bits():
         assert L.td_decay_workspace_bytes(C.byref(cfg), 0) > 0 and L.td_decay_workspace_bytes(C.byref(cfg), 1) > 0
     cfg.rows += 1
     assert L.td_decay_workspace_bytes(C.byref(cfg), 0) == 0 and b"rows must be" in L.td_last_error()
+
+
+def test_workspace_is_for_the_gradients_wanted():
+    """Fixed decays keep no chunk states (40 packed sequences of 131072 rows in all, 16 heads of 128 x 128: 4 GiB); shared heads have parts in float32
+    for the gradients that are asked for."""
+    L = _lib.lib()
+    cfg = _lib.DecayConfig(n_seq=40, rows=131072, heads=16, q_heads=16, k_heads=16, v_heads=16, dk=128, dv=128, dtype=_lib.BF16, packed=1, scale=1.0)
+    need = lambda b: L.td_decay_workspace_bytes(C.byref(cfg), b)  # noqa: E731
+    S, Q, K, V, D = _lib.DECAY_GRAD_SOME, _lib.DECAY_GRAD_Q, _lib.DECAY_GRAD_K, _lib.DECAY_GRAD_V, _lib.DECAY_GRAD_LOG_DECAY
+    every = need(_lib.DECAY_GRAD_ALL)
+    assert every == need(S | Q | K | V | D) == need(S | D) > 4 * 2 ** 30
+    state = 16 * 128 * 128 * 4
+    assert need(S) == need(S | Q | K | V) <= 2 * (131072 // 4096 + 40) * state + 2048
+    cfg.k_heads = cfg.v_heads = 4
+    part = 131072 * 16 * 128 * 4
+    assert need(S | Q) == need(S) and need(S | K) == need(S | V) == need(S) + part and need(S | K | V) == need(S) + 2 * part
+    for bad in (3, 4, 64, 66, -1):
+        assert need(bad) == 0 and b"backward must be" in L.td_last_error()

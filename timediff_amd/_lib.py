@@ -25,6 +25,7 @@ PROFILE_LAYER_INFER, PROFILE_LAYER_SAVE, PROFILE_BPTT_SWEEP = 1, 2, 4     # td_p
 HEAD_FUSION_AUTO, HEAD_FUSION_OFF, HEAD_FUSION_ON = 0, 1, 2             # td_set_head_fusion
 F32, BF16 = 0, 1                                                         # element types (td_decay_config.dtype, td_adamw_tensor.grad_dtype)
 DECAY_MAX_DIM, ADAMW_BLOCK = 128, 256
+DECAY_GRAD_ALL, DECAY_GRAD_SOME, DECAY_GRAD_Q, DECAY_GRAD_K, DECAY_GRAD_V, DECAY_GRAD_LOG_DECAY = 1, 2, 4, 8, 16, 32      # td_decay_workspace_bytes
 STEP_LAUNCH_AUTO, STEP_LAUNCH_OFF, STEP_LAUNCH_ON = 0, 1, 2             # td_set_step_launch
 
 

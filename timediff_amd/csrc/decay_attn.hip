@@ -179,8 +179,8 @@ bool wide(const td_decay_config *c, const View &v) {
 //   * with a workgroup for three in four compute units nothing is cut: 256 of 1024 rows, 128 x 128, take 85 / 379 us whole and 146 / 590
 //     cut for 512.  States of 32 x 32 have less to do between their loads and gain up to 512: 256 of 2048 rows 77 / 207 us
 //     cut, about 95 / 276 whole.  Lengths of packed sequences are not known here: one of them may be nearly all rows;
-//   * the backward pass keeps the states entering a segment's chunks (64 KB a chunk of 128 x 128), so its segments are 4096 rows
-//     at most: 2 GB in all 512 workgroups, where a sequence of 32768 rows in one piece would take 17 GB.
+//   * the backward pass of log_decay keeps the states entering a segment's chunks (64 KB a chunk of 128 x 128), so its segments are 4096
+//     rows at most: 2 GiB in 512 workgroups (4 in 1024), where a sequence of 32768 rows in one piece would take 16.
 void split(const td_decay_config *c, bool backward, int &len, int &segs, int64_t &slots) {
     const int64_t rows = total_rows(c), longest = c->rows;
     const int most = c->dk > c->dv ? c->dk : c->dv;
@@ -265,8 +265,10 @@ int share_sum(const td_decay_config *c, const float *parts, void *grad, int own_
 }
 
 constexpr size_t NO_WORKSPACE = 256;      // what a call that uses none asks for: 0 says that the configuration is bad
-struct Layout { size_t seg, seg2, chunks, slope, parts, parts2, total; };
-Layout layout(const td_decay_config *c, bool backward) {
+struct Layout { size_t seg, seg2, chunks, slope, parts, parts2, parts3, total; };
+// want: the `backward` of td_decay_workspace_bytes
+Layout layout(const td_decay_config *c, int want) {
+    const bool backward = want != 0, all = want == TD_DECAY_GRAD_ALL, slope = backward && (all || want & TD_DECAY_GRAD_LOG_DECAY);
     int len, segs;
     int64_t slots;
     split(c, backward, len, segs, slots);
@@ -277,11 +279,12 @@ Layout layout(const td_decay_config *c, bool backward) {
     w.seg = 0;
     w.seg2 = segs == 1 ? 0 : up256(slots * state);
     w.chunks = w.seg2 + (backward && segs != 1 ? up256(slots * state) : 0);
-    w.slope = w.chunks + (backward ? held * backward_groups(c, slots) : 0);
-    w.parts = w.slope + (backward ? up256(2 * (size_t)slots * c->heads * sizeof(double)) : 0);
-    const bool q = c->q_heads != c->heads, k = c->k_heads != c->heads, v = c->v_heads != c->heads;
-    w.parts2 = w.parts + (backward && q ? up256(rows * c->dk) : 0);
-    w.total = w.parts2 + (backward ? (k ? up256(rows * c->dk) : 0) + (v ? up256(rows * c->dv) : 0) : 0) + NO_WORKSPACE;
+    w.slope = w.chunks + (slope ? held * backward_groups(c, slots) : 0);
+    w.parts = w.slope + (slope ? up256(2 * (size_t)slots * c->heads * sizeof(double)) : 0);
+    const auto part = [&](int bit, int own, int d) { return backward && (all || want & bit) && own != c->heads ? up256(rows * d) : 0; };
+    w.parts2 = w.parts + part(TD_DECAY_GRAD_Q, c->q_heads, c->dk);
+    w.parts3 = w.parts2 + part(TD_DECAY_GRAD_K, c->k_heads, c->dk);
+    w.total = w.parts3 + part(TD_DECAY_GRAD_V, c->v_heads, c->dv) + NO_WORKSPACE;
     return w;
 }
 
@@ -291,13 +294,18 @@ bool aligned(const void *p) { return (uintptr_t)p % 16 == 0; }
 
 extern "C" size_t td_decay_workspace_bytes(const td_decay_config *cfg, int32_t backward) {
     if (check_config(cfg) != TD_OK) return 0;
-    return layout(cfg, backward != 0).total;
+    constexpr int known = TD_DECAY_GRAD_ALL | TD_DECAY_GRAD_SOME | TD_DECAY_GRAD_Q | TD_DECAY_GRAD_K | TD_DECAY_GRAD_V | TD_DECAY_GRAD_LOG_DECAY;
+    if (backward & ~known || (backward & ~TD_DECAY_GRAD_ALL && (backward & TD_DECAY_GRAD_ALL || !(backward & TD_DECAY_GRAD_SOME)))) {
+        td_set_error("backward must be 0, TD_DECAY_GRAD_ALL or TD_DECAY_GRAD_SOME with others, got %d", backward);
+        return 0;
+    }
+    return layout(cfg, backward).total;
 }
 
 extern "C" int td_decay_forward(const td_decay_config *cfg, const void *q, const void *k, const void *v, const float *log_decay,
                                 const int32_t *offsets, const float *state_in, void *o, float *state_out, void *workspace, void *stream) {
     if (int rc = check_config(cfg)) return rc;
-    TD_REQUIRE(log_decay && (workspace || layout(cfg, false).total == NO_WORKSPACE) && (cfg->rows == 0 || (q && k && v && o)), "null pointer");
+    TD_REQUIRE(log_decay && (workspace || layout(cfg, 0).total == NO_WORKSPACE) && (cfg->rows == 0 || (q && k && v && o)), "null pointer");
     TD_REQUIRE(!cfg->packed || offsets, "packed sequences need offsets");
     TD_REQUIRE(!state_out || state_out != state_in, "state_in and state_out must not be the same memory");
     hipStream_t st = (hipStream_t)stream;
@@ -318,18 +326,18 @@ extern "C" int td_decay_backward(const td_decay_config *cfg, const void *q, cons
                                  const int32_t *offsets, const float *state_in, const void *grad_o, const float *grad_state_out, void *grad_q,
                                  void *grad_k, void *grad_v, float *grad_log_decay, float *grad_state_in, void *workspace, void *stream) {
     if (int rc = check_config(cfg)) return rc;
-    TD_REQUIRE(log_decay && workspace && (cfg->rows == 0 || (q && k && v && grad_o)), "null pointer");
+    const bool slope = grad_log_decay != nullptr;
+    const Layout l = layout(cfg, TD_DECAY_GRAD_SOME | (grad_q ? TD_DECAY_GRAD_Q : 0) | (grad_k ? TD_DECAY_GRAD_K : 0) | (grad_v ? TD_DECAY_GRAD_V : 0) |
+                                     (slope ? TD_DECAY_GRAD_LOG_DECAY : 0));
+    TD_REQUIRE(log_decay && (workspace || l.total == NO_WORKSPACE) && (cfg->rows == 0 || (q && k && v && grad_o)), "null pointer");
     TD_REQUIRE(!cfg->packed || offsets, "packed sequences need offsets");
     hipStream_t st = (hipStream_t)stream;
-    const Layout l = layout(cfg, true);
     char *ws = (char *)workspace;
     const bool q_shared = cfg->q_heads != cfg->heads, k_shared = cfg->k_heads != cfg->heads, v_shared = cfg->v_heads != cfg->heads;
-    float *parts_q = (float *)(ws + l.parts), *parts_k = (float *)(ws + l.parts2);
-    float *parts_v = (float *)(ws + l.parts2 + (k_shared ? up256((size_t)total_rows(cfg) * cfg->heads * cfg->dk * sizeof(float)) : 0));
+    float *parts_q = (float *)(ws + l.parts), *parts_k = (float *)(ws + l.parts2), *parts_v = (float *)(ws + l.parts3);
     const View vq = view(cfg, q, cfg->q_stride, cfg->q_heads, cfg->dk), vk = view(cfg, k, cfg->k_stride, cfg->k_heads, cfg->dk),
                vv = view(cfg, v, cfg->v_stride, cfg->v_heads, cfg->dv), vo = view(cfg, grad_o, cfg->grad_o_stride, cfg->heads, cfg->dv);
     const bool vec = wide(cfg, vq) && wide(cfg, vk) && wide(cfg, vv) && wide(cfg, vo) && aligned(grad_q) && aligned(grad_k) && aligned(grad_v);
-    const bool slope = grad_log_decay != nullptr;
     Work w = {};
     w.chunk_states = (float *)(ws + l.chunks);
     w.ascending = grad_q || slope;

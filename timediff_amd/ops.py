@@ -337,6 +337,7 @@ class SamplerKernels:
 # -- decay attention (timediff_amd/decay_attention.py is the differentiable front) ------------------------------------------
 _ELEMENT = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
 _DECAY_FIELDS = struct.Struct("<10ifi12q")      # td_decay_config, packed in one call: these calls are as short as their launches
+_GRADS = (_lib.DECAY_GRAD_Q, _lib.DECAY_GRAD_K, _lib.DECAY_GRAD_V, _lib.DECAY_GRAD_LOG_DECAY)
 _NO_WORKSPACE = 256                             # td_decay_workspace_bytes of a call that uses none
 
 
@@ -455,7 +456,7 @@ def decay_backward(q, k, v, log_decay, scale, grad_o, offsets=None, state=None, 
         offsets = None if offsets is None else offsets.contiguous()
         grad_state = None if grad_state is None else grad_state.to(torch.float32).contiguous()
         cfg = _decay_config(q, k, v, log_decay, scale, offsets, grad_o)
-        ws = _decay_workspace(cfg, 1, device)
+        ws = _decay_workspace(cfg, _lib.DECAY_GRAD_SOME + sum(b for b, w in zip(_GRADS, want) if w), device)
         check(lib().td_decay_backward(cfg, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), _address(offsets), _address(state),
                                       grad_o.data_ptr(), _address(grad_state), *map(_address, new), _address(d_state), _address(ws), _raw_stream(index)))
     return (*new, d_state)
