@@ -46,3 +46,32 @@ def test_more_workgroups_than_one_launch_takes(dev):
             o, state = decay_attention(*(t[:, None] for t in (q, k, v)), ld, scale=0.5, initial_state=S, return_state=True)
         assert ((state.view(-1).double() - new).abs() <= 10 * 2.0 ** -24 * size).all()
         assert ((o.view(-1).double() - want).abs() <= 2.0 ** -8 * want.abs() + 20 * 2.0 ** -24 * size * q.double().view(-1).abs()).all()
+
+
+@pytest.mark.parametrize("B, T, H", [(1, 70, 1), (3, 100, 2), (9, 300, 4)])
+def test_odd_addresses_with_even_strides(B, T, H, dev):
+    """Strides that suit 16-byte reads and addresses that do not: the backward pass takes a kernel with a wider state than the workspace counts a
+    place for, so fewer places (one at least).  The same results as from aligned tensors: sums of up to T D products in another order, 2^-24
+    each of the sums of magnitudes on both sides, and a bfloat16 step where that crosses a border."""
+    import decay_reference as ref
+    from timediff_amd.decay_attention import decay_attention
+    Dk, Dv = 8, 72
+    g = torch.Generator().manual_seed(T)
+    x = [torch.randn(B, T, H, d, generator=g).to(BF16) for d in (Dk, Dk, Dv, Dv)]
+    ld = -torch.exp(torch.rand(H, generator=g) * 6 - 6)
+
+    def odd(t):
+        flat = torch.empty(t.numel() + 1, dtype=t.dtype, device=dev)
+        flat[1:] = t.to(dev).view(-1)
+        return flat[1:].view(t.shape)
+    res = []
+    for f in (lambda t: t.to(dev), odd):
+        leaf = [f(t).requires_grad_() for t in x[:3]] + [ld.to(dev).requires_grad_()]
+        o = decay_attention(*leaf)
+        res.append([o.detach(), *torch.autograd.grad(o, leaf, f(x[3]))])
+    size = ref.gradients(*(t.abs() for t in x[:3]), ld, x[3].abs())
+    size["o"] = ref.decay_attention(*(t.abs() for t in x[:3]), ld)[0]
+    for n, a, b in zip(("o", "q", "k", "v", "log_decay"), *res):
+        terms = T * (B if n == "log_decay" else 1) + T + Dv + 32
+        a, b = a.cpu().double(), b.cpu().double()
+        assert ((a - b).abs() <= (2.0 ** -7 if n != "log_decay" else 2.0 ** -23) * a.abs() + 2 * terms * 2.0 ** -24 * size[n]).all(), n
