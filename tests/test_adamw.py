@@ -89,3 +89,12 @@ def test_library_refuses_bad_tensors():
         assert L.td_adamw(C.byref(cfg), C.byref(t), 1, None) == 1 and text in L.td_last_error(), bad
     assert L.td_adamw(C.byref(cfg), None, 1, None) == 1
     assert L.td_adamw_record_set(None, C.byref(cfg), None) == 1
+
+
+@pytest.mark.parametrize("record", [torch.zeros(8), torch.zeros(31, dtype=torch.uint8), torch.zeros(64, dtype=torch.uint8)[::2], torch.zeros(40, dtype=torch.uint8)[1:33]])
+def test_records_that_are_none(record):
+    """A kernel would read a td_adamw_record there."""
+    with pytest.raises(ValueError, match="record must be the 32 bytes"):
+        adamw_(**_lists(), **HYPER, record=record)
+    with pytest.raises(ValueError, match="ROCm device"):
+        adamw_(**_lists(), **HYPER, record=torch.zeros(32, dtype=torch.uint8))

@@ -380,3 +380,11 @@ def test_written_params_are_noticed(dev):
         p = torch.ones(300, device=dev)
         adamw_([p, w], [torch.ones(300, device=dev) for _ in range(2)], *([torch.zeros(300, device=dev) for _ in range(2)] for _ in range(2)), **kw)
     assert (p < 1).all()
+
+
+def test_record_of_another_device(dev):
+    """A record in host memory would be read by the kernel: refused."""
+    from timediff_amd.optim import adamw_
+    x = _lists(1, dev, [300])
+    with pytest.raises(ValueError, match="record must be on the params' device"):
+        adamw_(**x, **HYPER, record=torch.zeros(32, dtype=torch.uint8))

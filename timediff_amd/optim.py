@@ -43,6 +43,8 @@ def adamw_(params, grads, exp_avgs, exp_avg_sqs, scales=None, *, lr, betas, eps,
             lists.append(("random", random, _WORDS, n))
     elif random is not None:
         raise ValueError("random is for 8-bit moments")
+    if record is not None and (record.dtype is not torch.uint8 or not record.is_contiguous() or record.numel() != C.sizeof(AdamwRecord) or record.data_ptr() % 8):
+        raise ValueError(f"record must be the {C.sizeof(AdamwRecord)} bytes of a td_adamw_record (uint8, at a multiple of 8)")
     for name, tensors, dtypes, sizes in lists:
         if len(tensors) != len(n):
             raise ValueError(f"{len(tensors)} {name} for {len(n)} params")
@@ -66,6 +68,8 @@ def adamw_(params, grads, exp_avgs, exp_avg_sqs, scales=None, *, lr, betas, eps,
             raise ValueError(f"{name} must be on one ROCm device, the params'")
     if grad_scale is not None and (grad_scale.dtype is not torch.float32 or grad_scale.numel() != 1 or grad_scale.get_device() != index):
         raise ValueError("grad_scale must be one float32 value on the params' device")
+    if record is not None and record.get_device() != index:
+        raise ValueError("record must be on the params' device")
     table[6::8] = array.array("q", n)
     if set(map(_DTYPE, grads)) != _F32:
         table[7::8] = array.array("q", [_lib.F32 if g.dtype is torch.float32 else _lib.BF16 for g in grads])
