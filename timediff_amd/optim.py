@@ -157,17 +157,17 @@ class AdamW(torch.optim.Optimizer):
             for p in live:
                 if p.grad.is_sparse:
                     raise RuntimeError("sparse gradients are not supported")
-            if not self.capturable:
-                for p in live:
-                    self._state(p)["step"] += 1
-            for step in sorted({self.state[p]["step"] for p in live}):
-                ps = [p for p in live if self.state[p]["step"] == step]
+            count = 0 if self.capturable else 1              # advance() has counted
+            for step in sorted({self._state(p)["step"] + count for p in live}):
+                ps = [p for p in live if self.state[p]["step"] + count == step]
                 st = [self.state[p] for p in ps]
                 cfg = self._config(i, step)
                 adamw_(ps, [p.grad.contiguous() for p in ps], [s["exp_avg"] for s in st], [s["exp_avg_sq"] for s in st],
                        [s["scales"] for s in st] if self.state_bits == 8 else None, lr=cfg.lr, betas=(cfg.beta1, cfg.beta2), eps=cfg.eps,
                        weight_decay=cfg.weight_decay, step=step, grad_scale=grad_scale, seed=cfg.seed,
                        record=self._records.get(i))
+                for s in st:
+                    s["step"] = step
         return loss
 
     def load_state_dict(self, state_dict):
