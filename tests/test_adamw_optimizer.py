@@ -39,3 +39,14 @@ def test_a_refused_step_is_not_counted(calls):
     opt.step()
     opt.step()
     assert [c[1] for c in calls] == [1, 2] and opt.state[ps[0]]["step"] == 2
+
+
+def test_params_at_neighbouring_steps(calls):
+    """A param one step behind another is stepped once."""
+    ps = _params(2)
+    opt = AdamW(ps)
+    ps[0].grad = torch.zeros(4)
+    opt.step()
+    ps[1].grad = torch.zeros(4)
+    opt.step()
+    assert [c[:2] for c in calls] == [([id(ps[0])], 1), ([id(ps[1])], 1), ([id(ps[0])], 2)]

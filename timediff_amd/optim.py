@@ -158,8 +158,10 @@ class AdamW(torch.optim.Optimizer):
                 if p.grad.is_sparse:
                     raise RuntimeError("sparse gradients are not supported")
             count = 0 if self.capturable else 1              # advance() has counted
-            for step in sorted({self._state(p)["step"] + count for p in live}):
-                ps = [p for p in live if self.state[p]["step"] + count == step]
+            at = {}
+            for p in live:
+                at.setdefault(self._state(p)["step"] + count, []).append(p)
+            for step, ps in sorted(at.items()):
                 st = [self.state[p] for p in ps]
                 cfg = self._config(i, step)
                 adamw_(ps, [p.grad.contiguous() for p in ps], [s["exp_avg"] for s in st], [s["exp_avg_sq"] for s in st],
