@@ -19,7 +19,13 @@ class Calls(list):
 @pytest.fixture
 def calls(monkeypatch):
     got = Calls()
+    got.records = []
+
+    def record(self, i, step):
+        self._records.setdefault(i, object())
+        got.records.append((i, step))
     monkeypatch.setattr(optim, "adamw_", got.adamw_)
+    monkeypatch.setattr(AdamW, "_record", record)
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: got.capturing)
     return got
 
@@ -50,3 +56,64 @@ def test_params_at_neighbouring_steps(calls):
     ps[1].grad = torch.zeros(4)
     opt.step()
     assert [c[:2] for c in calls] == [([id(ps[0])], 1), ([id(ps[1])], 1), ([id(ps[0])], 2)]
+
+
+@pytest.mark.parametrize("capturable", [False, True])
+def test_late_and_missing_gradients(capturable, calls):
+    """A param counts the steps that it takes part in, as torch.optim.AdamW's does, with capturable and without."""
+    ps = _params(3)
+    theirs = _params(3)
+    a, b = AdamW(ps, capturable=capturable), torch.optim.AdamW(theirs)
+    for step in range(6):
+        for i, (p, q) in enumerate(zip(ps, theirs)):
+            live = not (i == 1 and step < 3) and not (i == 2 and step % 2)
+            p.grad, q.grad = (torch.zeros(4), torch.zeros(4)) if live else (None, None)
+        a.step()
+        b.step()
+        for p, q in zip(ps, theirs):
+            assert a.state[p].get("step", 0) == (b.state[q]["step"].item() if b.state[q] else 0)
+    assert not any(c[3] for c in calls)                       # an eager step takes its numbers from the host
+
+
+def test_captured_steps_are_counted_for_their_params(calls):
+    """Two groups; one param never has a gradient.  An advance() with no gradient about counts them all, and the capture takes back what it does not
+    step; afterwards advance() counts the captured ones."""
+    ps = _params(4)
+    opt = AdamW([dict(params=ps[:2]), dict(params=ps[2:])], capturable=True)
+    steps = lambda: [opt.state[p]["step"] for p in ps]  # noqa: E731
+    opt.advance()
+    assert steps() == [1, 1, 1, 1] and calls.records == [(0, 1), (1, 1)]
+    for p in ps[:3]:
+        p.grad = torch.zeros(4)
+    calls.capturing = True
+    opt.step()
+    calls.capturing = False
+    assert steps() == [1, 1, 1, 0] and [c[1:2] + c[3:] for c in calls] == [(1, True), (1, True)]
+    ps[3].grad = torch.zeros(4)
+    opt.advance()
+    opt.advance()
+    assert steps() == [3, 3, 3, 0] and calls.records[-2:] == [(0, 3), (1, 3)]
+    opt.step()                                                # eager: each at its own step
+    assert steps() == [4, 4, 4, 1] and [c[1] for c in calls[-3:]] == [4, 1, 4] and not calls[-1][3]
+    calls.capturing = True
+    with pytest.raises(RuntimeError, match="must be at the same step, group 1 has \\[1, 4\\]"):
+        opt.step()
+    calls.capturing = False
+    opt.advance()                                             # the graph captured before goes on
+    assert steps() == [5, 5, 5, 1]
+
+
+def test_captures_that_are_refused(calls):
+    ps = _params(2)
+    opt = AdamW(ps[:1], capturable=True)
+    ps[0].grad, ps[1].grad = torch.zeros(4), torch.zeros(4)
+    calls.capturing = True
+    with pytest.raises(RuntimeError, match="one step\\(\\) or advance\\(\\) before the capture"):
+        opt.step()
+    calls.capturing = False
+    opt.step()
+    opt.add_param_group(dict(params=ps[1:]))                  # a group without a record yet
+    calls.capturing = True
+    with pytest.raises(RuntimeError, match="one step\\(\\) or advance\\(\\) before the capture"):
+        opt.step()
+    assert len(calls) == 1

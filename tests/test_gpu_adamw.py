@@ -388,3 +388,42 @@ def test_record_of_another_device(dev):
     x = _lists(1, dev, [300])
     with pytest.raises(ValueError, match="record must be on the params' device"):
         adamw_(**x, **HYPER, record=torch.zeros(32, dtype=torch.uint8))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_captured_steps_with_a_param_left_out(bits, dev):
+    """Eager steps with a late gradient, then a graph that steps all params but one, replayed with advance(), then eager steps of all: the bits of
+    the optimizer without capturable."""
+    from timediff_amd.optim import AdamW
+    ps, qs = _params(dev), _params(dev)
+    a, b = AdamW(ps, state_bits=bits, seed=1), AdamW(qs, state_bits=bits, seed=1, capturable=True)
+
+    def feed(step, skip=()):
+        for i, (p, q) in enumerate(zip(ps, qs)):
+            g = _grads(step, i, p.shape).to(dev)
+            if i in skip:
+                p.grad = q.grad = None
+            else:
+                p.grad = g
+                q.grad = g.clone() if q.grad is None else q.grad.copy_(g)
+    for step in range(3):
+        feed(step, skip=(1,) if step < 2 else ())
+        a.step()
+        b.step()
+    feed(3, skip=(1,))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        b.step()
+    for step in range(3, 6):
+        feed(step, skip=(1,))
+        a.step()
+        b.advance()
+        graph.replay()
+        torch.cuda.synchronize()
+    for step in range(6, 8):
+        feed(step)
+        a.step()
+        b.step()
+    for p, q in zip(ps, qs):
+        assert torch.equal(p, q)
+        assert a.state[p]["step"] == b.state[q]["step"]

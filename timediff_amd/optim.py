@@ -5,6 +5,7 @@ costs 2 bytes of state instead of 8: exp_avg holds m and exp_avg_sq holds sqrt(v
 for each 256 values (a moment's value is code.float() * scale), rounded stochastically.  No counterpart in the reference.
 """
 import array
+import collections
 import ctypes as C
 import struct
 
@@ -86,8 +87,9 @@ _CONFIG = struct.Struct("<5dqQQQii")            # td_adamw_config
 class AdamW(torch.optim.Optimizer):
     """torch.optim.AdamW's formula and arguments on td_adamw; params float32, grads float32 or bfloat16.
     state_bits: 32 or 8 (state: exp_avg, exp_avg_sq[, scales], step).  seed: of the 8-bit moments' stochastic rounding.
-    capturable: step() may be captured in a graph.  A captured step() reads step count, learning rate, weight decay and seed from
-    device records; call advance() before each replay (an eager step() calls it itself)."""
+    capturable: step() may be captured in a graph, after one eager step() or advance().  A captured step() reads step count, learning
+    rate, weight decay and seed from device records, one for each group: the params of a group that it steps must be at the same step.  Call
+    advance() before each replay of the graph captured last, which may hold one step().  An eager step() is the same with and without it."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, state_bits=32, seed=0, capturable=False):
         if state_bits not in (32, 8):
@@ -95,7 +97,7 @@ class AdamW(torch.optim.Optimizer):
         if not (lr >= 0 and eps >= 0 and weight_decay >= 0 and 0 <= betas[0] < 1 and 0 <= betas[1] < 1):
             raise ValueError(f"bad lr {lr}, betas {betas}, eps {eps} or weight_decay {weight_decay}")
         self.state_bits, self.seed, self.capturable = state_bits, int(seed), bool(capturable)
-        self._records = {}
+        self._records, self._captured, self._ahead = {}, {}, {}
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
 
     def add_param_group(self, group):
@@ -121,24 +123,58 @@ class AdamW(torch.optim.Optimizer):
         return AdamwConfig(lr=float(g["lr"]), beta1=g["betas"][0], beta2=g["betas"][1], eps=g["eps"], weight_decay=g["weight_decay"], step=step,
                            seed=(self.seed + (i << 32)) & (2 ** 64 - 1), state_bits=self.state_bits)
 
+    def _record(self, i, step):
+        """Writes the device record of group i for a step."""
+        rec = self._records.get(i)
+        if rec is None:
+            rec = self._records[i] = torch.zeros(C.sizeof(AdamwRecord), dtype=torch.uint8, device=self.param_groups[i]["params"][0].device)
+        with ops._on_device(rec.get_device()):
+            check(lib().td_adamw_record_set(ptr(rec), C.byref(self._config(i, step)), ops._raw_stream(rec.get_device())))
+
+    def _one_step(self, i, params):
+        """The step that all of `params` are at."""
+        steps = {self._state(p)["step"] for p in params}
+        if len(steps) > 1:
+            raise RuntimeError(f"capturable: the params of a group that a captured step() steps must be at the same step, group {i} has {sorted(steps)}")
+        return steps.pop()
+
     def advance(self):
-        """capturable: counts one step and writes what changes with it (step count, lr, weight decay, seed) to the device records
-        that a captured step() reads."""
+        """capturable: counts one step of the params that the captured step() steps (before a capture: of those that have a gradient, or of
+        all where none has) and writes what changes with it (step count, lr, weight decay, seed) to the device records."""
         if not self.capturable:
             raise RuntimeError("advance() belongs to AdamW(capturable=True)")
+        todo = []
         for i, g in enumerate(self.param_groups):
             if not g["params"]:
                 continue
-            if i not in self._records:
-                self._records[i] = torch.zeros(C.sizeof(AdamwRecord), dtype=torch.uint8, device=g["params"][0].device)
-            states = [self._state(p) for p in g["params"]]
-            if len({s["step"] for s in states}) != 1:
-                raise RuntimeError("capturable: the params of a group must be at the same step")
-            for s in states:
-                s["step"] += 1
-            rec = self._records[i]
-            with torch.cuda.device(rec.device):
-                check(lib().td_adamw_record_set(ptr(rec), C.byref(self._config(i, states[0]["step"])), ops._stream()))
+            for p in g["params"]:
+                self._state(p)
+            params = self._captured.get(i)
+            if params is None:
+                params = [p for p in g["params"] if p.grad is not None] or g["params"]
+            if params:
+                todo.append((i, params, self._one_step(i, params) + 1))
+        for i, params, step in todo:
+            for p in params:
+                self.state[p]["step"] = step
+            if i not in self._captured:
+                self._ahead.setdefault(i, collections.Counter()).update(map(id, params))
+            self._record(i, step)
+
+    def _capture(self):
+        """What a captured step() steps from now on: for each group the params with a gradient, all at the same step."""
+        for i, g in enumerate(self.param_groups):
+            live = [p for p in g["params"] if p.grad is not None]
+            if live and (i not in self._records or any(not self.state[p] for p in live)):
+                raise RuntimeError("step() under graph capture needs AdamW(capturable=True) and one step() or advance() before the capture")
+            if live:
+                self._one_step(i, live)
+        for i, g in enumerate(self.param_groups):
+            self._captured[i] = [p for p in g["params"] if p.grad is not None]
+            for p in g["params"]:                # an advance() before this capture may have counted others
+                if p.grad is None and i in self._ahead:
+                    self.state[p]["step"] -= self._ahead[i][id(p)]
+        self._ahead = {}
 
     @torch.no_grad()
     def step(self, closure=None, *, grad_scale=None):
@@ -148,16 +184,18 @@ class AdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         capturing = torch.cuda.is_current_stream_capturing()
-        if capturing and (not self.capturable or not self._records):
+        if capturing and not self.capturable:
             raise RuntimeError("step() under graph capture needs AdamW(capturable=True) and one step() or advance() before the capture")
-        if self.capturable and not capturing:
-            self.advance()
+        if capturing:
+            self._capture()
+        else:
+            self._ahead = {}
         for i, group in enumerate(self.param_groups):
             live = [p for p in group["params"] if p.grad is not None]
             for p in live:
                 if p.grad.is_sparse:
                     raise RuntimeError("sparse gradients are not supported")
-            count = 0 if self.capturable else 1              # advance() has counted
+            count = 0 if capturing else 1                    # advance() counts a captured step
             at = {}
             for p in live:
                 at.setdefault(self._state(p)["step"] + count, []).append(p)
@@ -166,10 +204,12 @@ class AdamW(torch.optim.Optimizer):
                 cfg = self._config(i, step)
                 adamw_(ps, [p.grad.contiguous() for p in ps], [s["exp_avg"] for s in st], [s["exp_avg_sq"] for s in st],
                        [s["scales"] for s in st] if self.state_bits == 8 else None, lr=cfg.lr, betas=(cfg.beta1, cfg.beta2), eps=cfg.eps,
-                       weight_decay=cfg.weight_decay, step=step, grad_scale=grad_scale, seed=cfg.seed,
-                       record=self._records.get(i))
+                       weight_decay=cfg.weight_decay, step=max(step, 1), grad_scale=grad_scale, seed=cfg.seed,
+                       record=self._records[i] if capturing else None)
                 for s in st:
                     s["step"] = step
+            if self.capturable and not capturing and group["params"]:        # what a capture finds: it makes nothing of its own
+                self._record(i, max(1, *(self._state(p)["step"] for p in group["params"])))
         return loss
 
     def load_state_dict(self, state_dict):
