@@ -1,4 +1,8 @@
 """The AdamW optimizer's own bookkeeping without a GPU: the calls that reach the kernels are recorded in place of adamw_."""
+import copy
+import io
+import pickle
+
 import pytest
 import torch
 
@@ -117,3 +121,45 @@ def test_captures_that_are_refused(calls):
     with pytest.raises(RuntimeError, match="one step\\(\\) or advance\\(\\) before the capture"):
         opt.step()
     assert len(calls) == 1
+
+
+def _saved(opt):
+    f = io.BytesIO()
+    torch.save(opt, f)
+    return torch.load(io.BytesIO(f.getvalue()), weights_only=False)
+
+
+# (pickle alone does not take torch's float8 tensors)
+@pytest.mark.parametrize("bits, way", [(32, copy.deepcopy), (8, copy.deepcopy), (32, lambda o: pickle.loads(pickle.dumps(o))), (32, _saved), (8, _saved)])
+def test_copies_step(bits, way, calls):
+    ps = _params(2)
+    opt = AdamW([dict(params=ps[:1]), dict(params=ps[1:])], state_bits=bits, seed=7, capturable=True)
+    for p in ps:
+        p.grad = torch.zeros(4)
+    opt.step()
+    other = way(opt)
+    assert (other.state_bits, other.capturable) == (bits, True) and other.param_groups[0]["params"][0] is not ps[0]
+    for g in other.param_groups:
+        for p in g["params"]:
+            p.grad = torch.zeros(4)
+    opt.step()
+    other.step()
+    assert [c[1:] for c in calls[-2:]] == [c[1:] for c in calls[-4:-2]] == [(2, 7, False), (2, 7 + 2 ** 32, False)]
+    assert other._records.keys() == {0, 1} and other._records[0] is not opt._records[0]
+
+
+def test_seed_is_saved(calls):
+    """A resumed run rounds from the saved stream; a state saved without one keeps the optimizer's own."""
+    ps = _params(1)
+    opt = AdamW(ps, state_bits=8, seed=11)
+    ps[0].grad = torch.zeros(4)
+    opt.step()
+    again = AdamW(ps, state_bits=8)
+    again.load_state_dict(opt.state_dict())
+    again.step()
+    old = opt.state_dict()
+    old["param_groups"] = [{k: v for k, v in g.items() if k != "seed"} for g in old["param_groups"]]
+    third = AdamW(ps, state_bits=8, seed=5)
+    third.load_state_dict(old)
+    third.step()
+    assert [c[1:3] for c in calls] == [(1, 11), (2, 11), (2, 5)]

@@ -86,7 +86,8 @@ _CONFIG = struct.Struct("<5dqQQQii")            # td_adamw_config
 
 class AdamW(torch.optim.Optimizer):
     """torch.optim.AdamW's formula and arguments on td_adamw; params float32, grads float32 or bfloat16.
-    state_bits: 32 or 8 (state: exp_avg, exp_avg_sq[, scales], step).  seed: of the 8-bit moments' stochastic rounding.
+    state_bits: 32 or 8 (state: exp_avg, exp_avg_sq[, scales], step).  seed: of the 8-bit moments' stochastic rounding, saved with the groups' other
+    options.
     capturable: step() may be captured in a graph, after one eager step() or advance().  A captured step() reads step count, learning
     rate, weight decay and seed from device records, one for each group: the params of a group that it steps must be at the same step.  Call
     advance() before each replay of the graph captured last, which may hold one step().  An eager step() is the same with and without it."""
@@ -96,9 +97,17 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"state_bits must be 32 or 8, got {state_bits}")
         if not (lr >= 0 and eps >= 0 and weight_decay >= 0 and 0 <= betas[0] < 1 and 0 <= betas[1] < 1):
             raise ValueError(f"bad lr {lr}, betas {betas}, eps {eps} or weight_decay {weight_decay}")
-        self.state_bits, self.seed, self.capturable = state_bits, int(seed), bool(capturable)
+        self.state_bits, self.capturable = state_bits, bool(capturable)
         self._records, self._captured, self._ahead = {}, {}, {}
-        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+        # (the seed is a group's option, so that it is saved and loaded with the others)
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, seed=int(seed)))
+
+    def __getstate__(self):
+        return dict(super().__getstate__(), state_bits=self.state_bits, capturable=self.capturable)
+
+    def __setstate__(self, state):
+        # a copy has no graph: device records and what a captured step() steps stay with the original
+        super().__setstate__(dict(state, _records={}, _captured={}, _ahead={}))
 
     def add_param_group(self, group):
         super().add_param_group(group)
@@ -121,7 +130,7 @@ class AdamW(torch.optim.Optimizer):
         g = self.param_groups[i]
         # each group rounds from a stream of its own
         return AdamwConfig(lr=float(g["lr"]), beta1=g["betas"][0], beta2=g["betas"][1], eps=g["eps"], weight_decay=g["weight_decay"], step=step,
-                           seed=(self.seed + (i << 32)) & (2 ** 64 - 1), state_bits=self.state_bits)
+                           seed=(g["seed"] + (i << 32)) & (2 ** 64 - 1), state_bits=self.state_bits)
 
     def _record(self, i, step):
         """Writes the device record of group i for a step."""
@@ -217,6 +226,8 @@ class AdamW(torch.optim.Optimizer):
             if ("scales" in s) != (self.state_bits == 8):
                 raise ValueError(f"the state was saved with {8 if 'scales' in s else 32}-bit moments, this optimizer has state_bits={self.state_bits}")
         super().load_state_dict(state_dict)
+        for g in self.param_groups:
+            g.setdefault("seed", self.defaults["seed"])
         if self.state_bits == 8:          # torch casts a state to its param's type: float32 holds every e4m3 value, so the way back is exact
             for s in self.state.values():
                 s["exp_avg"], s["exp_avg_sq"] = s["exp_avg"].to(torch.float8_e4m3fn), s["exp_avg_sq"].to(torch.float8_e4m3fn)
