@@ -163,3 +163,22 @@ def test_seed_is_saved(calls):
     third.load_state_dict(old)
     third.step()
     assert [c[1:3] for c in calls] == [(1, 11), (2, 11), (2, 5)]
+
+
+def test_torchs_state_is_loaded(calls):
+    ps, theirs = _params(2), _params(2)
+    old = torch.optim.AdamW(theirs, lr=0.5)
+    for q in theirs:
+        q.grad = torch.ones(4)
+    old.step()
+    old.step()
+    opt = AdamW(ps)
+    opt.load_state_dict(old.state_dict())
+    for p, q in zip(ps, theirs):
+        p.grad = torch.ones(4)
+        assert torch.equal(opt.state[p]["exp_avg"], old.state[q]["exp_avg"]) and torch.equal(opt.state[p]["exp_avg_sq"], old.state[q]["exp_avg_sq"])
+    opt.step()
+    assert [c[1] for c in calls] == [3] and opt.param_groups[0]["lr"] == 0.5
+    for option in ("amsgrad", "maximize"):
+        with pytest.raises(ValueError, match=option):
+            AdamW(ps).load_state_dict(torch.optim.AdamW(theirs, **{option: True}).state_dict())

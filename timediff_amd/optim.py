@@ -85,7 +85,8 @@ _CONFIG = struct.Struct("<5dqQQQii")            # td_adamw_config
 
 
 class AdamW(torch.optim.Optimizer):
-    """torch.optim.AdamW's formula and arguments on td_adamw; params float32, grads float32 or bfloat16.
+    """torch.optim.AdamW's formula on td_adamw, of its arguments lr, betas, eps and weight_decay (no amsgrad or maximize); params float32, grads
+    float32 or bfloat16.  With 32 bits its state dicts are loaded too.
     state_bits: 32 or 8 (state: exp_avg, exp_avg_sq[, scales], step).  seed: of the 8-bit moments' stochastic rounding, saved with the groups' other
     options.
     capturable: step() may be captured in a graph, after one eager step() or advance().  A captured step() reads step count, learning
@@ -222,12 +223,18 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def load_state_dict(self, state_dict):
+        for g in state_dict["param_groups"]:
+            for option in ("amsgrad", "maximize"):
+                if g.get(option):
+                    raise ValueError(f"the state was saved with {option}, which this optimizer does not have")
         for s in state_dict["state"].values():
             if ("scales" in s) != (self.state_bits == 8):
                 raise ValueError(f"the state was saved with {8 if 'scales' in s else 32}-bit moments, this optimizer has state_bits={self.state_bits}")
         super().load_state_dict(state_dict)
         for g in self.param_groups:
             g.setdefault("seed", self.defaults["seed"])
+        for s in self.state.values():
+            s["step"] = int(s["step"])            # torch's own is a tensor
         if self.state_bits == 8:          # torch casts a state to its param's type: float32 holds every e4m3 value, so the way back is exact
             for s in self.state.values():
                 s["exp_avg"], s["exp_avg_sq"] = s["exp_avg"].to(torch.float8_e4m3fn), s["exp_avg_sq"].to(torch.float8_e4m3fn)
