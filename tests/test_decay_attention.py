@@ -144,3 +144,22 @@ def test_workspace_is_of_the_kernels_own_state(dk, dv, side):
     with_slope, without = (L.td_decay_workspace_bytes(C.byref(cfg), b) for b in (_lib.DECAY_GRAD_ALL, _lib.DECAY_GRAD_SOME))
     most = 32 if max(dk, dv) <= 32 else 64 if max(dk, dv) <= 64 else 128
     assert with_slope - without == most * most * 4 + 256
+
+
+@pytest.mark.parametrize("name", ["q", "k", "v", "log_decay", "initial_state"])
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_is_refused(name, grad):
+    """A dual tensor, whether it also takes a gradient or not: its tangent would be dropped.  Without one the call goes on (to the next refusal here)."""
+    import torch.autograd.forward_ad as fwd
+    a = dict(q=_x(2, 5, 2, 8), k=_x(2, 5, 2, 8), v=_x(2, 5, 4, 6), log_decay=_x(4), initial_state=_x(2, 4, 8, 6))
+    with fwd.dual_level():
+        with pytest.raises(ValueError, match="one ROCm device"):
+            _call(**a)
+        dual = fwd.make_dual(a[name].requires_grad_(grad), torch.ones_like(a[name]))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            _call(**dict(a, **{name: dual}))
+        b = dict(q=a["q"][:, 0], k=a["k"][:, 0], v=a["v"][:, 0], log_decay=a["log_decay"], state=a["initial_state"])
+        b = {n: t.detach() for n, t in b.items()}
+        n = "state" if name == "initial_state" else name
+        with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+            decay_attention_step(**dict(b, **{n: fwd.make_dual(b[n], torch.ones_like(b[n]))}))

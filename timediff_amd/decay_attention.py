@@ -6,6 +6,7 @@ Per sequence and head, with g = exp(log_decay):  S_t = g S_{t-1} + k_t v_t^T,  o
 No counterpart in the reference.
 """
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import ops
@@ -33,6 +34,12 @@ class _DecayFn(torch.autograd.Function):
         return (*grads, None, None, None)
 
 
+def _no_tangents(*tensors):
+    """Refuses forward-mode derivatives: the kernels would drop them."""
+    if getattr(forward_ad, "_current_level", 0) >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError("decay attention has no forward-mode derivatives")
+
+
 def _claim(node):
     """Marks the nodes that gather the leaves' gradients with the stream of their first graph.  Such a node lives as long as any graph of
     its leaf, and a backward pass waits for its stream: under capture that stream would have to be the captured one."""
@@ -51,11 +58,12 @@ def decay_attention(q, k, v, log_decay, *, scale=None, offsets=None, initial_sta
     offsets[i] .. offsets[i + 1] - 1 (it may be empty), and o is (R, H, Dv); rows of no sequence come back as zeros and take no
     gradient.  Their values are read on the device when the kernels run.
     initial_state: (B or N, H, Dk, Dv) float32.  return_state: -> (o, state after the last row, the same shape).
-    Differentiable once in q, k, v, log_decay and initial_state.  Any strides with a contiguous last dimension are read in place.
+    Differentiable once, in backward mode, in q, k, v, log_decay and initial_state.  Any strides with a contiguous last dimension are read in place.
     Rows are computed 64 at a time: a NaN or an infinity in a row's q, k or v may also reach the rows of its 64 before it, so rows that pad
     a dense batch should hold finite values (packed rows of other sequences and of none are never read).
     A captured backward pass needs leaves of which no graph made on another stream is alive: refused otherwise.
     """
+    _no_tangents(q, k, v, log_decay, initial_state)
     ops.decay_check(q, k, v, log_decay, offsets, initial_state)
     scale = float(q.shape[-1] ** -0.5 if scale is None else scale)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, log_decay, initial_state)):
@@ -71,4 +79,5 @@ def decay_attention_step(q, k, v, log_decay, state, *, scale=None):
     contiguous, is updated in place.  No gradient: under an enabled grad mode, inputs that require one are refused."""
     if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, log_decay, state)):
         raise RuntimeError("decay_attention_step has no gradient: call it under torch.no_grad(), or decay_attention with initial_state")
+    _no_tangents(q, k, v, log_decay, state)
     return ops.decay_step(q, k, v, log_decay, state, float(q.shape[-1] ** -0.5 if scale is None else scale))
