@@ -50,8 +50,7 @@ def test_more_workgroups_than_one_launch_takes(dev):
 
 @pytest.mark.parametrize("B, T, H", [(1, 70, 1), (3, 100, 2), (9, 300, 4)])
 def test_odd_addresses_with_even_strides(B, T, H, dev):
-    """Strides that suit 16-byte reads and addresses that do not: the backward pass takes a kernel with a wider state than the workspace counts a
-    place for, so fewer places (one at least).  The same results as from aligned tensors: sums of up to T D products in another order, 2^-24
+    """Strides that suit 16-byte reads and addresses that do not take another kernel.  The same results as from aligned tensors: sums of up to T D products in another order, 2^-24
     each of the sums of magnitudes on both sides, and a bfloat16 step where that crosses a border."""
     import decay_reference as ref
     from timediff_amd.decay_attention import decay_attention

@@ -264,19 +264,10 @@ int share_sum(const td_decay_config *c, const float *parts, void *grad, int own_
     return TD_OK;
 }
 
-// Floats of a chunk's state in the backward kernel that decay_inst.hip takes
-int64_t held_state(const td_decay_config *c, bool vec) {
-    const auto side = [](int d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; };
-    const int most = side(c->dk > c->dv ? c->dk : c->dv);
-    if (!vec || most < 128) return most * most;
-    return (c->dk <= 64 ? 64 : 128) * (c->dv <= 64 ? 64 : 128);
-}
-int64_t held_chunks(int len) { return (len + CHUNK - 1) / CHUNK; }
-
-// Whether the tensors can be read 16 bytes at a time if their addresses allow it (a configuration has none)
-bool wide_strides(const td_decay_config *c) {
-    return wide(c, view(c, nullptr, c->q_stride, c->q_heads, c->dk)) && wide(c, view(c, nullptr, c->k_stride, c->k_heads, c->dk)) &&
-           wide(c, view(c, nullptr, c->v_stride, c->v_heads, c->dv)) && wide(c, view(c, nullptr, c->grad_o_stride, c->heads, c->dv));
+// Floats of the states of a segment's chunks in the backward kernel that decay_inst.hip takes
+int64_t held_states(const td_decay_config *c, int len) {
+    const int most = c->dk > c->dv ? c->dk : c->dv, side = most <= 32 ? 32 : 64;
+    return (int64_t)(c->dk <= 64 ? side : 128) * (c->dv <= 64 ? side : 128) * ((len + CHUNK - 1) / CHUNK);
 }
 
 constexpr size_t NO_WORKSPACE = 256;      // what a call that uses none asks for: 0 says that the configuration is bad
@@ -288,13 +279,11 @@ Layout layout(const td_decay_config *c, int want) {
     int64_t slots;
     split(c, backward, len, segs, slots);
     const size_t state = (size_t)c->heads * c->dk * c->dv * sizeof(float), rows = (size_t)total_rows(c) * c->heads * sizeof(float);
-    // a place for each workgroup; one at least of the kernel that tensors at odd addresses take
-    const size_t place = held_chunks(len) * sizeof(float), places = backward_groups(c, slots) * held_state(c, wide_strides(c)) * place, one = held_state(c, false) * place;
     Layout w;
     w.seg = 0;
     w.seg2 = segs == 1 ? 0 : up256(slots * state);
     w.chunks = w.seg2 + (backward && segs != 1 ? up256(slots * state) : 0);
-    w.slope = w.chunks + (slope ? (places > one ? places : one) : 0);
+    w.slope = w.chunks + (slope ? held_states(c, len) * sizeof(float) * backward_groups(c, slots) : 0);
     w.parts = w.slope + (slope ? up256(2 * (size_t)slots * c->heads * sizeof(double)) : 0);
     const auto part = [&](int bit, int own, int d) { return backward && (all || want & bit) && own != c->heads ? up256(rows * d) : 0; };
     w.parts2 = w.parts + part(TD_DECAY_GRAD_Q, c->q_heads, c->dk);
@@ -360,10 +349,6 @@ extern "C" int td_decay_backward(const td_decay_config *cfg, const void *q, cons
     Pass &Q = w.p, &R = w.r;
     Q = R = base_pass(cfg, true, log_decay, offsets);
     w.groups = backward_groups(cfg, Q.slots);
-    if (slope) {          // tensors at odd addresses may take a wider kernel than the workspace was asked for: fewer workgroups, one item after another
-        const int64_t fit = (int64_t)(l.slope - l.chunks) / (held_state(cfg, vec) * held_chunks(Q.seg_len) * (int64_t)sizeof(float));
-        if (fit < w.groups) w.groups = (int)fit;
-    }
     double *slopes = (double *)(ws + l.slope);
     Q.a = vo; Q.b = vv; Q.c = vk; Q.e = vq;
     Q.da = cfg->dv; Q.dc = cfg->dk; Q.st_a = 1; Q.st_c = cfg->dv;

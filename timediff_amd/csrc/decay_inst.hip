@@ -46,24 +46,15 @@ template <bool VEC, int DA, int DC> int launch(const Work &w, hipStream_t st) {
 
 }  // namespace
 
-// Sizes, strides or addresses that are not multiples of 16 bytes have kernels of their own; their backward pass takes the square that holds them (41 x 101
-// and 101 x 41, 16 sequences of 1024 rows, 8 heads: 559 and 576 us bfloat16, 531 and 546 float32; rectangles 591, 605, 513, 677; forward,
-// bfloat16: 117 and 154 us in rectangles, 179 and 167 in squares).
+// Sizes, strides or addresses that are not multiples of 16 bytes have kernels of their own, of the same sizes (in the square that holds them
+// 41 x 101 and 101 x 41 take longer; 16 sequences of 1024 rows, 8 heads, in rectangles and in squares: backward, bfloat16 432 and 454 us, 602 and 621;
+// float32 452 and 593, 629 and 653; forward, bfloat16 114 and 156, 187 and 180; float32 132 and 143, 214 and 205).
 int TD_CAT(td_decay_launch_, TD_INST_BF16, TD_INST_KIND)(const Work &w, int vec, hipStream_t st) {
     const Pass &P = TD_INST_KIND < 3 ? w.p : w.r;          // backward: (da, dc) = (dk, dv)
     const int most = P.da > P.dc ? P.da : P.dc;
-    if (vec) {
-        if (most <= 32) return launch<true, 32, 32>(w, st);
-        if (most <= 64) return launch<true, 64, 64>(w, st);
-        if (P.da <= 64) return launch<true, 64, 128>(w, st);
-        if (P.dc <= 64) return launch<true, 128, 64>(w, st);
-        return launch<true, 128, 128>(w, st);
-    }
-    if (most <= 32) return launch<false, 32, 32>(w, st);
-    if (most <= 64) return launch<false, 64, 64>(w, st);
-#if TD_INST_KIND < 3
-    if (P.da <= 64) return launch<false, 64, 128>(w, st);
-    if (P.dc <= 64) return launch<false, 128, 64>(w, st);
-#endif
-    return launch<false, 128, 128>(w, st);
+    if (most <= 32) return vec ? launch<true, 32, 32>(w, st) : launch<false, 32, 32>(w, st);
+    if (most <= 64) return vec ? launch<true, 64, 64>(w, st) : launch<false, 64, 64>(w, st);
+    if (P.da <= 64) return vec ? launch<true, 64, 128>(w, st) : launch<false, 64, 128>(w, st);
+    if (P.dc <= 64) return vec ? launch<true, 128, 64>(w, st) : launch<false, 128, 64>(w, st);
+    return vec ? launch<true, 128, 128>(w, st) : launch<false, 128, 128>(w, st);
 }
