@@ -233,11 +233,12 @@ int launch(const td_decay_config *c, Kind kind, const Pass &P, bool vec, hipStre
 }
 
 // Workgroups of the backward pass, each with its own place for the states of a segment's chunks, one (slot, head) after another: as many as the
-// chip holds: two a compute unit, four of two waves each (states up to 32 x 32: 512 sequences of 272 rows, 8 heads: 390 us with
-// 512 workgroups, 258 with 1024).  Packed slots have different lengths, and workgroups that wait for a place on the chip even that
-// out (20011 rows of 40 sequences, 8 heads of 64 x 128: 296 us with 512, 270 with 1024).
+// chip holds, two a compute unit and, of bfloat16 states up to 32 x 32 (53 KB of LDS, two waves), three: 512 sequences of 272 rows, 8 heads,
+// bfloat16: 300 us with 768 workgroups, 435 with 512, 410 with 1024; float32 (57 KB): 613, 502, 503.  Packed slots have different
+// lengths, and workgroups that wait for a place on the chip even that out (20011 rows of 40 sequences, 8 heads of 64 x 128: 332 us
+// with 512, 322 with 1024).
 int backward_groups(const td_decay_config *c, int64_t slots) {
-    const int64_t most = c->packed || (c->dk <= 32 && c->dv <= 32) ? 1024 : 512;
+    const int64_t most = c->packed ? 1024 : c->dtype == TD_BF16 && c->dk <= 32 && c->dv <= 32 ? 768 : 512;
     return (int)(slots * c->heads < most ? slots * c->heads : most);
 }
 
