@@ -340,7 +340,7 @@ TD_API int td_cls_backward(const td_rnn_config *cfg, const void *packT, const fl
  * q, k and v may have fewer heads than log_decay (q_heads, k_heads, v_heads divide heads; head h reads head
  * h / (heads / q_heads), ...): their gradients are the sums over the heads that share them.
  * Types: q, k, v, o and their gradients TD_F32 or TD_BF16 (dtype); log_decay, states and their gradients float32.  The
- * recurrence is computed in float32: bf16 matrix products whose rounded operands are carried as two or three bf16 terms.
+ * recurrence is computed in float32: bf16 matrix products whose rounded operands are carried as three bf16 terms.
  * Limits: dk, dv <= TD_DECAY_MAX_DIM, rows <= 2^31 - 129.  log_decay is meant to be <= 0 (-inf: no memory); a positive one grows as the formula says.
  * ------------------------------------------------------------------------------------------ */
 enum { TD_F32 = 0, TD_BF16 = 1 };

@@ -91,7 +91,7 @@ __global__ __launch_bounds__(256) void td_decay_share_sum_kernel(const float *__
 
 // One row: a workgroup of NT threads for each state, W threads across its columns, the NT / W groups of them sharing out the rows.  Bound by memory:
 // the state is read and written once (1024 x 8 states of 128 x 128: 4.4 TB/s).  W: the least of 16, 32, 64 and 128 that has every column (with
-// 128 for all of them 2048 x 8 states of 64 x 64 take 172 us, with 64 125; 4096 x 8 of 32 x 32 float32 147 and 55).
+// 128 for all of them 2048 x 8 states of 64 x 64 take 165 us, with 64 126; 4096 x 8 of 32 x 32 float32 112 and 55).
 template <typename T, int W, int NT>
 __global__ __launch_bounds__(NT) void td_decay_step_kernel(Pass P) {
     constexpr int GROUPS = NT / W;
@@ -127,8 +127,8 @@ template <typename T, int NT> void launch_step(const Pass &P, hipStream_t st) {
         else hipLaunchKernelGGL((td_decay_step_kernel<T, 128, NT>), grid, block, 0, st, P);
     });
 }
-// Few states that are not small: 1024 threads for each, of which the chip holds 512 (64 x 8 states of 128 x 128: 14 us a call, 22 with 256 threads; 65 x 8
-// take 23 either way)
+// Few states that are not small: 1024 threads for each, of which the chip holds 512 (64 x 8 states of 128 x 128: 13 us a call, 19 with 256 threads; 65 x 8
+// take 22, with 256)
 template <typename T> void launch_step(const Pass &P, hipStream_t st) {
     if (P.n_seq * P.heads <= 512 && P.da * P.dc >= 4096) launch_step<T, 1024>(P, st);
     else launch_step<T, 256>(P, st);
@@ -173,12 +173,15 @@ bool wide(const td_decay_config *c, const View &v) {
 
 // Segments: a sequence on its own is one after another, chunk by chunk, so few long ones are cut until the chip is full, which costs two launches
 // and a second reading of k and v.  Measured (bfloat16, forward / backward):
-//   * rows of a segment: 256 at least, and nothing is cut up to 512 rows: the chip is full with 512 workgroups (two a compute unit), or with 256
-//     where one workgroup's registers fill a compute unit (backward of wide states); cut for 256 instead of 512 those backward passes
-//     take 309 instead of 343 us at 128 sequences and heads of 1024 rows, 128 x 128;
-//   * with a workgroup for three in four compute units nothing is cut: 256 of 1024 rows, 128 x 128, take 85 / 379 us whole and 146 / 590
-//     cut for 512.  States of 32 x 32 have less to do between their loads and gain up to 512: 256 of 2048 rows 77 / 207 us
-//     cut, about 95 / 276 whole.  Lengths of packed sequences are not known here: one of them may be nearly all rows;
+//   * rows of a segment: 256 at least: the chip is full with 512 workgroups (two a compute unit), or with 256 where one workgroup's registers fill
+//     a compute unit (backward of wide states): cut for 256 instead of 512 those backward passes take 357 instead of 379 us at 128
+//     sequences and heads of 1024 rows, 128 x 128;
+//   * nothing is cut up to 512 rows: 1, 4 and 8 sequences of 512 rows, 8 heads, 64 x 64, take 25, 25 and 26 us whole and 27, 28 and 30 cut in two
+//     forward (128 x 128: 47, 48 and 48; 46, 51 and 55).  Backward they would gain: 85, 87 and 87 whole, 76, 78 and 81 cut (128 x 128: 167, 175
+//     and 178; 140, 154 and 167);
+//   * with a workgroup for three in four compute units nothing is cut: 256 of 1024 rows, 128 x 128, take 100 us whole forward and 155 cut for 512.
+//     States of 32 x 32 have less to do between their loads and gain up to 512: 256 of 2048 rows 81 / 220 us cut, 91 / 264
+//     whole.  Lengths of packed sequences are not known here: one of them may be nearly all rows;
 //   * the backward pass of log_decay keeps the states entering a segment's chunks (64 KB a chunk of 128 x 128), so its segments are 4096
 //     rows at most: 2 GiB in 512 workgroups (4 in 1024), where a sequence of 32768 rows in one piece would take 16.
 void split(const td_decay_config *c, bool backward, int &len, int &segs, int64_t &slots) {

@@ -16,13 +16,15 @@ typedef float T;
 
 // A wave for each 16 columns of the output (backward: of the narrower of its two outputs); the bfloat16 forward pass of 128 x 128 takes 32 columns
 // a wave, so that two workgroups share a compute unit.  Backward passes of four waves of which a compute unit holds one workgroup take a second team of
-// four.  Waves a SIMD is to hold: what the registers of each size allow with few or no spills.  Measured with 16 sequences of 1024
-// rows, 8 heads, unless said otherwise:
-//   forward, bfloat16: 128 x 128 4 waves of 32 columns 171 us, 8 of 16 199 (cut into segments); 64 x 128 8 waves, 4 a SIMD 56, 4 waves 60;
-//   forward, float32 (LDS holds one workgroup): 128 x 128, 64 sequences, 8 waves 423 us, 4 waves 805;
-//   backward, bfloat16: 128 x 128 8 waves 350, 4 waves 402; 64 x 128 one team 180, two 162 (one team at two workgroups a compute unit,
-//   spilling, 268); 64 x 64, 2048 sequences of 272 rows: two workgroups of one team 1.02 ms, of two teams (spilling) 1.26, three of one (spilling) 1.92;
-//   backward, float32: 64 x 64 one team 203, two 193; 64 x 128 414 and 326.
+// four.  Waves a SIMD that a kernel is built for: four in the bfloat16 forward pass of 64 x 128, three in forward passes up to 64 x 64 (float32
+// reaches two), else two (float32 forward of 128 x 64, with one workgroup of four waves in LDS: one).  At two the backward passes of aligned tensors
+// with log_decay's gradient spill, of 128 x 128 201 registers (bfloat16) and 415 (float32), of float32 128 x 64 245, and so does that of float32
+// 128 x 128 with fixed decays, 127; the others spill 50 or fewer.  (Odd addresses: 141, 28, 120, 0.)  Measured with 16 sequences of 1024 rows, 8 heads, unless said otherwise:
+//   forward, bfloat16: 128 x 128 4 waves of 32 columns 95 us, 8 of 16 101; 64 x 128 8 waves, 4 a SIMD 59, 4 waves 61;
+//   forward, float32 (LDS holds one workgroup): 128 x 128, 64 sequences, 8 waves 412 us, 4 waves 807;
+//   backward, bfloat16 (learned / fixed decays): 128 x 128 8 waves 357 / 226, 4 waves 367 / 258; 64 x 128 two teams 168 / 158, one 191 / 177;
+//   64 x 64, 2048 sequences of 272 rows: two workgroups of one team 1.05 / 0.91 ms, of two teams 1.40 / 1.24, three of one 1.56 / 0.90;
+//   backward, float32: 64 x 64 two teams 194 / 180, one 201 / 191; 64 x 128 332 / 303 and 414 / 381.
 template <bool VEC, int DA, int DC> int launch(const Work &w, hipStream_t st) {
     constexpr int size = DA + DC, NW = TD_INST_KIND == 0 && TD_INST_BF16 && size == 256 ? 4 : (TD_INST_KIND < 3 ? DC : DA < DC ? DA : DC) / 16;
     const Pass &P = w.p;

@@ -41,8 +41,8 @@ def _no_tangents(*tensors):
 
 
 def _claim(node):
-    """Marks the nodes that gather the leaves' gradients with the stream of their first graph.  Such a node lives as long as any graph of
-    its leaf, and a backward pass waits for its stream: under capture that stream would have to be the captured one."""
+    """Marks the nodes that gather the leaves' gradients (in their metadata) with the stream of decay attention's first graph.  Such a node lives as
+    long as any graph of its leaf, and a backward pass waits for its stream: under capture that stream would have to be the captured one."""
     stream = torch.cuda.current_stream().cuda_stream
     for leaf, _ in node.next_functions:
         if hasattr(leaf, "variable") and leaf.metadata.setdefault("decay_attention stream", stream) != stream and torch.cuda.is_current_stream_capturing():
@@ -60,8 +60,10 @@ def decay_attention(q, k, v, log_decay, *, scale=None, offsets=None, initial_sta
     initial_state: (B or N, H, Dk, Dv) float32.  return_state: -> (o, state after the last row, the same shape).
     Differentiable once, in backward mode, in q, k, v, log_decay and initial_state.  Any strides with a contiguous last dimension are read in place.
     Rows are computed 64 at a time: a NaN or an infinity in a row's q, k or v may also reach the rows of its 64 before it, so rows that pad
-    a dense batch should hold finite values (packed rows of other sequences and of none are never read).
-    A captured backward pass needs leaves of which no graph made on another stream is alive: refused otherwise.
+    a dense batch should hold finite values (packed rows of other sequences and of none are never read).  An infinity, of the inputs or of a
+    state that overflowed, may come out as NaN.
+    A captured backward pass needs leaves of which no graph made on another stream is alive, as torch's own operators do: refused where
+    decay_attention made that graph (a graph of other operators alone is not seen here, and the capture fails in torch).
     """
     _no_tangents(q, k, v, log_decay, initial_state)
     ops.decay_check(q, k, v, log_decay, offsets, initial_state)
