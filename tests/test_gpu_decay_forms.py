@@ -119,3 +119,20 @@ def test_more_items_than_workgroups(Dk, Dv, dtype, learned, dev):
             _close(n, t[pick], want[n], size[n], T, max(Dk, Dv))
     if learned:                       # the sum is double: each part's rounding to float32, and its own
         assert ((got["grad log_decay"].double() - slope).abs() <= 2.0 ** -24 * (parts + slope.abs())).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("first, second", [("q", "k"), ("grad_o", "v")])
+@pytest.mark.parametrize("Dk, Dv, T, rows", [(16, 16, 5, (1, 3)), (64, 64, 64, (0, 63)), (64, 64, 100, (70, 71)), (64, 128, 64, (17, 18)), (64, 128, 40, (2, 39)), (128, 128, 90, (5, 60)),
+                                             (41, 101, 64, (30, 33))])
+def test_products_of_later_rows_overflow(Dk, Dv, T, rows, first, second, dtype, dev):
+    """Row a of one tensor and a later row b of its partner hold 2^70: their product overflows and belongs to no result, since b is behind a.  All
+    others are finite."""
+    x = _inputs(T, (2, T), 2, (2, 2, 2, 2), Dk, Dv, dtype)
+    a, b = rows
+    x[first][:, a, :, 0] = 2.0 ** 70
+    x[second][:, b, :, 0] = 2.0 ** 70
+    want, size = _reference(x)
+    for learned in (True, False):
+        for n, t in _run(x, dev, learned).items():
+            _close(n, t, want[n], size[n], T, max(Dk, Dv))

@@ -359,8 +359,11 @@ template <int NW> struct Weights {
         }
     }
     __device__ __forceinline__ int apart(int m, int r, int g, int li) const { return (it[m] - jt[m]) * 16 + li - (g * 4 + r); }
-    // wa of the n rows there are
-    template <typename R> __device__ __forceinline__ float score(int m, int r, int n, int li) const { return R::FULL || it[m] * 16 + li < n ? wa[m][r] : 0.0f; }
+    // Whether a pair of rows counts: not those above the diagonal or behind the n-th row, where a product of finite values may have overflowed
+    template <typename R> __device__ __forceinline__ bool pair(int m, int r, int n, int g, int li) const {
+        return apart(m, r, g, li) >= 0 && (R::FULL || it[m] * 16 + li < n);
+    }
+    template <typename R> __device__ __forceinline__ float weigh(float s, int m, int r, int n, int g, int li) const { return pair<R>(m, r, n, g, li) ? s * wa[m][r] : 0.0f; }
 };
 
 // Which of a chunk's four row tiles a wave's outputs have.  NI = 4: all of them.  NI = 2: two teams of waves hold the same state, team 0 has the
@@ -727,7 +730,7 @@ __device__ __forceinline__ void out_sweep(const Pass &P, int item, OutLds<T, DA,
             if (it >= R::LIVE) continue;
             f32x4 s = X::score(la, lb, it, jt, g, li);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) s[r] *= w.template score<R>(m, r, n, li);
+            for (int r = 0; r < 4; ++r) s[r] = w.template weigh<R>(s[r], m, r, n, g, li);
             X::keep(s, scores, it, jt, lane);
         }
         if (SLOPE && team == 0) {
@@ -849,12 +852,12 @@ __device__ __forceinline__ void pair_sweep(const Pass &P, int item, PairLds<T, D
                     if (it >= R::LIVE) continue;
                     f32x4 s = X::score(lx, ly, it, jt, g, li);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) s[r] *= w.template score<R>(m, r, n, li);
+                    for (int r = 0; r < 4; ++r) s[r] = w.template weigh<R>(s[r], m, r, n, g, li);
                     X::keep(s, scores, it, jt, lane);
                     if (SL) {
                         const f32x4 other = V::score(lk, lq, it, jt, g, li);
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) sum += (float)w.apart(m, r, g, li) * s[r] * other[r];
+                        for (int r = 0; r < 4; ++r) sum += w.template pair<R>(m, r, n, g, li) ? (float)w.apart(m, r, g, li) * s[r] * other[r] : 0.0f;
                     }
                 }
                 const int64_t row0 = (packed ? 0 : (int64_t)at.n_seq * P.rows) + at.lo + t;
@@ -921,10 +924,9 @@ __device__ __forceinline__ void pair_sweep(const Pass &P, int item, PairLds<T, D
                 f32x4 sv = V::score(lk, lq, it, jt, g, li), sk = K::score(lv, lo, it, jt, g, li);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const float weight = w.template score<R>(m, r, n, li);
-                    sv[r] *= weight;
-                    if (SLOPE) sum += (float)w.apart(m, r, g, li) * sv[r] * sk[r];
-                    sk[r] *= weight;
+                    sv[r] = w.template weigh<R>(sv[r], m, r, n, g, li);
+                    if (SLOPE) sum += w.template pair<R>(m, r, n, g, li) ? (float)w.apart(m, r, g, li) * sv[r] * sk[r] : 0.0f;
+                    sk[r] = w.template weigh<R>(sk[r], m, r, n, g, li);
                 }
                 V::keep(sv, scores_v, it, jt, lane);
                 K::keep(sk, scores_k, it, jt, lane);
