@@ -91,7 +91,7 @@ __global__ __launch_bounds__(256) void td_decay_share_sum_kernel(const float *__
 
 // One row: a workgroup of NT threads for each state, W threads across its columns, the NT / W groups of them sharing out the rows.  Bound by memory:
 // the state is read and written once (1024 x 8 states of 128 x 128: 4.4 TB/s).  W: the least of 16, 32, 64 and 128 that has every column (with
-// 128 for all of them 2048 x 8 states of 64 x 64 take 165 us, with 64 126; 4096 x 8 of 32 x 32 float32 112 and 55).
+// 128 for all of them 2048 x 8 states of 64 x 64 take 167 us, with 64 126; 4096 x 8 of 32 x 32 float32 112 and 55).
 template <typename T, int W, int NT>
 __global__ __launch_bounds__(NT) void td_decay_step_kernel(Pass P) {
     constexpr int GROUPS = NT / W;
@@ -127,7 +127,7 @@ template <typename T, int NT> void launch_step(const Pass &P, hipStream_t st) {
         else hipLaunchKernelGGL((td_decay_step_kernel<T, 128, NT>), grid, block, 0, st, P);
     });
 }
-// Few states that are not small: 1024 threads for each, of which the chip holds 512 (64 x 8 states of 128 x 128: 13 us a call, 19 with 256 threads; 65 x 8
+// Few states that are not small: 1024 threads for each, of which the chip holds 512 (64 x 8 states of 128 x 128: 14 us a call, 19 with 256 threads; 65 x 8
 // take 22, with 256)
 template <typename T> void launch_step(const Pass &P, hipStream_t st) {
     if (P.n_seq * P.heads <= 512 && P.da * P.dc >= 4096) launch_step<T, 1024>(P, st);
@@ -174,13 +174,13 @@ bool wide(const td_decay_config *c, const View &v) {
 // Segments: a sequence on its own is one after another, chunk by chunk, so few long ones are cut until the chip is full, which costs two launches
 // and a second reading of k and v.  Measured (bfloat16, forward / backward):
 //   * rows of a segment: 256 at least: the chip is full with 512 workgroups (two a compute unit), or with 256 where one workgroup's registers fill
-//     a compute unit (backward of wide states): cut for 256 instead of 512 those backward passes take 357 instead of 379 us at 128
+//     a compute unit (backward of wide states): cut for 256 instead of 512 those backward passes take 371 instead of 409 us at 128
 //     sequences and heads of 1024 rows, 128 x 128;
-//   * nothing is cut up to 512 rows: 1, 4 and 8 sequences of 512 rows, 8 heads, 64 x 64, take 25, 25 and 26 us whole and 27, 28 and 30 cut in two
-//     forward (128 x 128: 47, 48 and 48; 46, 51 and 55).  Backward they would gain: 85, 87 and 87 whole, 76, 78 and 81 cut (128 x 128: 167, 175
-//     and 178; 140, 154 and 167);
-//   * with a workgroup for three in four compute units nothing is cut: 256 of 1024 rows, 128 x 128, take 100 us whole forward and 155 cut for 512.
-//     States of 32 x 32 have less to do between their loads and gain up to 512: 256 of 2048 rows 81 / 220 us cut, 91 / 264
+//   * nothing is cut up to 512 rows: 1, 4 and 8 sequences of 512 rows, 8 heads, 64 x 64, take 25, 26 and 26 us whole and 27, 29 and 30 cut in two
+//     forward (128 x 128: 47, 48 and 48; 46, 51 and 55).  Backward they would gain: 87, 88 and 88 whole, 77, 79 and 83 cut (128 x 128: 164, 173
+//     and 177; 138, 152 and 166);
+//   * with a workgroup for three in four compute units nothing is cut: 256 of 1024 rows, 128 x 128, take 103 us whole forward and 155 cut for 512.
+//     States of 32 x 32 have less to do between their loads and gain up to 512: 256 of 2048 rows 84 / 233 us cut, 95 / 282
 //     whole.  Lengths of packed sequences are not known here: one of them may be nearly all rows;
 //   * the backward pass of log_decay keeps the states entering a segment's chunks (64 KB a chunk of 128 x 128), so its segments are 4096
 //     rows at most: 2 GiB in 512 workgroups (4 in 1024), where a sequence of 32768 rows in one piece would take 16.
@@ -237,9 +237,9 @@ int launch(const td_decay_config *c, Kind kind, const Pass &P, bool vec, hipStre
 
 // Workgroups of the backward pass, each with its own place for the states of a segment's chunks, one (slot, head) after another: as many as the
 // chip holds, two a compute unit and, of bfloat16 states up to 32 x 32 (53 KB of LDS, two waves), three: 512 sequences of 272 rows, 8 heads,
-// bfloat16: 300 us with 768 workgroups, 435 with 512, 410 with 1024; float32 (57 KB): 613, 502, 503.  Packed slots have different
-// lengths, and workgroups that wait for a place on the chip even that out (20011 rows of 40 sequences, 8 heads of 64 x 128: 332 us
-// with 512, 322 with 1024).
+// bfloat16: 319 us with 768 workgroups, 466 with 512, 440 with 1024; float32 (57 KB): 636, 517, 519.  Packed slots have different
+// lengths, and workgroups that wait for a place on the chip even that out (20011 rows of 40 sequences, 8 heads of 64 x 128: 336 us
+// with 512, 326 with 1024).
 int backward_groups(const td_decay_config *c, int64_t slots) {
     const int64_t most = c->packed ? 1024 : c->dtype == TD_BF16 && c->dk <= 32 && c->dv <= 32 ? 768 : 512;
     return (int)(slots * c->heads < most ? slots * c->heads : most);
