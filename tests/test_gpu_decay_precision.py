@@ -128,3 +128,19 @@ def test_growing_states_of_short_sequences(T, log_decay, D, dtype, dev):
         assert torch.isfinite(d).all(), n
         room = ((4 if n == "log_decay" else 1) * T + 2 * D + 32) * 2.0 ** -24 * size[n] + (2.0 ** -8 if dtype is BF16 and n in "qkv" else 2.0 ** -24) * want[n].abs()
         assert ((d - want[n]).abs() <= room).all(), n
+
+
+def test_states_of_long_sequences(dev):
+    """float32 states of 16384 rows in one piece, with positive inputs and hardly any decay, so that they grow evenly: every chunk of 64 rows
+    rounds them three times (the decay and two sums of 32 rows), by 2^-24 at most and in independent directions.  The state at a rounding is t / T of the
+    last, so the norm of what they leave is at most sqrt(3 x 256 / 3) 2^-24 of the state's."""
+    from timediff_amd.decay_attention import decay_attention
+    B, T, D = 192, 16384, 40
+    g = torch.Generator(device=dev).manual_seed(2)
+    q, k, v = (torch.rand(B, T, 1, D, generator=g, device=dev) for _ in range(3))
+    ld = torch.tensor([-1e-6], device=dev)
+    _, s = decay_attention(q, k, v, ld, return_state=True)
+    w = torch.exp(ld.double() * torch.arange(T - 1, -1, -1, device=dev))[:, None]
+    for b in (0, 1, 100, 191):
+        exact = (k[b, :, 0].double() * w).t() @ v[b, :, 0].double()
+        assert (s[b, 0].double() - exact).norm() <= 16 * 2.0 ** -24 * exact.norm(), b
