@@ -216,8 +216,8 @@ typedef Rows<CHUNK / 32, false> Half;
 // One chunk's rows of one tensor on their way from memory to LDS.  Memory is read in the order of its rows (n of them from `low` on), a
 // reversed pass turns them round in LDS.  The loads go into registers while the chunk before is computed (unless there are too many of them:
 // 64 bytes of each tensor a thread; 4 bytes at a time in workgroups of 512 threads, whose registers four tensors would fill, 32: 101 x 101 float32,
-// 16 sequences of 1024 rows, 8 heads: 748 us backward, 926 with 64.  Rectangles, two of whose tensors take 32 anyway, would gain with 64:
-// 41 x 101 452 and 382, 101 x 41 600 and 543).
+// 16 sequences of 1024 rows, 8 heads: 852 us backward, 1032 with 64.  Rectangles, two of whose tensors take 32 anyway, would gain with 64:
+// 41 x 101 458 and 381, 101 x 41 589 and 581).
 // WIDE: 16 bytes each, at 32-bit offsets from the chunk's first row; else (odd sizes, strides or addresses) 4 bytes each.  They are never
 // skipped, so that their registers have one writer: a lane without a row or a column of its own reads its neighbours', and
 // nothing of that is stored.

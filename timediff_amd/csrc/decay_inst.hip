@@ -18,14 +18,14 @@ typedef float T;
 // a wave, so that two workgroups share a compute unit.  Backward passes of four waves of which a compute unit holds one workgroup take a second team of
 // four.  Waves a SIMD that a kernel is built for: four in the bfloat16 forward pass of 64 x 128, three in forward passes up to 64 x 64 (float32
 // reaches two), else two (float32 forward of 128 x 64, with one workgroup of four waves in LDS: one).  At two the backward passes of aligned tensors
-// with log_decay's gradient spill, of 128 x 128 199 registers (bfloat16) and 415 (float32), of float32 128 x 64 245, and so does that of float32
-// 128 x 128 with fixed decays, 127; the others spill 50 or fewer.  (Odd addresses: 134, 28, 108, 0.)  Measured with 16 sequences of 1024
+// with log_decay's gradient spill, of 128 x 128 199 registers (bfloat16) and 475 (float32), of float32 128 x 64 253, and so does that of float32
+// 128 x 128 with fixed decays, 179; the others spill 50 or fewer.  (Odd addresses: 134, 143, 131, 18.)  Measured with 16 sequences of 1024
 // rows, 8 heads, unless said otherwise:
-//   forward, bfloat16: 128 x 128 4 waves of 32 columns 95 us, 8 of 16 101; 64 x 128 8 waves, 4 a SIMD 59, 4 waves 61;
-//   forward, float32 (LDS holds one workgroup): 128 x 128, 64 sequences, 8 waves 413 us, 4 waves 807;
-//   backward, bfloat16 (learned / fixed decays): 128 x 128 8 waves 371 / 225, 4 waves 367 / 259; 64 x 128 two teams 169 / 158, one 192 / 179;
-//   64 x 64, 2048 sequences of 272 rows: two workgroups of one team 1.07 / 0.93 ms, of two teams 1.42 / 1.26, three of one 1.59 / 0.90;
-//   backward, float32: 64 x 64 two teams 197 / 181, one 202 / 191; 64 x 128 333 / 304 and 414 / 383.
+//   forward, bfloat16: 128 x 128 4 waves of 32 columns 95 us, 8 of 16 102; 64 x 128 8 waves, 4 a SIMD 59, 4 waves 61;
+//   forward, float32 (LDS holds one workgroup): 128 x 128, 64 sequences, 8 waves 418 us, 4 waves 824;
+//   backward, bfloat16 (learned / fixed decays): 128 x 128 8 waves 370 / 226, 4 waves 368 / 259; 64 x 128 two teams 170 / 159, one 193 / 180;
+//   64 x 64, 2048 sequences of 272 rows: two workgroups of one team 1.07 / 0.94 ms, of two teams 1.43 / 1.27, three of one 1.60 / 0.92;
+//   backward, float32: 64 x 64 two teams 197 / 180, one 202 / 190; 64 x 128 335 / 310 and 419 / 386.
 template <bool VEC, int DA, int DC> int launch(const Work &w, hipStream_t st) {
     constexpr int size = DA + DC, NW = TD_INST_KIND == 0 && TD_INST_BF16 && size == 256 ? 4 : (TD_INST_KIND < 3 ? DC : DA < DC ? DA : DC) / 16;
     const Pass &P = w.p;
@@ -50,8 +50,8 @@ template <bool VEC, int DA, int DC> int launch(const Work &w, hipStream_t st) {
 }  // namespace
 
 // Sizes, strides or addresses that are not multiples of 16 bytes have kernels of their own, of the same sizes (in the square that holds them
-// 41 x 101 and 101 x 41 take longer; 16 sequences of 1024 rows, 8 heads, in rectangles and in squares: backward, bfloat16 430 and 458 us, 615 and 637;
-// float32 452 and 600, 663 and 688; forward, bfloat16 113 and 156, 188 and 183; float32 134 and 144, 188 and 179).
+// 41 x 101 and 101 x 41 take longer; 16 sequences of 1024 rows, 8 heads, in rectangles and in squares: backward, bfloat16 432 and 458 us, 616 and 639;
+// float32 458 and 589, 769 and 790; forward, bfloat16 114 and 156, 188 and 183; float32 134 and 146, 189 and 180).
 int TD_CAT(td_decay_launch_, TD_INST_BF16, TD_INST_KIND)(const Work &w, int vec, hipStream_t st) {
     const Pass &P = TD_INST_KIND < 3 ? w.p : w.r;          // backward: (da, dc) = (dk, dv)
     const int most = P.da > P.dc ? P.da : P.dc;
