@@ -237,9 +237,9 @@ int launch(const td_decay_config *c, Kind kind, const Pass &P, bool vec, hipStre
 
 // Workgroups of the backward pass, each with its own place for the states of a segment's chunks, one (slot, head) after another: as many as the
 // chip holds, two a compute unit and, of bfloat16 states up to 32 x 32 (53 KB of LDS, two waves), three: 512 sequences of 272 rows, 8 heads,
-// bfloat16: 319 us with 768 workgroups, 466 with 512, 440 with 1024; float32 (57 KB): 636, 517, 519 (before its states summed 32 rows first: 525 now).  Packed slots have different
-// lengths, and workgroups that wait for a place on the chip even that out (20011 rows of 40 sequences, 8 heads of 64 x 128: 336 us
-// with 512, 326 with 1024).
+// bfloat16: 319 us with 768 workgroups, 466 with 512, 440 with 1024; float32 (57 KB): 636, 517, 519 (before its states summed 32 rows first: with
+// 512 524 now).  Packed slots have different lengths, and workgroups that wait for a place on the chip even that out (20011 rows of 40
+// sequences, 8 heads of 64 x 128: 336 us with 512, 326 with 1024).
 int backward_groups(const td_decay_config *c, int64_t slots) {
     const int64_t most = c->packed ? 1024 : c->dtype == TD_BF16 && c->dk <= 32 && c->dv <= 32 ? 768 : 512;
     return (int)(slots * c->heads < most ? slots * c->heads : most);

@@ -91,7 +91,8 @@ class AdamW(torch.optim.Optimizer):
     options.
     capturable: step() may be captured in a graph, after one eager step() or advance().  A captured step() reads step count, learning
     rate, weight decay and seed from device records, one for each group: the params of a group that it steps must be at the same step.  Call
-    advance() before each replay of the graph captured last, which may hold one step().  An eager step() is the same with and without it."""
+    advance() before each replay of the graph captured last, which may hold one step().  An eager step() is the same with and without it.
+    load_state_dict() makes new state tensors and records, which no earlier graph knows: capture again after it."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, state_bits=32, seed=0, capturable=False):
         if state_bits not in (32, 8):
